@@ -123,8 +123,8 @@ typedef struct {
  * communicator (if one is bound). */
 int o64_create(o64_handle_t *out, int device);
 int o64_destroy(o64_handle_t h);
-/* Synchronises `stream`, reads and clears the device status word: O64_OK or
- * O64_ERR_TIMEOUT.  `detail`, if not NULL, receives the raw word (which wait gave up). */
+/* Synchronises `stream`, reads and clears the device status word: O64_OK, O64_ERR_TIMEOUT, or
+ * O64_ERR_CONFORM where a grouped product met offsets that do not ascend within its rows.  `detail`, if not NULL, receives the raw word (which wait gave up). */
 int o64_last_status(o64_handle_t h, void *stream, int *detail);
 /* Budget of the kernels' bounded device-side waits for later calls on this handle, in microseconds
  * (0 = the default, two seconds; the environment variable O64_WAIT_BUDGET_US sets the default of new
@@ -214,13 +214,88 @@ int o64_gemm_fp8_scaled_kn(o64_handle_t h, int64_t M, int64_t N, int64_t K, cons
  * has a relative in the reference's MATMUL of INTEGER*1 arrays, which returns INTEGER*1
  * (osprey/crayf90/fe90/intrin.h:4294, osprey/libfi/matrix/i1gemmx.f) - there by wrap-around, here by
  * scaling and saturation; the elementwise vocabulary is the one of O64_ACT_*. */
-enum { O64_OUT_BF16 = 0, O64_OUT_S8 = 1, O64_OUT_E4M3 = 2 };
+enum { O64_OUT_BF16 = 0, O64_OUT_S8 = 1, O64_OUT_E4M3 = 2, O64_OUT_F32 = 3 };
 int o64_gemm_fp8_scaled_ex(o64_handle_t h, int64_t M, int64_t N, int64_t K, const void *A8, int64_t lda,
                            const void *B8, int64_t ldb, const float *scaleA, const float *scaleB,
                            const float *bias, int act, void *C, int64_t ldc, int out_kind, void *stream);
 int o64_gemm_s8_scaled(o64_handle_t h, int64_t M, int64_t N, int64_t K, const int8_t *A, int64_t lda,
                        const int8_t *B, int64_t ldb, const float *scaleA, const float *scaleB,
                        const float *bias, int act, void *C, int64_t ldc, int out_kind, void *stream);
+
+/* ---- around the products of a feed-forward layer ----------------------------------------
+ * Operators the reference's element types and loop nests do not know: they take device pointers only
+ * (O64_ERR_RANK for host memory or another GPU's), allocate nothing, use no scratch of the handle and
+ * may be captured into a CUDA graph; two calls on different streams of one handle do not touch each
+ * other's memory.  Operands whose base or pitch is not a multiple of 16 bytes are O64_ERR_ALIGN where
+ * a product says so. */
+
+/* RMS norm with the residual's addition, rows of N columns (1 <= N <= 32768):
+ *   s = x + r      h[j] = s[j] / sqrt(mean(s^2) + eps) * w[j]
+ * X, R, S, Y [T,N] row-major; X, R and S bf16; R NULL: s = x; S NULL: the sum is not stored (S may be X
+ * or R itself).  s is rounded to bf16 for S only: the norm is taken of the fp32 sum.  W: N values, bf16
+ * or, with w_f32 != 0, fp32.  out_kind O64_OUT_BF16, or O64_OUT_E4M3 with
+ *   scale = max |h| over a block / 448 (1 where that is no normal number), q = e4m3(h / scale)
+ * where scale_block = 128 makes blocks of 128 columns, scales [T][ceil(N/128)] with ldscales floats
+ * between rows (what the block-scaled products read), and scale_block = 0 one block per row, scales[T]
+ * at a distance of ldscales (scaleA of o64_gemm_fp8_scaled with ldscales = 1).  A NaN makes its block's
+ * scale NaN.  rstd (may be NULL): 1 / sqrt(mean(s^2) + eps) for each row, for the backward pass. */
+int o64_rmsnorm_bf16(o64_handle_t h, int64_t T, int64_t N, const void *X, int64_t ldx, const void *R, int64_t ldr,
+                     void *S, int64_t lds, const void *W, int w_f32, float eps, int out_kind, int scale_block, void *Y,
+                     int64_t ldy, float *scales, int64_t ldscales, float *rstd, void *stream);
+
+/* Its gradient: with n = s * rstd and g = dy * w,
+ *   dx = rstd * (g - n * mean(g * n)) + dr        dw[j] = sum over rows of dy[j] * n[j]
+ * dx is the gradient of x and of the residual.  dY, S, dR, dX [T,N] bf16 (dX may be dY or dR), rstd
+ * [T]; dR NULL: nothing arrives on the stream's other path; dW (fp32, N values) NULL: not wanted.
+ * workspace: device memory of at least o64_rmsnorm_bf16_backward_workspace(T, N) bytes when dW is
+ * wanted.  dw is added in a fixed order: the same call gives the same bits. */
+size_t o64_rmsnorm_bf16_backward_workspace(int64_t T, int64_t N);
+int o64_rmsnorm_bf16_backward(o64_handle_t h, int64_t T, int64_t N, const void *dY, int64_t lddy, const void *S, int64_t lds,
+                              const void *W, int w_f32, const float *rstd, const void *dR, int64_t lddr, void *dX,
+                              int64_t lddx, float *dW, void *workspace, void *stream);
+
+/* e4m3 product with a scale for each block of 128:
+ *   C[m,n] = bf16( sum over blocks b of K: scaleA[m,b] * scaleB[n/128,b] * (sum of A8 B8 over block b) )
+ * A8 [M,K], scaleA [M][ceil(K/128)] (ldsa floats between rows).  transB != 0: B8 [N,K], scaleB
+ * [ceil(N/128)][ceil(K/128)]; transB == 0: B8 [K,N], scaleB [ceil(K/128)][ceil(N/128)] - a weight [N,K]
+ * passed this way (its N the sum's index) gives the gradient of the product's input.  Sums inside a
+ * block and over blocks are fp32.  Bases and pitches of A8 and B8: multiples of 16 bytes. */
+int o64_gemm_fp8_block(o64_handle_t h, int64_t M, int64_t N, int64_t K, const void *A8, int64_t lda, const float *scaleA,
+                       int64_t ldsa, const void *B8, int64_t ldb, int transB, const float *scaleB, int64_t ldsb, void *C,
+                       int64_t ldc, void *stream);
+
+/* H = silu(gate) * up of the two halves of one product of that kind: B8 [2N,K] (gate rows 0 .. N-1, up
+ * rows N .. 2N-1; N a multiple of 128), scaleB [2N/128][ceil(K/128)].  H [M,N] bf16, or O64_OUT_E4M3 with
+ * scaleH [M][N/128] (ldsh floats between rows) made as in o64_rmsnorm_bf16: the operand of the next
+ * block-scaled product. */
+int o64_gemm_fp8_block_swiglu(o64_handle_t h, int64_t M, int64_t N, int64_t K, const void *A8, int64_t lda, const float *scaleA,
+                              int64_t ldsa, const void *B8, int64_t ldb, const float *scaleB, int64_t ldsb, void *H, int64_t ldh,
+                              int out_kind, float *scaleH, int64_t ldsh, void *stream);
+
+/* Products grouped by expert.  The T rows of A are sorted by group; offsets (device memory, G + 1 ints,
+ * ascending within 0 .. T) bound them: group g has rows offsets[g] .. offsets[g+1]-1, possibly none.
+ * Group g multiplies B + g * stride_b ([N,K], or [K,N] with transB == 0).  Rows of C before offsets[0]
+ * and from offsets[G] on are left as they are.  Offsets that are not ascending within 0 .. T are never
+ * followed out of the operands; the rows concerned are undefined and o64_last_status reports
+ * O64_ERR_CONFORM.  Scales of the e4m3 forms as above, stride_sb floats between the groups' scales of B.
+ * Bases, pitches and strides of A and B: multiples of 16 bytes. */
+int o64_gemm_grouped_bf16(o64_handle_t h, int64_t G, int64_t T, int64_t N, int64_t K, const void *A, int64_t lda,
+                          const int32_t *offsets, const void *B, int64_t ldb, int64_t stride_b, int transB, void *C, int64_t ldc,
+                          void *stream);
+int o64_gemm_grouped_fp8_block(o64_handle_t h, int64_t G, int64_t T, int64_t N, int64_t K, const void *A8, int64_t lda,
+                               const float *scaleA, int64_t ldsa, const int32_t *offsets, const void *B8, int64_t ldb,
+                               int64_t stride_b, int transB, const float *scaleB, int64_t ldsb, int64_t stride_sb, void *C,
+                               int64_t ldc, void *stream);
+int o64_gemm_grouped_fp8_block_swiglu(o64_handle_t h, int64_t G, int64_t T, int64_t N, int64_t K, const void *A8, int64_t lda,
+                                      const float *scaleA, int64_t ldsa, const int32_t *offsets, const void *B8, int64_t ldb,
+                                      int64_t stride_b, const float *scaleB, int64_t ldsb, int64_t stride_sb, void *H,
+                                      int64_t ldh, int out_kind, float *scaleH, int64_t ldsh, void *stream);
+/* Gradient of the weights of o64_gemm_grouped_bf16 (transB != 0): dB[g] = dC[rows of g]^T * A[rows of g],
+ * dC [T,N] and A [T,K] bf16, dB [N,K] per group, stride_db elements apart, O64_OUT_BF16 or O64_OUT_F32; zero
+ * for a group without rows.  (The gradient of A is o64_gemm_grouped_bf16 itself on dC with transB == 0.) */
+int o64_gemm_grouped_bf16_wgrad(o64_handle_t h, int64_t G, int64_t T, int64_t N, int64_t K, const void *dC, int64_t lddc,
+                                const void *A, int64_t lda, const int32_t *offsets, void *dB, int64_t lddb, int64_t stride_db,
+                                int out_kind, void *stream);
 
 /* C = A*B^T: int8 operands, A [M,K], B [N,K], int32 accumulate and result, exact.  The
  * reference's integer kernels are instances of the same template

@@ -15,7 +15,7 @@ ERR_RANK, ERR_CONFORM, ERR_NOMEM, ERR_ALIGN, ERR_DTYPE, ERR_TIMEOUT, ERR_CUDA, E
 ACT_NONE, ACT_RELU, ACT_GELU_TANH, ACT_GELU_ERF, ACT_SILU = range(5)
 KIND_F32, KIND_BF16, KIND_FP8, KIND_S8 = range(4)
 GATHER_NONE, GATHER_ROWMAJOR, GATHER_SLABS, GATHER_PUSH = range(4)
-OUT_BF16, OUT_S8, OUT_E4M3 = range(3)
+OUT_BF16, OUT_S8, OUT_E4M3, OUT_F32 = range(4)
 UNIQUE_ID_BYTES = 128
 STATIC_SCRATCH_BYTES = 16 << 20
 
@@ -25,6 +25,8 @@ EXPORTS = [
     "o64_plan_get", "o64_plan_set", "o64_plan_model", "o64_plan_tune", "o64_plan_tune_clear", "o64_plan_save", "o64_plan_load", "o64_plan_count", "o64_linear_f32", "o64_gemm_bf16", "o64_gemm_bf16_swiglu",
     "o64_gemm_fp8_scaled", "o64_gemm_fp8_scaled_ex", "o64_gemm_fp8_scaled_kn", "o64_gemm_s8_scaled", "o64_gemm_s8s8_s32", "o64_gemm_s8s8_s32_static", "o64_naive_gemm", "o64_comm_unique_id",
     "o64_comm_init", "o64_comm_destroy", "o64_comm_alloc_result", "o64_gemm_s8_sharded_workspace", "o64_gemm_s8_sharded", "o64_gemm_bf16_sharded",
+    "o64_rmsnorm_bf16", "o64_rmsnorm_bf16_backward", "o64_rmsnorm_bf16_backward_workspace", "o64_gemm_fp8_block", "o64_gemm_fp8_block_swiglu",
+    "o64_gemm_grouped_bf16", "o64_gemm_grouped_fp8_block", "o64_gemm_grouped_fp8_block_swiglu", "o64_gemm_grouped_bf16_wgrad",
     "sgemm_", "_s4gemmx__", "_s4gemvx__", "_MATMUL_S4S4", "o64_compat_last_status", "o64_compat_handle",
     "dgemm_", "_sgemmx__", "_sgemvx__", "_MATMUL_SS",
     "_i1gemmx__", "_i1i2gemmx__", "_i1i4gemmx__", "_i1jgemmx__", "_i2gemmx__", "_i2i4gemmx__", "_i2jgemmx__",
@@ -179,6 +181,16 @@ def lib():
     L.o64_gemm_s8_sharded_workspace.restype = ctypes.c_size_t
     L.o64_gemm_s8_sharded.argtypes = [vp, i64, i64, i64, vp, i64, vp, i64, vp, ci, vp, vp]
     L.o64_gemm_bf16_sharded.argtypes = [vp, i64, i64, i64, vp, i64, vp, i64, vp, ci, ctypes.POINTER(Epilogue), vp]
+    L.o64_rmsnorm_bf16.argtypes = [vp, i64, i64, vp, i64, vp, i64, vp, i64, vp, ci, cf, ci, ci, vp, i64, vp, i64, vp, vp]
+    L.o64_rmsnorm_bf16_backward_workspace.argtypes = [i64, i64]
+    L.o64_rmsnorm_bf16_backward_workspace.restype = ctypes.c_size_t
+    L.o64_rmsnorm_bf16_backward.argtypes = [vp, i64, i64, vp, i64, vp, i64, vp, ci, vp, vp, i64, vp, i64, vp, vp, vp]
+    L.o64_gemm_fp8_block.argtypes = [vp, i64, i64, i64, vp, i64, vp, i64, vp, i64, ci, vp, i64, vp, i64, vp]
+    L.o64_gemm_fp8_block_swiglu.argtypes = [vp, i64, i64, i64, vp, i64, vp, i64, vp, i64, vp, i64, vp, i64, ci, vp, i64, vp]
+    L.o64_gemm_grouped_bf16.argtypes = [vp, i64, i64, i64, i64, vp, i64, vp, vp, i64, i64, ci, vp, i64, vp]
+    L.o64_gemm_grouped_fp8_block.argtypes = [vp, i64, i64, i64, i64, vp, i64, vp, i64, vp, vp, i64, i64, ci, vp, i64, i64, vp, i64, vp]
+    L.o64_gemm_grouped_fp8_block_swiglu.argtypes = [vp, i64, i64, i64, i64, vp, i64, vp, i64, vp, vp, i64, i64, vp, i64, i64, vp, i64, ci, vp, i64, vp]
+    L.o64_gemm_grouped_bf16_wgrad.argtypes = [vp, i64, i64, i64, i64, vp, i64, vp, i64, vp, vp, i64, i64, ci, vp]
     L.sgemm_.argtypes = [ctypes.c_char_p, ctypes.c_char_p, pi, pi, pi, pf, vp, pi, vp, pi, pf, vp, pi]
     L.sgemm_.restype = None
     L._s4gemmx__.argtypes = [pi, pi, pi, pf, vp, pi, pi, vp, pi, pi, pf, vp, pi, pi]

@@ -19,6 +19,8 @@
 #include <vector>
 
 #include "../../include/o64gemm.h"
+#include "grouped.cuh"
+#include "norm.cuh"
 #include "simt_kernels.cuh"
 #include "umma_gemm.cuh"
 
@@ -248,7 +250,7 @@ extern "C" int o64_last_status(o64_handle_t h, void *stream, int *detail) {
         CUDA_TRY(cudaMemsetAsync(h->status_word, 0, sizeof(int), s));
         // a kernel that gave up may have left words of the last-wave K split set
         if (h->tail_flags) CUDA_TRY(cudaMemsetAsync(h->tail_flags, 0, kTailFlagWords * sizeof(unsigned), s));
-        return O64_ERR_TIMEOUT;
+        return word == kBadOffsets ? O64_ERR_CONFORM : O64_ERR_TIMEOUT;
     }
     return O64_OK;
 }
@@ -795,6 +797,177 @@ extern "C" int o64_gemm_s8s8_s32(o64_handle_t h, int64_t M, int64_t N, int64_t K
                                  void *stream) {
     return umma_entry(h, O64_KIND_S8, false, EPI_S32, M, N, K, A, lda, B, nullptr, ldb, C, ldc, nullptr,
                       nullptr, nullptr, O64_ACT_NONE, stream);
+}
+
+// ---- around the products of a feed-forward layer --------------------------------------------
+// Device pointers of the handle's device only: nothing here stages, repacks or allocates.
+static bool device_operands(o64_handle_t h, std::initializer_list<const void *> ptrs) {
+    for (const void *p : ptrs)
+        if (p && ptr_class(p, h->device) != PTR_DEVICE) return false;
+    return true;
+}
+
+extern "C" int o64_rmsnorm_bf16(o64_handle_t h, int64_t T, int64_t N, const void *X, int64_t ldx, const void *R, int64_t ldr,
+                                void *S, int64_t lds, const void *W, int w_f32, float eps, int out_kind, int scale_block, void *Y,
+                                int64_t ldy, float *scales, int64_t ldscales, float *rstd, void *stream) {
+    if (!h || T < 0 || N < 0) return O64_ERR_RANK;
+    if (out_kind != O64_OUT_BF16 && out_kind != O64_OUT_E4M3) return O64_ERR_DTYPE;
+    const bool e4m3 = out_kind == O64_OUT_E4M3;
+    if (e4m3 && scale_block != 0 && scale_block != 128) return O64_ERR_DTYPE;
+    if (T == 0 || N == 0) return O64_OK;
+    if (N > kNormMaxCols || T > INT32_MAX || !X || !W || !Y || (e4m3 && !scales)) return O64_ERR_RANK;
+    if (ldx < N || ldy < N || (R && ldr < N) || (S && lds < N)) return O64_ERR_CONFORM;
+    if (e4m3 && ldscales < (scale_block ? (N + 127) / 128 : 1)) return O64_ERR_CONFORM;
+    if (!device_operands(h, {X, R, S, W, Y, scales, rstd})) return O64_ERR_RANK;
+    DeviceGuard g(h->device);
+    NormCall c;
+    c.T = T, c.N = N, c.X = X, c.ldx = ldx, c.R = R, c.ldr = ldr, c.S = S, c.lds = lds, c.W = W, c.w_f32 = w_f32 != 0;
+    c.eps = eps, c.out_kind = out_kind, c.row_scale = scale_block == 0, c.Y = Y, c.ldy = ldy, c.scales = scales;
+    c.ldscales = ldscales, c.rstd = rstd, c.stream = (cudaStream_t)stream;
+    return norm_forward(c, h->num_sms);
+}
+
+extern "C" size_t o64_rmsnorm_bf16_backward_workspace(int64_t T, int64_t N) {
+    if (T <= 0 || N <= 0 || N > kNormMaxCols) return 0;
+    return (size_t)norm_backward_partials(T, N) * (size_t)N * sizeof(float);
+}
+
+extern "C" int o64_rmsnorm_bf16_backward(o64_handle_t h, int64_t T, int64_t N, const void *dY, int64_t lddy, const void *S,
+                                         int64_t lds, const void *W, int w_f32, const float *rstd, const void *dR, int64_t lddr,
+                                         void *dX, int64_t lddx, float *dW, void *workspace, void *stream) {
+    if (!h || T < 0 || N < 0) return O64_ERR_RANK;
+    if (N == 0) return O64_OK;
+    if (N > kNormMaxCols || T > INT32_MAX) return O64_ERR_RANK;
+    DeviceGuard g(h->device);
+    cudaStream_t s = (cudaStream_t)stream;
+    if (T == 0) {  // the sum over no rows
+        if (!dW) return O64_OK;
+        if (!device_operands(h, {dW})) return O64_ERR_RANK;
+        CUDA_TRY(cudaMemsetAsync(dW, 0, (size_t)N * 4, s));
+        return O64_OK;
+    }
+    if (!dY || !S || !W || !rstd || !dX || (dW && !workspace)) return O64_ERR_RANK;
+    if (lddy < N || lds < N || lddx < N || (dR && lddr < N)) return O64_ERR_CONFORM;
+    if (!device_operands(h, {dY, S, W, rstd, dR, dX, dW, workspace})) return O64_ERR_RANK;
+    NormBackwardCall c;
+    c.T = T, c.N = N, c.dY = dY, c.lddy = lddy, c.S = S, c.lds = lds, c.W = W, c.w_f32 = w_f32 != 0, c.rstd = rstd;
+    c.dR = dR, c.lddr = lddr, c.dX = dX, c.lddx = lddx, c.dW = dW, c.workspace = static_cast<float *>(workspace), c.stream = s;
+    return norm_backward(c);
+}
+
+// Checks what the grouped and block-scaled products have in common and launches.  Returns O64_ERR_* or O64_OK.
+static int grouped_entry(o64_handle_t h, GroupedCall c, void *stream) {
+    if (!h || c.G < 0 || c.T < 0 || c.N < 0 || c.K < 0) return O64_ERR_RANK;
+    const bool swiglu = gepi_swiglu(c.epi);
+    const bool scaled = c.kind == O64_KIND_FP8;
+    if (c.G > INT32_MAX || c.T > INT32_MAX || c.N > INT32_MAX / 2 || c.K > INT32_MAX) return O64_ERR_RANK;
+    if (c.G == 0 || c.N == 0 || (c.wgrad ? c.K == 0 : c.T == 0)) return O64_OK;
+    if (swiglu && c.N % 128) return O64_ERR_CONFORM;
+    const int64_t c_rows = c.wgrad ? c.N : c.T, c_cols = c.wgrad ? c.K : c.N;
+    if (!c.C || (c.epi == GEPI_SWIGLU_E4M3 && !c.scale_c)) return O64_ERR_RANK;
+    if (c.ldc < c_cols || (c.wgrad && c.G > 1 && c.stride_c < (c_rows - 1) * c.ldc + c_cols)) return O64_ERR_CONFORM;
+    if (c.epi == GEPI_SWIGLU_E4M3 && c.ldsc < c.N / 128) return O64_ERR_CONFORM;
+    if (!device_operands(h, {c.A, c.B, c.C, c.scale_a, c.scale_b, c.scale_c, c.offsets})) return O64_ERR_RANK;
+    DeviceGuard g(h->device);
+    c.status_word = h->status_word;
+    c.num_sms = h->num_sms;
+    c.wait_ns = h->wait_ns;
+    c.stream = (cudaStream_t)stream;
+    if ((c.wgrad ? c.T : c.K) == 0) return grouped_zero_launch(c);  // the empty sum
+    const int elem = scaled ? 1 : 2;
+    if (!c.A || !c.B || (scaled && (!c.scale_a || !c.scale_b))) return O64_ERR_RANK;
+    if (c.wgrad) {
+        if (c.lda < c.N || c.ldb < c.K) return O64_ERR_CONFORM;
+    } else {
+        const int64_t b_out = swiglu ? 2 * c.N : c.N;
+        const int64_t b_rows = c.b_kn ? c.K : b_out, b_cols = c.b_kn ? b_out : c.K;
+        if (c.lda < c.K || c.ldb < b_cols || (c.G > 1 && c.stride_b < (b_rows - 1) * c.ldb + b_cols)) return O64_ERR_CONFORM;
+        if (scaled) {
+            const int64_t sb_rows = (b_rows + 127) / 128, sb_cols = (b_cols + 127) / 128;
+            if (c.ldsa < (c.K + 127) / 128 || c.ldsb < sb_cols) return O64_ERR_CONFORM;
+            if (c.G > 1 && c.stride_sb < (sb_rows - 1) * c.ldsb + sb_cols) return O64_ERR_CONFORM;
+        }
+        if (c.G > 1 && (c.stride_b * elem) % 16) return O64_ERR_ALIGN;
+    }
+    if (!tma_aligned(c.A, c.lda, elem) || !tma_aligned(c.B, c.ldb, elem)) return O64_ERR_ALIGN;
+    return grouped_pair_launch(c);
+}
+
+static GroupedCall grouped_call(int kind, int epi, int64_t G, int64_t T, int64_t N, int64_t K, const void *A, int64_t lda,
+                                const int32_t *offsets, const void *B, int64_t ldb, int64_t stride_b, bool b_kn, void *C,
+                                int64_t ldc) {
+    GroupedCall c;
+    c.kind = kind, c.epi = epi, c.G = G, c.T = T, c.N = N, c.K = K, c.A = A, c.lda = lda, c.offsets = offsets;
+    c.B = B, c.ldb = ldb, c.stride_b = stride_b, c.b_kn = b_kn, c.C = C, c.ldc = ldc;
+    return c;
+}
+
+static void grouped_scales(GroupedCall *c, const float *sa, int64_t ldsa, const float *sb, int64_t ldsb, int64_t stride_sb) {
+    c->scale_a = sa, c->ldsa = ldsa, c->scale_b = sb, c->ldsb = ldsb, c->stride_sb = stride_sb;
+}
+
+extern "C" int o64_gemm_grouped_bf16(o64_handle_t h, int64_t G, int64_t T, int64_t N, int64_t K, const void *A, int64_t lda,
+                                     const int32_t *offsets, const void *B, int64_t ldb, int64_t stride_b, int transB, void *C,
+                                     int64_t ldc, void *stream) {
+    if (!offsets && G > 0) return O64_ERR_RANK;
+    return grouped_entry(h, grouped_call(O64_KIND_BF16, GEPI_BF16, G, T, N, K, A, lda, offsets, B, ldb, stride_b, transB == 0, C, ldc),
+                         stream);
+}
+
+extern "C" int o64_gemm_grouped_fp8_block(o64_handle_t h, int64_t G, int64_t T, int64_t N, int64_t K, const void *A8, int64_t lda,
+                                          const float *scaleA, int64_t ldsa, const int32_t *offsets, const void *B8, int64_t ldb,
+                                          int64_t stride_b, int transB, const float *scaleB, int64_t ldsb, int64_t stride_sb, void *C,
+                                          int64_t ldc, void *stream) {
+    if (!offsets && G > 0) return O64_ERR_RANK;
+    GroupedCall c = grouped_call(O64_KIND_FP8, GEPI_BF16, G, T, N, K, A8, lda, offsets, B8, ldb, stride_b, transB == 0, C, ldc);
+    grouped_scales(&c, scaleA, ldsa, scaleB, ldsb, stride_sb);
+    return grouped_entry(h, c, stream);
+}
+
+extern "C" int o64_gemm_grouped_fp8_block_swiglu(o64_handle_t h, int64_t G, int64_t T, int64_t N, int64_t K, const void *A8,
+                                                 int64_t lda, const float *scaleA, int64_t ldsa, const int32_t *offsets,
+                                                 const void *B8, int64_t ldb, int64_t stride_b, const float *scaleB, int64_t ldsb,
+                                                 int64_t stride_sb, void *H, int64_t ldh, int out_kind, float *scaleH, int64_t ldsh,
+                                                 void *stream) {
+    if (!offsets && G > 0) return O64_ERR_RANK;
+    if (out_kind != O64_OUT_BF16 && out_kind != O64_OUT_E4M3) return O64_ERR_DTYPE;
+    GroupedCall c = grouped_call(O64_KIND_FP8, out_kind == O64_OUT_E4M3 ? GEPI_SWIGLU_E4M3 : GEPI_SWIGLU_BF16, G, T, N, K, A8, lda,
+                                 offsets, B8, ldb, stride_b, false, H, ldh);
+    grouped_scales(&c, scaleA, ldsa, scaleB, ldsb, stride_sb);
+    if (out_kind == O64_OUT_E4M3) c.scale_c = scaleH, c.ldsc = ldsh;
+    return grouped_entry(h, c, stream);
+}
+
+extern "C" int o64_gemm_fp8_block(o64_handle_t h, int64_t M, int64_t N, int64_t K, const void *A8, int64_t lda, const float *scaleA,
+                                  int64_t ldsa, const void *B8, int64_t ldb, int transB, const float *scaleB, int64_t ldsb, void *C,
+                                  int64_t ldc, void *stream) {
+    GroupedCall c = grouped_call(O64_KIND_FP8, GEPI_BF16, 1, M, N, K, A8, lda, nullptr, B8, ldb, 0, transB == 0, C, ldc);
+    grouped_scales(&c, scaleA, ldsa, scaleB, ldsb, 0);
+    return grouped_entry(h, c, stream);
+}
+
+extern "C" int o64_gemm_fp8_block_swiglu(o64_handle_t h, int64_t M, int64_t N, int64_t K, const void *A8, int64_t lda,
+                                         const float *scaleA, int64_t ldsa, const void *B8, int64_t ldb, const float *scaleB,
+                                         int64_t ldsb, void *H, int64_t ldh, int out_kind, float *scaleH, int64_t ldsh,
+                                         void *stream) {
+    if (out_kind != O64_OUT_BF16 && out_kind != O64_OUT_E4M3) return O64_ERR_DTYPE;
+    GroupedCall c = grouped_call(O64_KIND_FP8, out_kind == O64_OUT_E4M3 ? GEPI_SWIGLU_E4M3 : GEPI_SWIGLU_BF16, 1, M, N, K, A8, lda,
+                                 nullptr, B8, ldb, 0, false, H, ldh);
+    grouped_scales(&c, scaleA, ldsa, scaleB, ldsb, 0);
+    if (out_kind == O64_OUT_E4M3) c.scale_c = scaleH, c.ldsc = ldsh;
+    return grouped_entry(h, c, stream);
+}
+
+extern "C" int o64_gemm_grouped_bf16_wgrad(o64_handle_t h, int64_t G, int64_t T, int64_t N, int64_t K, const void *dC, int64_t lddc,
+                                           const void *A, int64_t lda, const int32_t *offsets, void *dB, int64_t lddb,
+                                           int64_t stride_db, int out_kind, void *stream) {
+    if (!offsets && G > 0) return O64_ERR_RANK;
+    if (out_kind != O64_OUT_BF16 && out_kind != O64_OUT_F32) return O64_ERR_DTYPE;
+    GroupedCall c = grouped_call(O64_KIND_BF16, out_kind == O64_OUT_F32 ? GEPI_F32 : GEPI_BF16, G, T, N, K, dC, lddc, offsets, A, lda, 0,
+                                 false, dB, lddb);
+    c.wgrad = true;
+    c.stride_c = stride_db;
+    return grouped_entry(h, c, stream);
 }
 
 // Test hook: o64_gemm_bf16 (B [N,K], no epilogue) run by the kernel the handle's pin selects, in an

@@ -1,0 +1,119 @@
+// Products grouped by expert, and the e4m3 product with a scale for each block of 128: host-side
+// interface and the pieces the kernels share (umma_grouped.cu: CTA pairs on 256 x 256 tiles;
+// umma_grouped_rows.cu: few rows an expert).
+#pragma once
+#include <cuda.h>
+
+#include "umma_common.cuh"
+
+namespace o64 {
+
+// What is left in the accumulators becomes ...
+enum : int {
+    GEPI_BF16 = 0,         // bf16
+    GEPI_F32 = 1,          // fp32 as it is
+    GEPI_SWIGLU_BF16 = 2,  // silu(gate) * up, bf16
+    GEPI_SWIGLU_E4M3 = 3   // silu(gate) * up, e4m3 with a scale for each 128 columns of a row
+};
+__host__ __device__ constexpr bool gepi_swiglu(int e) { return e >= GEPI_SWIGLU_BF16; }
+__host__ __device__ constexpr int gepi_bytes(int e) { return e == GEPI_F32 ? 4 : (e == GEPI_SWIGLU_E4M3 ? 1 : 2); }
+
+// Status-word codes.  0x6..: the group offsets in device memory are not ascending within 0 .. T.
+constexpr int kBadOffsets = 0x601;
+constexpr int kWaitGroupProducer = 0x701, kWaitGroupFull = 0x702, kWaitGroupAccEmpty = 0x703, kWaitGroupAccFull = 0x704,
+              kWaitGroupTail = 0x705, kWaitGroupHalf = 0x706;
+
+// One call.  Rows T of A are sorted by group; offsets (device, G + 1 ints) bound the groups; NULL: one
+// group of T rows.  B is [G][N][K] (or [G][K][N]: b_kn), C is [T][N].  wgrad: A is dC [T][N], B is the
+// forward's A [T][K], C is [G][N][K] and the sum runs over a group's rows.  swiglu: N counts the result's
+// columns, B has 2 N rows.  Leading dimensions in elements.
+struct GroupedCall {
+    int kind = O64_KIND_BF16;  // O64_KIND_BF16, or O64_KIND_FP8 with block scales
+    bool b_kn = false, wgrad = false;
+    int epi = GEPI_BF16;
+    int64_t G = 1, T = 0, N = 0, K = 0;
+    const void *A = nullptr, *B = nullptr;
+    void *C = nullptr;
+    int64_t lda = 0, ldb = 0, stride_b = 0, ldc = 0, stride_c = 0;
+    const float *scale_a = nullptr, *scale_b = nullptr;  // [T][K/128]; [G][B rows/128][B columns/128]
+    int64_t ldsa = 0, ldsb = 0, stride_sb = 0;
+    float *scale_c = nullptr;
+    int64_t ldsc = 0;
+    const int *offsets = nullptr;
+    int *status_word = nullptr;
+    int num_sms = 148;
+    unsigned long long wait_ns = 0;
+    cudaStream_t stream = nullptr;
+};
+
+struct GroupedParams {
+    int G, T, N, K;  // N: columns of C
+    int rows_m;      // wgrad: rows of one C
+    int num_m_tiles, num_n_tiles;
+    int num_k_blocks;
+    void *C;
+    long long ldc, stride_c;
+    const float *scale_a, *scale_b;
+    long long ldsa, ldsb, stride_sb;
+    float *scale_c;
+    long long ldsc;
+    const int *offsets;
+    int vec_ok, tma_store;
+    int *status;
+    unsigned long long wait_ns;
+};
+
+// A group's rows, kept inside [0, T) whatever the offsets say; *bad: they are not ascending within 0 .. T.
+__device__ __forceinline__ void group_rows(const GroupedParams &p, int g, int &begin, int &end, bool *bad = nullptr) {
+    if (!p.offsets) {
+        begin = 0;
+        end = p.T;
+        return;
+    }
+    const int a = __ldg(p.offsets + g), b = __ldg(p.offsets + g + 1);
+    begin = min(max(a, 0), p.T);
+    end = min(max(b, begin), p.T);
+    if (bad) *bad = a < 0 || b < a || b > p.T;
+}
+
+int grouped_pair_launch(const GroupedCall &c);
+// Sets the rows of the groups (wgrad: every C) to the empty sum: K == 0, or a weight gradient over no rows.
+int grouped_zero_launch(const GroupedCall &c);
+
+int encode_3d(CUtensorMap *tm, int elem, const void *base, int64_t cols, int64_t rows, int64_t depth, int64_t ld, int64_t stride,
+              int box_cols, int box_rows, bool promote);
+
+__device__ __forceinline__ void tma_load_3d_pair(uint32_t smem_dst, const void *tmap, int x, int y, int z, uint32_t bar) {
+    asm volatile(
+        "cp.async.bulk.tensor.3d.cta_group::2.shared::cluster.global.mbarrier::complete_tx::bytes "
+        "[%0], [%1, {%2, %3, %4}], [%5];" ::"r"(smem_dst), "l"(tmap), "r"(x), "r"(y), "r"(z), "r"(bar)
+        : "memory");
+}
+__device__ __forceinline__ void tma_load_3d_hint(uint32_t smem_dst, const void *tmap, int x, int y, int z, uint32_t bar,
+                                                 uint64_t policy) {
+    asm volatile(
+        "cp.async.bulk.tensor.3d.shared::cluster.global.mbarrier::complete_tx::bytes.L2::cache_hint "
+        "[%0], [%1, {%2, %3, %4}], [%5], %6;" ::"r"(smem_dst), "l"(tmap), "r"(x), "r"(y), "r"(z), "r"(bar), "l"(policy)
+        : "memory");
+}
+__device__ __forceinline__ void tma_store_3d(const void *tmap, uint32_t smem_src, int x, int y, int z) {
+    asm volatile("cp.async.bulk.tensor.3d.global.shared::cta.bulk_group [%0, {%2, %3, %4}], [%1];" ::"l"(tmap), "r"(smem_src),
+                 "r"(x), "r"(y), "r"(z)
+                 : "memory");
+}
+
+// silu(g) * u
+__device__ __forceinline__ float silu_mul(float g, float u) { return g / (1.0f + __expf(-g)) * u; }
+
+// amax / 448, or 1 where that is no normal number (NaN stays NaN).
+__device__ __forceinline__ float block_scale_of(float amax) {
+    const float s = amax / 448.0f;
+    return s < 1.17549435e-38f ? 1.0f : s;
+}
+__device__ __forceinline__ float fmax_nan(float a, float b) {
+    float r;
+    asm("max.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(a), "f"(b));
+    return r;
+}
+
+}  // namespace o64

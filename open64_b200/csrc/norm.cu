@@ -1,0 +1,399 @@
+// RMS norm in front of (and, in training, behind) the products: the residual's addition, the norm and
+// the 8-bit operand the next product reads, in one pass over the row.
+//
+//   s = x + r          h[j] = s[j] / sqrt(mean(s^2) + eps) * w[j]
+//   e4m3: scale = max |h| over 128 columns (or the row) / 448, q = e4m3(h / scale)
+//
+// A row of at most 32768 columns stays in the registers of one group of threads between the two
+// things that need all of it (the mean, the largest value), so every operand crosses HBM once.  The
+// norm is taken of the sum in fp32; the stream s that goes on to the next layer is that sum rounded
+// to bf16 once.
+//
+// Gradient, with n = s * rstd, g = dy * w:   dx = rstd * (g - n * mean(g n)) + dr   (x and r receive
+// the same one),   dw[j] = sum over rows of dy n.  The sum over rows runs in two fixed stages (a
+// partial row per thread group, then one addition per column), so that it does not depend on timing.
+#include <cuda_bf16.h>
+#include <cuda_fp8.h>
+
+#include "norm.cuh"
+
+namespace o64 {
+
+namespace {
+
+constexpr int kNormMaxThreads = 512;
+constexpr float kE4m3Max = 448.0f;
+constexpr float kMinNormal = 1.17549435e-38f;
+
+__device__ __forceinline__ float max_nan(float a, float b) {  // NaN wins, as in a maximum of the definition
+    float r;
+    asm("max.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(a), "f"(b));
+    return r;
+}
+
+// Eight consecutive bf16 values of a row; columns >= n read as zero.
+template <bool VEC>
+__device__ __forceinline__ void load8(const __nv_bfloat16 *row, int col, int n, float (&v)[8]) {
+    if constexpr (VEC) {
+        uint4 raw = make_uint4(0, 0, 0, 0);
+        if (col < n) raw = *reinterpret_cast<const uint4 *>(row + col);
+        const uint32_t w[4] = {raw.x, raw.y, raw.z, raw.w};
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            v[2 * i] = __uint_as_float(w[i] << 16);
+            v[2 * i + 1] = __uint_as_float(w[i] & 0xffff0000u);
+        }
+    } else {
+#pragma unroll
+        for (int i = 0; i < 8; ++i) v[i] = col + i < n ? __bfloat162float(row[col + i]) : 0.0f;
+    }
+}
+
+template <bool VEC>
+__device__ __forceinline__ void store8(__nv_bfloat16 *row, int col, int n, const float (&v)[8]) {
+    if constexpr (VEC) {
+        if (col < n) {
+            uint32_t w[4];
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                const __nv_bfloat162 p = __floats2bfloat162_rn(v[2 * i], v[2 * i + 1]);
+                w[i] = *reinterpret_cast<const uint32_t *>(&p);
+            }
+            *reinterpret_cast<uint4 *>(row + col) = make_uint4(w[0], w[1], w[2], w[3]);
+        }
+    } else {
+#pragma unroll
+        for (int i = 0; i < 8; ++i)
+            if (col + i < n) row[col + i] = __float2bfloat16_rn(v[i]);
+    }
+}
+
+template <bool VEC>
+__device__ __forceinline__ void load_w8(const void *w, bool f32, int col, int n, float (&v)[8]) {
+    if (f32) {
+        const float *p = static_cast<const float *>(w);
+        if (VEC && col < n) {
+            const float4 a = __ldg(reinterpret_cast<const float4 *>(p + col));
+            const float4 b = __ldg(reinterpret_cast<const float4 *>(p + col) + 1);
+            v[0] = a.x, v[1] = a.y, v[2] = a.z, v[3] = a.w, v[4] = b.x, v[5] = b.y, v[6] = b.z, v[7] = b.w;
+        } else {
+#pragma unroll
+            for (int i = 0; i < 8; ++i) v[i] = col + i < n ? __ldg(p + col + i) : 0.0f;
+        }
+    } else {
+        load8<VEC>(static_cast<const __nv_bfloat16 *>(w), col, n, v);
+    }
+}
+
+// Sum / maximum over the blockDim.x threads of one row (threadIdx.y counts the rows of the block).
+// `slot`: shared floats, one per warp of the block; each reduction of a loop uses other ones in turn.
+template <bool MAX>
+__device__ __forceinline__ float row_reduce(float v, float *slot) {
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) {
+        const float x = __shfl_xor_sync(0xffffffffu, v, o);
+        v = MAX ? max_nan(v, x) : v + x;
+    }
+    const int warps = blockDim.x >> 5;
+    if (warps == 1) return v;
+    float *mine = slot + threadIdx.y * warps;
+    if ((threadIdx.x & 31) == 0) mine[threadIdx.x >> 5] = v;
+    __syncthreads();
+    float r = mine[0];
+    for (int i = 1; i < warps; ++i) r = MAX ? max_nan(r, mine[i]) : r + mine[i];
+    return r;
+}
+
+struct FwdParams {
+    long long T;
+    int N;
+    const __nv_bfloat16 *X, *R;
+    __nv_bfloat16 *S;
+    long long ldx, ldr, lds, ldy, ldscales;
+    const void *W;
+    void *Y;
+    float *scales, *rstd;
+    float eps;
+    int w_f32, row_scale;
+};
+
+__device__ __forceinline__ float scale_of(float amax) {
+    const float s = amax / kE4m3Max;
+    return s < kMinNormal ? 1.0f : s;  // (NaN stays NaN)
+}
+
+// Columns of thread t: (i * blockDim.x + t) * 8 .. + 7 for i < NV, so that 16 neighbouring threads hold
+// one scale block of 128.
+template <int NV, bool VEC, bool E4M3>
+__global__ void __launch_bounds__(kNormMaxThreads) norm_forward_kernel(const FwdParams p) {
+    __shared__ float slots[2][16];
+    const long long row = (long long)blockIdx.x * blockDim.y + threadIdx.y;
+    const bool live = row < p.T;  // every thread takes part in the reductions
+    const int n = live ? p.N : 0;
+    const __nv_bfloat16 *x = p.X + (live ? row * p.ldx : 0);
+    const __nv_bfloat16 *r = p.R ? p.R + (live ? row * p.ldr : 0) : nullptr;
+    float v[NV][8];
+    float sq = 0.0f;
+#pragma unroll
+    for (int i = 0; i < NV; ++i) load8<VEC>(x, (i * blockDim.x + threadIdx.x) * 8, n, v[i]);
+    if (r) {
+#pragma unroll
+        for (int i = 0; i < NV; ++i) {
+            float a[8];
+            load8<VEC>(r, (i * blockDim.x + threadIdx.x) * 8, n, a);
+#pragma unroll
+            for (int e = 0; e < 8; ++e) v[i][e] += a[e];
+        }
+    }
+#pragma unroll
+    for (int i = 0; i < NV; ++i)
+#pragma unroll
+        for (int e = 0; e < 8; ++e) sq = fmaf(v[i][e], v[i][e], sq);
+    if (p.S) {
+#pragma unroll
+        for (int i = 0; i < NV; ++i) store8<VEC>(p.S + (live ? row * p.lds : 0), (i * blockDim.x + threadIdx.x) * 8, n, v[i]);
+    }
+    const float rstd = 1.0f / sqrtf(row_reduce<false>(sq, slots[0]) / (float)p.N + p.eps);
+    if (p.rstd && live && threadIdx.x == 0) p.rstd[row] = rstd;
+    float top = 0.0f;
+#pragma unroll
+    for (int i = 0; i < NV; ++i) {
+        float w[8];
+        load_w8<VEC>(p.W, p.w_f32, (i * blockDim.x + threadIdx.x) * 8, p.N, w);
+#pragma unroll
+        for (int e = 0; e < 8; ++e) {
+            v[i][e] = v[i][e] * rstd * w[e];
+            // past the row's end there is 0 * rstd, which may be NaN: not part of any maximum
+            if (E4M3 && p.row_scale && (i * blockDim.x + threadIdx.x) * 8 + e < n) top = max_nan(top, fabsf(v[i][e]));
+        }
+    }
+    if constexpr (!E4M3) {
+#pragma unroll
+        for (int i = 0; i < NV; ++i)
+            store8<VEC>(static_cast<__nv_bfloat16 *>(p.Y) + (live ? row * p.ldy : 0), (i * blockDim.x + threadIdx.x) * 8, n, v[i]);
+    } else {
+        float scale = 1.0f;
+        if (p.row_scale) {
+            scale = scale_of(row_reduce<true>(top, slots[1]));
+            if (live && threadIdx.x == 0) p.scales[row * p.ldscales] = scale;
+        }
+        uint8_t *y = static_cast<uint8_t *>(p.Y) + (live ? row * p.ldy : 0);
+#pragma unroll
+        for (int i = 0; i < NV; ++i) {
+            const int col = (i * blockDim.x + threadIdx.x) * 8;
+            if (!p.row_scale) {
+                float m = 0.0f;
+#pragma unroll
+                for (int e = 0; e < 8; ++e)
+                    if (col + e < n) m = max_nan(m, fabsf(v[i][e]));
+#pragma unroll
+                for (int o = 8; o > 0; o >>= 1) m = max_nan(m, __shfl_xor_sync(0xffffffffu, m, o));
+                scale = scale_of(m);
+                if (col < n && (threadIdx.x & 15) == 0) p.scales[row * p.ldscales + col / 128] = scale;
+            }
+            // one reciprocal per block instead of a division per value: within an ulp of h / scale before
+            // the rounding to four bits
+            const float inv = 1.0f / scale;
+            uint32_t q[2] = {0, 0};
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+                const float2 two = make_float2(v[i][2 * e] * inv, v[i][2 * e + 1] * inv);
+                q[e >> 1] |= (uint32_t)__nv_cvt_float2_to_fp8x2(two, __NV_SATFINITE, __NV_E4M3) << (16 * (e & 1));
+            }
+            if constexpr (VEC) {
+                if (col < n) *reinterpret_cast<uint2 *>(y + col) = make_uint2(q[0], q[1]);
+            } else {
+#pragma unroll
+                for (int e = 0; e < 8; ++e)
+                    if (col + e < n) y[col + e] = (uint8_t)(q[e >> 2] >> (8 * (e & 3)));
+            }
+        }
+    }
+}
+
+struct BwdParams {
+    long long T;
+    int N;
+    const __nv_bfloat16 *dY, *S, *dR;
+    __nv_bfloat16 *dX;
+    long long lddy, lds, lddr, lddx;
+    const void *W;
+    const float *rstd;
+    float *partial;  // [gridDim.x * blockDim.y][N], or NULL
+    int w_f32;
+};
+
+// Each thread group walks the rows grid-stride and keeps its columns' share of dW in registers.
+template <int NV, bool VEC>
+__global__ void __launch_bounds__(kNormMaxThreads) norm_backward_kernel(const BwdParams p) {
+    __shared__ float slots[2][16];
+    float dw[NV][8];
+#pragma unroll
+    for (int i = 0; i < NV; ++i)
+#pragma unroll
+        for (int e = 0; e < 8; ++e) dw[i][e] = 0.0f;
+    const long long group = (long long)blockIdx.x * blockDim.y + threadIdx.y;
+    const long long groups = (long long)gridDim.x * blockDim.y;
+    int turn = 0;
+    // all rows of a block's groups go through the same number of rounds (the reductions synchronise the block)
+    for (long long row = group; row - threadIdx.y < p.T; row += groups, turn ^= 1) {
+        const bool live = row < p.T;
+        const int n = live ? p.N : 0;
+        const long long at = live ? row : 0;
+        const float rstd = p.rstd[at];
+        float g[NV][8], nn[NV][8];
+        float dot = 0.0f;
+#pragma unroll
+        for (int i = 0; i < NV; ++i) {
+            const int col = (i * blockDim.x + threadIdx.x) * 8;
+            load8<VEC>(p.dY + at * p.lddy, col, n, g[i]);
+            load8<VEC>(p.S + at * p.lds, col, n, nn[i]);
+        }
+#pragma unroll
+        for (int i = 0; i < NV; ++i) {
+            const int col = (i * blockDim.x + threadIdx.x) * 8;
+            float w[8];
+            load_w8<VEC>(p.W, p.w_f32, col, p.N, w);
+#pragma unroll
+            for (int e = 0; e < 8; ++e) {
+                nn[i][e] = col + e < n ? nn[i][e] * rstd : 0.0f;
+                dw[i][e] = fmaf(g[i][e], nn[i][e], dw[i][e]);
+                g[i][e] *= w[e];
+                dot = fmaf(g[i][e], nn[i][e], dot);
+            }
+        }
+        const float mean = row_reduce<false>(dot, slots[turn]) / (float)p.N;
+#pragma unroll
+        for (int i = 0; i < NV; ++i) {
+            const int col = (i * blockDim.x + threadIdx.x) * 8;
+            float out[8], dr[8];
+            if (p.dR) load8<VEC>(p.dR + at * p.lddr, col, n, dr);
+#pragma unroll
+            for (int e = 0; e < 8; ++e) {
+                out[e] = rstd * (g[i][e] - nn[i][e] * mean);
+                if (p.dR) out[e] += dr[e];
+            }
+            store8<VEC>(p.dX + at * p.lddx, col, n, out);
+        }
+    }
+    if (p.partial) {
+        float *dst = p.partial + group * p.N;
+#pragma unroll
+        for (int i = 0; i < NV; ++i)
+#pragma unroll
+            for (int e = 0; e < 8; ++e) {
+                const int col = (i * blockDim.x + threadIdx.x) * 8 + e;
+                if (col < p.N) dst[col] = dw[i][e];
+            }
+    }
+}
+
+// dW[j] = sum over the partial rows: 32 columns per block, 16 threads down the rows of each.
+__global__ void __launch_bounds__(512) norm_dw_kernel(const float *partial, long long rows, int N, float *dW) {
+    __shared__ float part[16][33];
+    const int col = blockIdx.x * 32 + threadIdx.x;
+    float s = 0.0f;
+    if (col < N)
+        for (long long r = threadIdx.y; r < rows; r += 16) s += partial[r * N + col];
+    part[threadIdx.y][threadIdx.x] = s;
+    __syncthreads();
+    if (threadIdx.y == 0 && col < N) {
+#pragma unroll
+        for (int i = 1; i < 16; ++i) s += part[i][threadIdx.x];
+        dW[col] = s;
+    }
+}
+
+bool vec8(const void *p, int64_t ld) { return !p || ((reinterpret_cast<uintptr_t>(p) & 15u) == 0 && ld % 8 == 0); }
+
+// Threads per row (a multiple of 32) for NV vectors of eight columns a thread.
+int threads_for(int64_t N, int nv) { return (int)((((N + 7) / 8 + nv - 1) / nv + 31) / 32 * 32); }
+
+// The largest number of columns a thread may have decides between few and many threads per row: few rows
+// want the row spread thin (latency), many rows want loads in flight per thread.
+int pick_nv(int64_t N, int smallest) {
+    int nv = smallest;
+    while (threads_for(N, nv) > kNormMaxThreads) nv *= 2;
+    return nv;
+}
+
+template <int NV, bool VEC>
+int launch_forward(const FwdParams &p, bool e4m3, dim3 grid, dim3 block, cudaStream_t s) {
+    if (e4m3)
+        norm_forward_kernel<NV, VEC, true><<<grid, block, 0, s>>>(p);
+    else
+        norm_forward_kernel<NV, VEC, false><<<grid, block, 0, s>>>(p);
+    return cudaGetLastError() == cudaSuccess ? O64_OK : O64_ERR_CUDA;
+}
+
+}  // namespace
+
+int norm_forward(const NormCall &c, int num_sms) {
+    const bool e4m3 = c.out_kind == O64_OUT_E4M3;
+    const bool y_ok = e4m3 ? (reinterpret_cast<uintptr_t>(c.Y) & 7u) == 0 && c.ldy % 8 == 0 : vec8(c.Y, c.ldy);
+    const bool vec = c.N % 8 == 0 && vec8(c.X, c.ldx) && vec8(c.R, c.ldr) && vec8(c.S, c.lds) && y_ok && vec8(c.W, 8);
+    FwdParams p;
+    p.T = c.T, p.N = (int)c.N;
+    p.X = static_cast<const __nv_bfloat16 *>(c.X), p.ldx = c.ldx;
+    p.R = static_cast<const __nv_bfloat16 *>(c.R), p.ldr = c.ldr;
+    p.S = static_cast<__nv_bfloat16 *>(c.S), p.lds = c.lds;
+    p.W = c.W, p.w_f32 = c.w_f32, p.eps = c.eps;
+    p.Y = c.Y, p.ldy = c.ldy, p.scales = c.scales, p.ldscales = c.ldscales, p.rstd = c.rstd, p.row_scale = c.row_scale;
+    const int nv = pick_nv(c.N, c.T <= 2 * num_sms ? 1 : 4);
+    const int tpr = threads_for(c.N, nv);
+    const int rows = tpr >= 128 ? 1 : 128 / tpr;
+    const dim3 block(tpr, rows), grid((unsigned)((c.T + rows - 1) / rows));
+    switch (nv) {
+    case 1: return vec ? launch_forward<1, true>(p, e4m3, grid, block, c.stream) : launch_forward<1, false>(p, e4m3, grid, block, c.stream);
+    case 2: return vec ? launch_forward<2, true>(p, e4m3, grid, block, c.stream) : launch_forward<2, false>(p, e4m3, grid, block, c.stream);
+    case 4: return vec ? launch_forward<4, true>(p, e4m3, grid, block, c.stream) : launch_forward<4, false>(p, e4m3, grid, block, c.stream);
+    default: return vec ? launch_forward<8, true>(p, e4m3, grid, block, c.stream) : launch_forward<8, false>(p, e4m3, grid, block, c.stream);
+    }
+}
+
+static void backward_shape(int64_t T, int64_t N, int *nv, dim3 *block, int64_t *blocks) {
+    *nv = pick_nv(N, 2);
+    const int tpr = threads_for(N, *nv);
+    const int rows = tpr >= 128 ? 1 : 128 / tpr;
+    *block = dim3(tpr, rows);
+    const int64_t want = (T + rows - 1) / rows;
+    *blocks = want < 444 ? want : 444;  // three blocks per SM
+}
+
+int64_t norm_backward_partials(int64_t T, int64_t N) {
+    int nv;
+    dim3 block;
+    int64_t blocks;
+    backward_shape(T, N, &nv, &block, &blocks);
+    return blocks * block.y;
+}
+
+int norm_backward(const NormBackwardCall &c) {
+    int nv;
+    dim3 block;
+    int64_t blocks;
+    backward_shape(c.T, c.N, &nv, &block, &blocks);
+    const bool vec = c.N % 8 == 0 && vec8(c.dY, c.lddy) && vec8(c.S, c.lds) && vec8(c.dR, c.lddr) && vec8(c.dX, c.lddx) && vec8(c.W, 8);
+    BwdParams p;
+    p.T = c.T, p.N = (int)c.N;
+    p.dY = static_cast<const __nv_bfloat16 *>(c.dY), p.lddy = c.lddy;
+    p.S = static_cast<const __nv_bfloat16 *>(c.S), p.lds = c.lds;
+    p.dR = static_cast<const __nv_bfloat16 *>(c.dR), p.lddr = c.lddr;
+    p.dX = static_cast<__nv_bfloat16 *>(c.dX), p.lddx = c.lddx;
+    p.W = c.W, p.w_f32 = c.w_f32, p.rstd = c.rstd;
+    p.partial = c.dW ? c.workspace : nullptr;
+    const unsigned grid = (unsigned)blocks;
+    switch (nv) {
+    case 2: vec ? norm_backward_kernel<2, true><<<grid, block, 0, c.stream>>>(p) : norm_backward_kernel<2, false><<<grid, block, 0, c.stream>>>(p); break;
+    case 4: vec ? norm_backward_kernel<4, true><<<grid, block, 0, c.stream>>>(p) : norm_backward_kernel<4, false><<<grid, block, 0, c.stream>>>(p); break;
+    default: vec ? norm_backward_kernel<8, true><<<grid, block, 0, c.stream>>>(p) : norm_backward_kernel<8, false><<<grid, block, 0, c.stream>>>(p); break;
+    }
+    if (cudaGetLastError() != cudaSuccess) return O64_ERR_CUDA;
+    if (c.dW) {
+        norm_dw_kernel<<<(unsigned)((c.N + 31) / 32), dim3(32, 16), 0, c.stream>>>(c.workspace, blocks * block.y, (int)c.N, c.dW);
+        if (cudaGetLastError() != cudaSuccess) return O64_ERR_CUDA;
+    }
+    return O64_OK;
+}
+
+}  // namespace o64

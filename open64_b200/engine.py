@@ -50,6 +50,70 @@ def _rowmajor(t, name):
     return t
 
 
+def _want(t, name, dtypes, shape=None):
+    """An operand of the given element type(s) and shape (None: any extent), or the library's error."""
+    if t.dtype not in dtypes:
+        raise O64Error(_lib.ERR_DTYPE, f"{name}: {t.dtype}")
+    if not t.is_cuda:
+        raise O64Error(_lib.ERR_RANK, f"{name}: not device memory")
+    if shape is not None:
+        if t.dim() != len(shape):
+            raise O64Error(_lib.ERR_RANK, f"{name}: rank {t.dim()}")
+        for have, need in zip(t.shape, shape):
+            if need is not None and have != need:
+                raise O64Error(_lib.ERR_CONFORM, f"{name}: {tuple(t.shape)}")
+    return t
+
+
+def _ld(t):
+    """Elements between rows of a matrix whose columns are contiguous (a single row: any pitch, here one that TMA takes)."""
+    return t.stride(-2) if t.shape[-2] > 1 else t.shape[-1] + -t.shape[-1] % 16
+
+
+def _laid_out(t):
+    """Contiguous columns, and rows (and matrices) that do not overlap."""
+    rows, cols = t.shape[-2:]
+    return ((cols <= 1 or t.stride(-1) == 1) and (rows <= 1 or t.stride(-2) >= cols) and
+            (t.dim() < 3 or t.shape[0] <= 1 or t.stride(0) >= (rows - 1) * _ld(t) + cols))
+
+
+def _rows(t):
+    """`t` as the library reads a matrix: itself, or a copy."""
+    return t if _laid_out(t) else t.contiguous()
+
+
+def _out(t, name):
+    """A result's memory is the caller's: it is used as it lies or refused, never copied."""
+    if not _laid_out(t):
+        raise O64Error(_lib.ERR_CONFORM, f"{name}: strides {t.stride()}")
+    return t
+
+
+def _tma(t):
+    """`t` as TMA can read it (contiguous columns; base, pitch and matrix stride multiples of 16 bytes): itself,
+    or a copy whose rows are padded."""
+    t = _rows(t)
+    e = t.element_size()
+    if (t.data_ptr() % 16 == 0 and (_ld(t) * e) % 16 == 0 and
+            (t.dim() < 3 or t.shape[0] <= 1 or (t.stride(0) * e) % 16 == 0)):
+        return t
+    if 0 in t.shape:
+        return t
+    cols = t.shape[-1]
+    padded = torch.empty((*t.shape[:-1], cols + -cols % (16 // e)), dtype=t.dtype, device=t.device)
+    padded = padded[..., :cols]
+    padded.copy_(t)
+    return padded
+
+
+def _stride0(t):
+    return t.stride(0) if t.shape[0] > 1 else 0
+
+
+_E4M3, _BF16, _F32 = torch.float8_e4m3fn, torch.bfloat16, torch.float32
+_OUT_DTYPE = {_lib.OUT_BF16: _BF16, _lib.OUT_E4M3: _E4M3, _lib.OUT_F32: _F32}
+
+
 class Engine:
     """One handle on one device.  Not thread-safe; make one per thread or per stream user."""
 
@@ -235,6 +299,202 @@ class Engine:
                                               _ptr(scaleA), _ptr(scaleB), _ptr(bias), _act(act), _ptr(out),
                                               out.stride(0), out_kind, _stream(A8)), "o64_gemm_fp8_scaled_kn")
         return out
+
+    # ---- around the products of a feed-forward layer -----------------------------------
+    def rms_norm(self, x, weight, residual=None, eps=1e-6, out_kind=_lib.OUT_BF16, scale_block=128, out=None, scales=None,
+                 summed=None, rstd=None):
+        """RMS norm of x [T,N] (+ residual), times weight: (y, scales, summed, rstd).
+
+        y is bf16, or e4m3 (out_kind OUT_E4M3) with `scales` [T, ceil(N/128)] (scale_block 128) or [T]
+        (scale_block 0, one per row; None for bf16).  `summed` is x + residual in bf16 (x itself without a
+        residual); pass summed=x or summed=residual to add in place.  rstd [T] is what rms_norm_backward
+        needs."""
+        _want(x, "x", (_BF16,), (None, None))
+        T, N = x.shape
+        x = _rows(x)
+        _want(weight, "weight", (_BF16, _F32), (N,))
+        weight = weight.contiguous()
+        if out_kind not in (_lib.OUT_BF16, _lib.OUT_E4M3) or scale_block not in (0, 128):
+            raise O64Error(_lib.ERR_DTYPE, "rms_norm")
+        if residual is None:
+            if summed is not None:
+                raise O64Error(_lib.ERR_CONFORM, "rms_norm: summed without a residual")
+        else:
+            _want(residual, "residual", (_BF16,), (T, N))
+            residual = _rows(residual)
+            summed = torch.empty((T, N), dtype=_BF16, device=x.device) if summed is None else _out(_want(summed, "summed", (_BF16,), (T, N)), "summed")
+        dtype = _OUT_DTYPE[out_kind]
+        y = torch.empty((T, N), dtype=dtype, device=x.device) if out is None else _out(_want(out, "out", (dtype,), (T, N)), "out")
+        ldscales = 0
+        if out_kind == _lib.OUT_E4M3:
+            shape = (T, -(-N // 128)) if scale_block else (T,)
+            scales = torch.empty(shape, dtype=_F32, device=x.device) if scales is None else _want(scales, "scales", (_F32,), shape)
+            if scale_block:
+                ldscales = _ld(_out(scales, "scales"))
+            else:
+                ldscales = scales.stride(0) if T > 1 else 1
+        elif scales is not None:
+            raise O64Error(_lib.ERR_DTYPE, "rms_norm: scales of a bf16 result")
+        rstd = torch.empty((T,), dtype=_F32, device=x.device) if rstd is None else _want(rstd, "rstd", (_F32,), (T,))
+        if T > 1 and rstd.stride(0) != 1:
+            raise O64Error(_lib.ERR_CONFORM, "rms_norm: rstd is not contiguous")
+        check(self.lib.o64_rmsnorm_bf16(self._h, T, N, x.data_ptr(), _ld(x), None if residual is None else residual.data_ptr(),
+                                        0 if residual is None else _ld(residual), None if residual is None else summed.data_ptr(),
+                                        0 if residual is None else _ld(summed), weight.data_ptr(), 1 if weight.dtype == _F32 else 0, eps,
+                                        out_kind, scale_block, y.data_ptr(), _ld(y), None if scales is None else scales.data_ptr(),
+                                        ldscales, rstd.data_ptr(), _stream(x)), "o64_rmsnorm_bf16")
+        return y, scales, (x if residual is None else summed), rstd
+
+    def rms_norm_backward(self, dy, summed, weight, rstd, dresidual=None, dx=None):
+        """Gradients of rms_norm: (dx, dweight).  dx [T,N] bf16 is the gradient of x and of the residual;
+        `dresidual` is what arrives on the stream from beyond the norm (added to dx); dweight fp32."""
+        _want(dy, "dy", (_BF16,), (None, None))
+        T, N = dy.shape
+        _want(summed, "summed", (_BF16,), (T, N))
+        _want(weight, "weight", (_BF16, _F32), (N,))
+        _want(rstd, "rstd", (_F32,), (T,))
+        dy, summed, weight, rstd = _rows(dy), _rows(summed), weight.contiguous(), rstd.contiguous()
+        if dresidual is not None:
+            dresidual = _rows(_want(dresidual, "dresidual", (_BF16,), (T, N)))
+        dx = torch.empty((T, N), dtype=_BF16, device=dy.device) if dx is None else _out(_want(dx, "dx", (_BF16,), (T, N)), "dx")
+        dw = torch.empty((N,), dtype=_F32, device=dy.device)
+        ws = torch.empty((self.lib.o64_rmsnorm_bf16_backward_workspace(T, N) // 4,), dtype=_F32, device=dy.device)
+        check(self.lib.o64_rmsnorm_bf16_backward(self._h, T, N, dy.data_ptr(), _ld(dy), summed.data_ptr(), _ld(summed), weight.data_ptr(),
+                                                 1 if weight.dtype == _F32 else 0, rstd.data_ptr(),
+                                                 None if dresidual is None else dresidual.data_ptr(),
+                                                 0 if dresidual is None else _ld(dresidual), dx.data_ptr(), _ld(dx), dw.data_ptr(),
+                                                 ws.data_ptr(), _stream(dy)), "o64_rmsnorm_bf16_backward")
+        return dx, dw
+
+    def _block_operands(self, A8, scaleA, B8, scaleB, transB, swiglu, groups):
+        """Checks an e4m3 product with block scales; returns (M, N, K, A8, scaleA, B8, scaleB) as the library reads them."""
+        _want(A8, "A8", (_E4M3,), (None, None))
+        M, K = A8.shape
+        lead = () if groups is None else (groups,)
+        _want(B8, "B8", (_E4M3,), (*lead, None, K) if transB else (*lead, K, None))
+        rows, cols = B8.shape[-2:]
+        n = rows if transB else cols
+        if swiglu and n % 256:
+            raise O64Error(_lib.ERR_CONFORM, "swiglu: gate and up need a multiple of 128 rows each")
+        _want(scaleA, "scaleA", (_F32,), (M, -(-K // 128)))
+        _want(scaleB, "scaleB", (_F32,), (*lead, -(-rows // 128), -(-cols // 128)))
+        return M, n // 2 if swiglu else n, K, _tma(A8), _rows(scaleA), _tma(B8), _rows(scaleB)
+
+    def _swiglu_out(self, M, N, out_kind, out, scales, device):
+        if out_kind not in (_lib.OUT_BF16, _lib.OUT_E4M3):
+            raise O64Error(_lib.ERR_DTYPE, "swiglu")
+        dtype = _OUT_DTYPE[out_kind]
+        out = torch.empty((M, N), dtype=dtype, device=device) if out is None else _out(_want(out, "out", (dtype,), (M, N)), "out")
+        if out_kind == _lib.OUT_E4M3:
+            shape = (M, N // 128)
+            scales = torch.empty(shape, dtype=_F32, device=device) if scales is None else _out(_want(scales, "scales", (_F32,), shape), "scales")
+        elif scales is not None:
+            raise O64Error(_lib.ERR_DTYPE, "swiglu: scales of a bf16 result")
+        return out, scales
+
+    @staticmethod
+    def _bf16_out(out, M, N, device):
+        return torch.empty((M, N), dtype=_BF16, device=device) if out is None else _out(_want(out, "out", (_BF16,), (M, N)), "out")
+
+    @staticmethod
+    def _offsets(offsets, groups):
+        _want(offsets, "offsets", (torch.int32,), (groups + 1,))
+        return offsets.contiguous()
+
+    def gemm_fp8_block(self, A8, scaleA, B8, scaleB, transB=True, out=None):
+        """bf16 sum over blocks of 128 of K of scaleA[m,b] * scaleB[n/128,b] * (A8 @ B8^T in block b).  A8 [M,K],
+        scaleA [M, ceil(K/128)]; B8 [N,K] (or [K,N]: transB False), scaleB one value per 128 x 128 of B8."""
+        M, N, K, A8, scaleA, B8, scaleB = self._block_operands(A8, scaleA, B8, scaleB, transB, False, None)
+        out = self._bf16_out(out, M, N, A8.device)
+        check(self.lib.o64_gemm_fp8_block(self._h, M, N, K, A8.data_ptr(), _ld(A8), scaleA.data_ptr(), _ld(scaleA), B8.data_ptr(), _ld(B8),
+                                          1 if transB else 0, scaleB.data_ptr(), _ld(scaleB), out.data_ptr(), _ld(out), _stream(A8)),
+              "o64_gemm_fp8_block")
+        return out
+
+    def gemm_fp8_block_swiglu(self, A8, scaleA, B8, scaleB, out_kind=_lib.OUT_E4M3, out=None, scales=None):
+        """silu(gate) * up of the halves of a block-scaled product with B8 [2N,K] (gate rows, then up rows; N a
+        multiple of 128): (h [M,N], scales [M, N/128]) with h e4m3, or bf16 and None."""
+        M, N, K, A8, scaleA, B8, scaleB = self._block_operands(A8, scaleA, B8, scaleB, True, True, None)
+        out, scales = self._swiglu_out(M, N, out_kind, out, scales, A8.device)
+        check(self.lib.o64_gemm_fp8_block_swiglu(self._h, M, N, K, A8.data_ptr(), _ld(A8), scaleA.data_ptr(), _ld(scaleA), B8.data_ptr(),
+                                                 _ld(B8), scaleB.data_ptr(), _ld(scaleB), out.data_ptr(), _ld(out), out_kind,
+                                                 None if scales is None else scales.data_ptr(), 0 if scales is None else _ld(scales),
+                                                 _stream(A8)), "o64_gemm_fp8_block_swiglu")
+        return out, scales
+
+    def gemm_grouped_bf16(self, A, offsets, B, transB=True, out=None):
+        """A[rows of g] @ op(B[g]) for each group g: A [T,K] bf16 sorted by group, offsets int32 [G+1] on the
+        device, B [G,N,K] (or [G,K,N]: transB False).  Rows outside offsets[0] .. offsets[G] are left as they are."""
+        _want(A, "A", (_BF16,), (None, None))
+        T, K = A.shape
+        _want(B, "B", (_BF16,), (None, None, K) if transB else (None, K, None))
+        G, N = B.shape[0], B.shape[1] if transB else B.shape[2]
+        offsets = self._offsets(offsets, G)
+        A, B = _tma(A), _tma(B)
+        out = self._bf16_out(out, T, N, A.device)
+        check(self.lib.o64_gemm_grouped_bf16(self._h, G, T, N, K, A.data_ptr(), _ld(A), offsets.data_ptr(), B.data_ptr(), _ld(B), _stride0(B),
+                                             1 if transB else 0, out.data_ptr(), _ld(out), _stream(A)), "o64_gemm_grouped_bf16")
+        return out
+
+    def gemm_grouped_bf16_wgrad(self, dC, A, offsets, out_kind=_lib.OUT_BF16, out=None):
+        """dC[rows of g]^T @ A[rows of g] for each group: dC [T,N], A [T,K] bf16 -> [G,N,K] bf16 or (OUT_F32) fp32."""
+        _want(dC, "dC", (_BF16,), (None, None))
+        T, N = dC.shape
+        _want(A, "A", (_BF16,), (T, None))
+        K = A.shape[1]
+        if out_kind not in (_lib.OUT_BF16, _lib.OUT_F32):
+            raise O64Error(_lib.ERR_DTYPE, "gemm_grouped_bf16_wgrad")
+        _want(offsets, "offsets", (torch.int32,), (None,))
+        G = offsets.shape[0] - 1
+        if G < 0:
+            raise O64Error(_lib.ERR_CONFORM, "offsets: one more than groups")
+        offsets = offsets.contiguous()
+        dtype = _OUT_DTYPE[out_kind]
+        out = torch.empty((G, N, K), dtype=dtype, device=dC.device) if out is None else _out(_want(out, "out", (dtype,), (G, N, K)), "out")
+        dC, A = _tma(dC), _tma(A)
+        check(self.lib.o64_gemm_grouped_bf16_wgrad(self._h, G, T, N, K, dC.data_ptr(), _ld(dC), A.data_ptr(), _ld(A), offsets.data_ptr(),
+                                                   out.data_ptr(), _ld(out), _stride0(out), out_kind, _stream(dC)),
+              "o64_gemm_grouped_bf16_wgrad")
+        return out
+
+    def gemm_grouped_fp8_block(self, A8, scaleA, offsets, B8, scaleB, transB=True, out=None):
+        """gemm_fp8_block by group: A8 [T,K] sorted by group, B8 [G,N,K] (or [G,K,N]), scaleB one per 128 x 128."""
+        if B8.dim() != 3:
+            raise O64Error(_lib.ERR_RANK, f"B8: rank {B8.dim()}")
+        T, N, K, A8, scaleA, B8, scaleB = self._block_operands(A8, scaleA, B8, scaleB, transB, False, B8.shape[0])
+        offsets = self._offsets(offsets, B8.shape[0])
+        out = self._bf16_out(out, T, N, A8.device)
+        check(self.lib.o64_gemm_grouped_fp8_block(self._h, B8.shape[0], T, N, K, A8.data_ptr(), _ld(A8), scaleA.data_ptr(), _ld(scaleA),
+                                                  offsets.data_ptr(), B8.data_ptr(), _ld(B8), _stride0(B8), 1 if transB else 0,
+                                                  scaleB.data_ptr(), _ld(scaleB), _stride0(scaleB), out.data_ptr(), _ld(out), _stream(A8)),
+              "o64_gemm_grouped_fp8_block")
+        return out
+
+    def gemm_grouped_fp8_block_swiglu(self, A8, scaleA, offsets, B8, scaleB, out_kind=_lib.OUT_E4M3, out=None, scales=None):
+        """gemm_fp8_block_swiglu by group: B8 [G,2N,K]."""
+        if B8.dim() != 3:
+            raise O64Error(_lib.ERR_RANK, f"B8: rank {B8.dim()}")
+        T, N, K, A8, scaleA, B8, scaleB = self._block_operands(A8, scaleA, B8, scaleB, True, True, B8.shape[0])
+        offsets = self._offsets(offsets, B8.shape[0])
+        out, scales = self._swiglu_out(T, N, out_kind, out, scales, A8.device)
+        check(self.lib.o64_gemm_grouped_fp8_block_swiglu(self._h, B8.shape[0], T, N, K, A8.data_ptr(), _ld(A8), scaleA.data_ptr(),
+                                                         _ld(scaleA), offsets.data_ptr(), B8.data_ptr(), _ld(B8), _stride0(B8),
+                                                         scaleB.data_ptr(), _ld(scaleB), _stride0(scaleB), out.data_ptr(), _ld(out),
+                                                         out_kind, None if scales is None else scales.data_ptr(),
+                                                         0 if scales is None else _ld(scales), _stream(A8)),
+              "o64_gemm_grouped_fp8_block_swiglu")
+        return out, scales
+
+    def mlp_swiglu_fp8(self, x, norm_weight, W13, scale13, W2, scale2, residual=None, offsets=None, eps=1e-6):
+        """The 8-bit feed-forward block: norm(x + residual) in e4m3, silu(gate) * up in e4m3, down projection.
+        W13 [2F,D] and W2 [D,F] e4m3 with a scale per 128 x 128 - or [G,2F,D] and [G,D,F] with `offsets`,
+        rows of x sorted by expert.  Returns (out bf16, the stream after the addition)."""
+        a, sa, stream, _ = self.rms_norm(x, norm_weight, residual, eps, _lib.OUT_E4M3)
+        if offsets is None:
+            h, sh = self.gemm_fp8_block_swiglu(a, sa, W13, scale13)
+            return self.gemm_fp8_block(h, sh, W2, scale2), stream
+        h, sh = self.gemm_grouped_fp8_block_swiglu(a, sa, offsets, W13, scale13)
+        return self.gemm_grouped_fp8_block(h, sh, offsets, W2, scale2), stream
 
     def gemm_s8_scaled(self, A, B, scaleA=None, scaleB=None, bias=None, act="none", out_kind=_lib.OUT_BF16, out=None):
         """convert(act(float(A @ B^T) * sA[m] * sB[n] + bias[n])), int8 operands: bf16, or int8 again
