@@ -21,7 +21,7 @@ __host__ __device__ constexpr int gepi_bytes(int e) { return e == GEPI_F32 ? 4 :
 // Status-word codes.  0x6..: the group offsets in device memory are not ascending within 0 .. T.
 constexpr int kBadOffsets = 0x601;
 constexpr int kWaitGroupProducer = 0x701, kWaitGroupFull = 0x702, kWaitGroupAccEmpty = 0x703, kWaitGroupAccFull = 0x704,
-              kWaitGroupTail = 0x705, kWaitGroupHalf = 0x706;
+              kWaitGroupTail = 0x705, kWaitGroupHalf = 0x706, kWaitGroupScales = 0x707;
 
 // One call.  Rows T of A are sorted by group; offsets (device, G + 1 ints) bound the groups; NULL: one
 // group of T rows.  B is [G][N][K] (or [G][K][N]: b_kn), C is [T][N].  wgrad: A is dC [T][N], B is the
@@ -59,6 +59,7 @@ struct GroupedParams {
     long long ldsc;
     const int *offsets;
     int vec_ok, tma_store;
+    int sa_vec;  // the rows of scale_a are 16-byte aligned
     int *status;
     unsigned long long wait_ns;
 };

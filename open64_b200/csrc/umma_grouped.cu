@@ -19,7 +19,14 @@
 // the second the matching up columns).  One packed multiply-add serves two values: 64 of them a thread
 // and block against 512 cycles of MMA.
 //
-// Warp roles (320 threads a CTA): 0 loads, 1 issues the MMAs (first CTA of the pair), 2..9 add and store.
+// The scales reach the adding warps through a small ring in shared memory that a warp of its own fills four
+// K blocks ahead: fetched by each thread for itself two blocks ahead, they cost 600 to 800 cycles a block
+// (32 rows are 32 sectors, and the move from one pipeline register to the next waits for the load).
+//
+// Warp roles (three warpgroups a CTA): 0 loads, 1 issues the MMAs (first CTA of the pair), 2 fetches scales,
+// 4..11 add and store.
+// The sums take 128 registers of a thread and two chunks on their way from tensor memory 64 more, so the
+// first warpgroup gives its registers up (setmaxnreg: 128 x 56 + 256 x 224 = the 384 x 168 of the launch).
 // Every wait is bounded, as in the other kernels.
 #include <cstdio>
 #include <cstdlib>
@@ -31,15 +38,20 @@ namespace o64 {
 
 namespace {
 
-constexpr int kGpThreads = 320;
+constexpr int kGpThreads = 384;
+constexpr int kGpLoaderRegs = 56, kGpAdderRegs = 224;
+static_assert(128 * kGpLoaderRegs + 256 * kGpAdderRegs <= kGpThreads * 168, "registers of the launch");
 constexpr int kGpStages = 6;
 constexpr int kGpTileM = 256, kGpTileN = 256;
 constexpr int kGpStageBytes = 2 * kABytes;  // this CTA's 128 rows of A and its 128 of B
 constexpr int kGpRing = kGpStages * kGpStageBytes;
 constexpr int kGpStaging = kGpRing;                       // 8 warps x 4 KB
-constexpr int kGpAmax = kGpStaging + 8 * kEpiStagingBytesPerWarp;  // [2][128] floats
-constexpr int kGpBars = kGpAmax + 1024;
-constexpr int kGpNumBars = 2 * kGpStages + 9;
+constexpr int kGpScaleSlots = 3;
+constexpr int kGpScaleFloats = 132;  // this CTA's 128 rows, then the two column blocks
+constexpr int kGpScales = kGpStaging + 8 * kEpiStagingBytesPerWarp;
+constexpr int kGpBars = kGpScales + kGpScaleSlots * kGpScaleFloats * 4;
+constexpr int kGpNumBars = 2 * kGpStages + 9 + 2 * kGpScaleSlots;
+static_assert(kGpBars % 8 == 0, "barriers");
 constexpr int kGpTmemPtr = kGpBars + 8 * kGpNumBars;
 constexpr int kGpAbort = kGpTmemPtr + 4;
 constexpr int kGpTotal = kGpAbort + 4;
@@ -55,19 +67,19 @@ struct GroupTile {
 // The tile list, walked forward only.
 struct TileWalk {
     int g = 0;
-    long long base = 0;  // tiles before group g
+    int base = 0;  // tiles before group g
 };
 
 template <bool WGRAD>
-__device__ __forceinline__ bool next_tile(const GroupedParams &p, TileWalk &w, long long t, int block_k, GroupTile &tile) {
+__device__ __forceinline__ bool next_tile(const GroupedParams &p, TileWalk &w, int t, int block_k, GroupTile &tile) {
     for (; w.g < p.G; ++w.g) {
         group_rows(p, w.g, tile.begin, tile.end);
         const int rows = tile.end - tile.begin;
         const int mt = WGRAD ? p.num_m_tiles : (rows + kGpTileM - 1) / kGpTileM;
-        const long long tiles = (long long)mt * p.num_n_tiles;
+        const int tiles = mt * p.num_n_tiles;  // (the host has checked that all of them fit an int)
         if (t < w.base + tiles) {
             // bands of eight row tiles, rows fastest: a band's rows of A and one column block of B stay in L2
-            const int r = (int)(t - w.base);
+            const int r = t - w.base;
             const int per_band = 8 * p.num_n_tiles;
             const int band = r / per_band, in = r - band * per_band;
             const int height = min(mt - band * 8, 8);
@@ -117,6 +129,8 @@ grouped_pair_kernel(const __grid_constant__ CUtensorMap tm_a, const __grid_const
     auto acc_full_bar = [&](int b) { return bar_base + 8u * (2 * kGpStages + b); };
     auto acc_empty_bar = [&](int b) { return bar_base + 8u * (2 * kGpStages + 2 + b); };
     const uint32_t tail_bar = bar_base + 8u * (2 * kGpStages + 4);
+    auto scale_full_bar = [&](int s) { return bar_base + 8u * (2 * kGpStages + 9 + s); };
+    auto scale_empty_bar = [&](int s) { return bar_base + 8u * (2 * kGpStages + 9 + kGpScaleSlots + s); };
     auto half_bar = [&](int quarter) { return bar_base + 8u * (2 * kGpStages + 5 + quarter); };
     volatile uint32_t *tmem_ptr_smem = reinterpret_cast<volatile uint32_t *>(smem_gen + kGpTmemPtr);
     volatile int *abort_flag = reinterpret_cast<volatile int *>(smem_gen + kGpAbort);
@@ -137,6 +151,10 @@ grouped_pair_kernel(const __grid_constant__ CUtensorMap tm_a, const __grid_const
             mbar_init(acc_empty_bar(b), 16);  // eight warps in each CTA
         }
         mbar_init(tail_bar, 1);
+        for (int s = 0; s < kGpScaleSlots; ++s) {
+            mbar_init(scale_full_bar(s), 1);
+            mbar_init(scale_empty_bar(s), 8);
+        }
         for (int q = 0; q < 4; ++q) mbar_init(half_bar(q), 2);  // the two warps that share 32 rows
         *abort_flag = 0;
         fence_mbar_init();
@@ -148,7 +166,7 @@ grouped_pair_kernel(const __grid_constant__ CUtensorMap tm_a, const __grid_const
         tmem_alloc(smem_u32(smem_gen + kGpTmemPtr), kTmemCols);
         tmem_relinquish();
     }
-    if (p.offsets && blockIdx.x == 0 && warp == 9) {  // offsets that are not ascending within 0 .. T are reported
+    if (p.offsets && blockIdx.x == 0 && warp == 2) {  // offsets that are not ascending within 0 .. T are reported
         for (int g = lane; g < p.G; g += 32) {
             int b, e;
             bool bad;
@@ -166,6 +184,8 @@ grouped_pair_kernel(const __grid_constant__ CUtensorMap tm_a, const __grid_const
         *abort_flag = 1;
     }
 
+    if (warp < 4) {
+    asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kGpLoaderRegs));
     if (warp == 0) {
         // ------------------------------ loads (both CTAs) -----------------------------------
         const bool leader = elect_one();
@@ -174,7 +194,7 @@ grouped_pair_kernel(const __grid_constant__ CUtensorMap tm_a, const __grid_const
         bool ok = true;
         TileWalk walk;
         GroupTile t;
-        for (long long i = pair_id; ok && next_tile<WGRAD>(p, walk, i, kBlockK, t); i += num_pairs) {
+        for (int i = pair_id; ok && next_tile<WGRAD>(p, walk, i, kBlockK, t); i += num_pairs) {
             const int m0 = t.mb * kGpTileM + (int)rank * kBlockM;
             const int n0 = t.nb * kOutN;
             for (int kb = 0; kb < t.kbs; ++kb) {
@@ -250,8 +270,11 @@ grouped_pair_kernel(const __grid_constant__ CUtensorMap tm_a, const __grid_const
             constexpr uint32_t kBAdvance = kBMn ? (kMmaK * kRowBytes) >> 4 : 2;
             int stage = 0;
             uint32_t phase = 0;
-            long long uses = 0;  // accumulator buffers taken so far
+            uint32_t uses = 0;  // accumulator buffers taken so far
             bool ok = true;
+            // the next stage's barrier is probed before this stage's MMAs are issued, so that the probe's
+            // latency opens no gap between them
+            uint32_t ready = mbar_test_wait(full_bar(0), 0);
             TileWalk walk;
             GroupTile t;
             auto take = [&] {
@@ -260,16 +283,21 @@ grouped_pair_kernel(const __grid_constant__ CUtensorMap tm_a, const __grid_const
                 ok = __all_sync(0xffffffffu, ok);
                 tc_fence_after();
             };
-            for (long long i = pair_id; ok && next_tile<WGRAD>(p, walk, i, kBlockK, t); i += num_pairs) {
+            for (int i = pair_id; ok && next_tile<WGRAD>(p, walk, i, kBlockK, t); i += num_pairs) {
                 if (!kScaled && t.kbs > 0) take();
                 for (int kb = 0; ok && kb < t.kbs; ++kb) {
                     if (kScaled) {
                         take();
                         if (!ok) break;
                     }
-                    ok = mbar_wait_bounded(full_bar(stage), phase, abort_flag, p.status, kWaitGroupFull, p.wait_ns);
-                    ok = __all_sync(0xffffffffu, ok);
-                    if (!ok) break;
+                    if (!__all_sync(0xffffffffu, ready)) {
+                        ok = mbar_wait_bounded(full_bar(stage), phase, abort_flag, p.status, kWaitGroupFull, p.wait_ns);
+                        ok = __all_sync(0xffffffffu, ok);
+                        if (!ok) break;
+                    }
+                    const int next_stage = (stage + 1 == kGpStages) ? 0 : stage + 1;
+                    const uint32_t next_phase = (stage + 1 == kGpStages) ? (phase ^ 1u) : phase;
+                    const uint32_t next_ready = mbar_test_wait(full_bar(next_stage), next_phase);
                     tc_fence_after();
                     const uint32_t a_addr = smem_base + stage * kGpStageBytes;
                     const uint32_t b_addr = a_addr + kABytes;
@@ -289,10 +317,9 @@ grouped_pair_kernel(const __grid_constant__ CUtensorMap tm_a, const __grid_const
                     }
                     __syncwarp();
                     if (kScaled) ++uses;
-                    if (++stage == kGpStages) {
-                        stage = 0;
-                        phase ^= 1u;
-                    }
+                    stage = next_stage;
+                    phase = next_phase;
+                    ready = next_ready;
                 }
                 if (!kScaled && t.kbs > 0) {
                     if (ok && leader) tc_commit_pair_mask(acc_full_bar(uses & 1), 3);
@@ -302,20 +329,86 @@ grouped_pair_kernel(const __grid_constant__ CUtensorMap tm_a, const __grid_const
             }
         }
         __syncwarp();
+    } else if (kScaled && warp == 2) {
+        // ------------------------------ scales (both CTAs) ----------------------------------
+        float *ring = reinterpret_cast<float *>(smem_gen + kGpScales);
+        int slot = 0;
+        uint32_t phase = 0;
+        bool ok = true;
+        TileWalk walk;
+        GroupTile t;
+        for (int i = pair_id; ok && next_tile<WGRAD>(p, walk, i, kBlockK, t); i += num_pairs) {
+            // lane l carries rows l, l + 32, l + 64, l + 96 and, for l < 2, one of the two runs of columns
+            const int n0 = t.nb * kOutN;
+            const float *sa[4];
+#pragma unroll
+            for (int r = 0; r < 4; ++r)
+                sa[r] = p.scale_a + (long long)min(t.begin + t.mb * kGpTileM + (int)rank * kBlockM + r * 32 + lane, t.end - 1) * p.ldsa;
+            // the block of 128 columns of C (SwiGLU: of gate, or of up) behind run `lane`
+            const int blk = kSwiglu ? ((lane & 1 ? p.N + n0 : n0) >> 7) : min((n0 >> 7) + (lane & 1), (p.N - 1) >> 7);
+            const float *sb = p.scale_b + (long long)t.g * p.stride_sb + (B_KN ? (long long)blk : blk * p.ldsb);
+            const long long sb_step = B_KN ? p.ldsb : 1;
+            float next[5][4];
+            auto fetch = [&](int kb) __attribute__((always_inline)) {
+#pragma unroll
+                for (int r = 0; r < 4; ++r) {
+                    if (p.sa_vec && kb + 4 <= t.kbs) {
+                        const float4 x = __ldg(reinterpret_cast<const float4 *>(sa[r] + kb));
+                        next[r][0] = x.x, next[r][1] = x.y, next[r][2] = x.z, next[r][3] = x.w;
+                    } else {
+#pragma unroll
+                        for (int u = 0; u < 4; ++u) next[r][u] = kb + u < t.kbs ? __ldg(sa[r] + kb + u) : 0.0f;
+                    }
+                }
+#pragma unroll
+                for (int u = 0; u < 4; ++u) next[4][u] = lane < 2 && kb + u < t.kbs ? __ldg(sb + (kb + u) * sb_step) : 0.0f;
+            };
+            fetch(0);
+#pragma unroll 1
+            for (int kb0 = 0; ok && kb0 < t.kbs; kb0 += 4) {
+                float now[5][4];
+#pragma unroll
+                for (int r = 0; r < 5; ++r)
+#pragma unroll
+                    for (int u = 0; u < 4; ++u) now[r][u] = next[r][u];
+                fetch(kb0 + 4);
+#pragma unroll
+                for (int u = 0; u < 4; ++u) {
+                    if (kb0 + u >= t.kbs) break;
+                    ok = mbar_wait_bounded(scale_empty_bar(slot), phase ^ 1u, abort_flag, p.status, kWaitGroupScales, p.wait_ns);
+                    ok = __all_sync(0xffffffffu, ok);
+                    if (!ok) break;
+                    float *dst = ring + slot * kGpScaleFloats;
+#pragma unroll
+                    for (int r = 0; r < 4; ++r) dst[r * 32 + lane] = now[r][u];
+                    if (lane < 2) dst[128 + lane] = now[4][u];
+                    __syncwarp();
+                    if (lane == 0) mbar_arrive(scale_full_bar(slot));
+                    if (++slot == kGpScaleSlots) {
+                        slot = 0;
+                        phase ^= 1u;
+                    }
+                }
+            }
+        }
+        __syncwarp();
+    }
     } else {
+        asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(kGpAdderRegs));
         // ------------------------------ sums, tails and stores (both CTAs) ------------------
         const int quarter = warp & 3;
-        const int half = (warp - 2) >> 2;
-        uint8_t *staging = smem_gen + kGpStaging + (warp - 2) * kEpiStagingBytesPerWarp;
+        const int half = (warp - 4) >> 2;
+        uint8_t *staging = smem_gen + kGpStaging + (warp - 4) * kEpiStagingBytesPerWarp;
         uint4 *patch = reinterpret_cast<uint4 *>(staging);
         const int sw = lane & 7;
         const uint32_t t_lane = tmem_base + (uint32_t(quarter * 32) << 16) + half * 64;
-        long long uses = 0;
+        uint32_t uses = 0;
         bool ok = true;
-        [[maybe_unused]] uint32_t half_phase = 0;
+        [[maybe_unused]] uint32_t half_phase = 0, slot_phase = 0;
+        [[maybe_unused]] int slot = 0;
         TileWalk walk;
         GroupTile t;
-        for (long long i = pair_id; ok && next_tile<WGRAD>(p, walk, i, kBlockK, t); i += num_pairs) {
+        for (int i = pair_id; ok && next_tile<WGRAD>(p, walk, i, kBlockK, t); i += num_pairs) {
             const int n0 = t.nb * kOutN;
             const int slab0 = t.mb * kGpTileM + (int)rank * kBlockM + quarter * 32;  // of the group's rows (or of dB's)
             float2 acc[2][32];
@@ -325,49 +418,46 @@ grouped_pair_kernel(const __grid_constant__ CUtensorMap tm_a, const __grid_const
                 for (int j = 0; j < 32; ++j) acc[r][j] = make_float2(0.0f, 0.0f);
 
             if constexpr (kScaled) {
-                // this thread's row of A, and the two columns blocks of B
-                const long long arow = min(t.begin + slab0 + lane, t.end - 1);
-                const float *sa = p.scale_a + arow * p.ldsa;
-                const int nblk0 = B_KN ? 0 : (n0 >> 7), nblk1 = kSwiglu ? ((p.N + n0) >> 7) : nblk0 + 1;
-                const int last_blk = (p.N - 1) >> 7;
-                const float *sbg = p.scale_b + (long long)t.g * p.stride_sb;
-                // [N,K] weights: one row of scales per 128 columns of C; [K,N]: one column of them
-                const float *sb0 = B_KN ? sbg + (n0 >> 7) : sbg + (long long)nblk0 * p.ldsb;
-                const float *sb1 = B_KN ? sbg + min((n0 >> 7) + 1, last_blk)
-                                        : sbg + (long long)(kSwiglu ? nblk1 : min(nblk1, last_blk)) * p.ldsb;
-                const long long sb_step = B_KN ? p.ldsb : 1;
-                float a_next = 0.0f, b0_next = 0.0f, b1_next = 0.0f;
-                if (t.kbs > 0) a_next = __ldg(sa), b0_next = __ldg(sb0), b1_next = __ldg(sb1);
+                const float *ring = reinterpret_cast<const float *>(smem_gen + kGpScales);
+#pragma unroll 1
                 for (int kb = 0; kb < t.kbs; ++kb, ++uses) {
-                    const float s0 = a_next * b0_next, s1 = a_next * b1_next;
-                    if (kb + 1 < t.kbs) {
-                        a_next = __ldg(sa + kb + 1);
-                        b0_next = __ldg(sb0 + (kb + 1) * sb_step);
-                        b1_next = __ldg(sb1 + (kb + 1) * sb_step);
-                    }
                     if (lane == 0)
-                        ok = mbar_wait_bounded(acc_full_bar(uses & 1), (uint32_t)((uses >> 1) & 1), abort_flag, p.status,
+                        ok = mbar_wait_bounded(scale_full_bar(slot), slot_phase, abort_flag, p.status, kWaitGroupScales, p.wait_ns) &&
+                             mbar_wait_bounded(acc_full_bar(uses & 1), (uint32_t)((uses >> 1) & 1), abort_flag, p.status,
                                                kWaitGroupAccFull, p.wait_ns);
                     ok = __shfl_sync(0xffffffffu, ok, 0);
                     if (!ok) break;
                     tc_fence_after();
                     const uint32_t t_row = t_lane + (uint32_t)(uses & 1) * kGpTileN;
-#pragma unroll
-                    for (int c = 0; c < 4; ++c) {
-                        uint32_t v[32];
-                        tmem_ld_32x32(t_row + (c >> 1) * 128 + (c & 1) * 32, v);
-                        tmem_ld_wait();
-                        if (c == 3) {  // everything of this buffer is in registers
-                            tc_fence_before();
-                            __syncwarp();
-                            if (lane == 0) mbar_arrive_cluster(map_to_cta(acc_empty_bar(uses & 1), 0));
-                        }
-                        const float s = (c >> 1) ? s1 : s0;
+                    // 64 columns at a time; the second 64 set out as soon as the registers of the first are free
+                    uint32_t va[32], vb[32];
+                    tmem_ld_32x32(t_row, va);
+                    tmem_ld_32x32(t_row + 32, vb);
+                    const float s = ring[slot * kGpScaleFloats + quarter * 32 + lane];
+                    const float2 sb = *reinterpret_cast<const float2 *>(ring + slot * kGpScaleFloats + 128);
+                    auto add = [&](const uint32_t(&v)[32], float2(&sum)[32], int at, float f) __attribute__((always_inline)) {
 #pragma unroll
                         for (int j = 0; j < 16; ++j)
-                            acc[c >> 1][(c & 1) * 16 + j] =
-                                __ffma2_rn(make_float2(__uint_as_float(v[2 * j]), __uint_as_float(v[2 * j + 1])), make_float2(s, s),
-                                           acc[c >> 1][(c & 1) * 16 + j]);
+                            sum[at + j] = __ffma2_rn(make_float2(__uint_as_float(v[2 * j]), __uint_as_float(v[2 * j + 1])),
+                                                     make_float2(f, f), sum[at + j]);
+                    };
+                    tmem_ld_wait();
+                    add(va, acc[0], 0, s * sb.x);
+                    tmem_ld_32x32(t_row + 128, va);
+                    add(vb, acc[0], 16, s * sb.x);
+                    tmem_ld_32x32(t_row + 160, vb);
+                    tmem_ld_wait();
+                    tc_fence_before();  // everything of this buffer is in registers
+                    __syncwarp();
+                    if (lane == 0) {
+                        mbar_arrive_cluster(map_to_cta(acc_empty_bar(uses & 1), 0));
+                        mbar_arrive(scale_empty_bar(slot));
+                    }
+                    add(va, acc[1], 0, s * sb.y);
+                    add(vb, acc[1], 16, s * sb.y);
+                    if (++slot == kGpScaleSlots) {
+                        slot = 0;
+                        slot_phase ^= 1u;
                     }
                 }
             } else if (t.kbs > 0) {
@@ -400,13 +490,13 @@ grouped_pair_kernel(const __grid_constant__ CUtensorMap tm_a, const __grid_const
             constexpr int kOutElem = gepi_bytes(EPI);
             uint8_t *c_group = static_cast<uint8_t *>(p.C) + (WGRAD ? (long long)t.g * p.stride_c * kOutElem : 0);
             // sends the patch out: `cols` result columns from column `col` on, kOutElem bytes each
-            auto send = [&](int col, int cols) {
+            auto send = [&](int col, int cols) __attribute__((always_inline)) {
                 const int bytes = cols * kOutElem;
                 if (p.tma_store && bytes == 128 && rows_here >= 32 && col + cols <= p.N) {
                     fence_proxy_async_smem();
                     __syncwarp();
                     if (lane == 0) {
-                        tma_store_3d(&tm_c, smem_base + kGpStaging + (warp - 2) * kEpiStagingBytesPerWarp, col * kOutElem, (int)grow0,
+                        tma_store_3d(&tm_c, smem_base + kGpStaging + (warp - 4) * kEpiStagingBytesPerWarp, col * kOutElem, (int)grow0,
                                      WGRAD ? t.g : 0);
                         bulk_commit_group();
                     }
@@ -446,7 +536,6 @@ grouped_pair_kernel(const __grid_constant__ CUtensorMap tm_a, const __grid_const
                 }
             };
             if constexpr (EPI == GEPI_SWIGLU_E4M3) {
-                float *amax_all = reinterpret_cast<float *>(smem_gen + kGpAmax);
                 // the two warps that share these rows (a bounded wait like all others: no named barrier)
                 auto meet = [&] {
                     __syncwarp();
@@ -466,16 +555,16 @@ grouped_pair_kernel(const __grid_constant__ CUtensorMap tm_a, const __grid_const
                     amax = fmax_nan(amax, fmax_nan(fabsf(h.x), fabsf(h.y)));
                 }
                 // the row's other 64 columns are with the warp of the other half
-                amax_all[half * 128 + quarter * 32 + lane] = amax;
+                patch_free();
+                reinterpret_cast<float *>(patch)[lane] = amax;
                 meet();
                 if (!ok) break;
-                amax = fmax_nan(amax, amax_all[(half ^ 1) * 128 + quarter * 32 + lane]);
-                meet();  // read before the next tile writes it
+                amax = fmax_nan(amax, reinterpret_cast<const float *>(smem_gen + kGpStaging + ((half ^ 1) * 4 + (warp & 3)) * kEpiStagingBytesPerWarp)[lane]);
+                meet();  // read before the values overwrite it
                 if (!ok) break;
                 const float scale = block_scale_of(amax);
                 if (half == 0 && lane < rows_here) p.scale_c[(grow0 + lane) * p.ldsc + t.nb] = scale;
                 const float inv = 1.0f / scale;
-                patch_free();
 #pragma unroll
                 for (int q = 0; q < 4; ++q) {
                     uint32_t w[4];
@@ -572,6 +661,7 @@ static GroupedParams grouped_params(const GroupedCall &c) {
     const int elem = gepi_bytes(c.epi);
     p.vec_ok = (reinterpret_cast<uintptr_t>(c.C) & 15u) == 0 && (c.ldc * elem) % 16 == 0 && (c.stride_c * elem) % 16 == 0;
     p.tma_store = 0;
+    p.sa_vec = (reinterpret_cast<uintptr_t>(c.scale_a) & 15u) == 0 && c.ldsa % 4 == 0;
     p.num_m_tiles = (int)((c.N + kGpTileM - 1) / kGpTileM);
     const int out_n = gepi_swiglu(c.epi) ? kGpTileN / 2 : kGpTileN;
     p.num_n_tiles = (int)((p.N + out_n - 1) / out_n);
@@ -603,6 +693,7 @@ static int launch_grouped(const CUtensorMap &ta, const CUtensorMap &tb, const CU
     // one pair per two SMs; no more than there can be tiles
     const long long most = WGRAD ? (long long)p.G * p.num_m_tiles * p.num_n_tiles
                                  : ((long long)p.T / kGpTileM + (p.G < p.T ? p.G : p.T)) * p.num_n_tiles;
+    if (most > INT32_MAX - num_sms) return O64_ERR_RANK;  // the walk counts tiles in 32 bits
     const int pairs = (int)(most < num_sms / 2 ? (most < 1 ? 1 : most) : num_sms / 2);
     kern<<<2 * pairs, kGpThreads, kGpDynamic, stream>>>(ta, tb, tc, p);
     return cudaGetLastError() == cudaSuccess ? O64_OK : O64_ERR_CUDA;
