@@ -890,7 +890,7 @@ static int grouped_entry(o64_handle_t h, GroupedCall c, void *stream) {
         if (c.G > 1 && (c.stride_b * elem) % 16) return O64_ERR_ALIGN;
     }
     if (!tma_aligned(c.A, c.lda, elem) || !tma_aligned(c.B, c.ldb, elem)) return O64_ERR_ALIGN;
-    return grouped_pair_launch(c);
+    return grouped_launch(c);
 }
 
 static GroupedCall grouped_call(int kind, int epi, int64_t G, int64_t T, int64_t N, int64_t K, const void *A, int64_t lda,

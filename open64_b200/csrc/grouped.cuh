@@ -59,6 +59,7 @@ struct GroupedParams {
     long long ldsc;
     const int *offsets;
     int vec_ok, tma_store;
+    int split;   // few rows: CTAs that share a tile's K blocks
     int sa_vec;  // the rows of scale_a are 16-byte aligned
     int *status;
     unsigned long long wait_ns;
@@ -77,7 +78,10 @@ __device__ __forceinline__ void group_rows(const GroupedParams &p, int g, int &b
     if (bad) *bad = a < 0 || b < a || b > p.T;
 }
 
-int grouped_pair_launch(const GroupedCall &c);
+int grouped_launch(const GroupedCall &c);
+// Few rows a group (weights [N,K]): the kernel that reads every weight once for them.
+bool grouped_rows_fits(const GroupedCall &c);
+int grouped_rows_launch(const GroupedCall &c, const GroupedParams &p);
 // Sets the rows of the groups (wgrad: every C) to the empty sum: K == 0, or a weight gradient over no rows.
 int grouped_zero_launch(const GroupedCall &c);
 
@@ -90,11 +94,10 @@ __device__ __forceinline__ void tma_load_3d_pair(uint32_t smem_dst, const void *
         "[%0], [%1, {%2, %3, %4}], [%5];" ::"r"(smem_dst), "l"(tmap), "r"(x), "r"(y), "r"(z), "r"(bar)
         : "memory");
 }
-__device__ __forceinline__ void tma_load_3d_hint(uint32_t smem_dst, const void *tmap, int x, int y, int z, uint32_t bar,
-                                                 uint64_t policy) {
+__device__ __forceinline__ void tma_load_3d(uint32_t smem_dst, const void *tmap, int x, int y, int z, uint32_t bar) {
     asm volatile(
-        "cp.async.bulk.tensor.3d.shared::cluster.global.mbarrier::complete_tx::bytes.L2::cache_hint "
-        "[%0], [%1, {%2, %3, %4}], [%5], %6;" ::"r"(smem_dst), "l"(tmap), "r"(x), "r"(y), "r"(z), "r"(bar), "l"(policy)
+        "cp.async.bulk.tensor.3d.shared::cluster.global.mbarrier::complete_tx::bytes "
+        "[%0], [%1, {%2, %3, %4}], [%5];" ::"r"(smem_dst), "l"(tmap), "r"(x), "r"(y), "r"(z), "r"(bar)
         : "memory");
 }
 __device__ __forceinline__ void tma_store_3d(const void *tmap, uint32_t smem_src, int x, int y, int z) {

@@ -661,6 +661,7 @@ static GroupedParams grouped_params(const GroupedCall &c) {
     const int elem = gepi_bytes(c.epi);
     p.vec_ok = (reinterpret_cast<uintptr_t>(c.C) & 15u) == 0 && (c.ldc * elem) % 16 == 0 && (c.stride_c * elem) % 16 == 0;
     p.tma_store = 0;
+    p.split = 1;
     p.sa_vec = (reinterpret_cast<uintptr_t>(c.scale_a) & 15u) == 0 && c.ldsa % 4 == 0;
     p.num_m_tiles = (int)((c.N + kGpTileM - 1) / kGpTileM);
     const int out_n = gepi_swiglu(c.epi) ? kGpTileN / 2 : kGpTileN;
@@ -699,8 +700,9 @@ static int launch_grouped(const CUtensorMap &ta, const CUtensorMap &tb, const CU
     return cudaGetLastError() == cudaSuccess ? O64_OK : O64_ERR_CUDA;
 }
 
-int grouped_pair_launch(const GroupedCall &c) {
+int grouped_launch(const GroupedCall &c) {
     GroupedParams p = grouped_params(c);
+    if (grouped_rows_fits(c)) return grouped_rows_launch(c, p);
     const int elem = c.kind == O64_KIND_BF16 ? 2 : 1;
     const int block_k = kRowBytes / elem;
     CUtensorMap ta, tb, tc;

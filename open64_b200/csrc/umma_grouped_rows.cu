@@ -1,0 +1,582 @@
+// Products grouped by expert, and the block-scaled e4m3 product, for few rows: every weight is read once
+// for a handful of rows of A, so the weights' way from HBM is all that counts.
+//
+// The operands change places: 128 rows of a weight are the MMA's M and the rows of A its N (16, 32 or 64),
+// so that nothing is spent on rows that are not there - shared memory, TMEM reads and sums go by 16 rows, not
+// by 128 - and the ring holds nearly 200 KB of weights on their way per SM.  A thread then owns one column
+// of C (one weight row) and all rows of the tile.  With the SwiGLU tail a tile is 128 gate and the 128
+// matching up rows: two accumulators, joined through shared memory.
+//
+// Tiles go group by group, a group's row tiles next to each other (they share the weight block in L2).  When
+// there are too few of them to fill the GPU, a cluster of S CTAs divides a tile's K blocks; the partial sums
+// meet in distributed shared memory and are added in rank order, each CTA finishing its share of the rows.
+//
+// Warps: 0 loads, 1 issues the MMAs, 2 fetches scales, 4.. add (four for each weight block).  Launched so that
+// its set-up overlaps the previous kernel of the stream (it waits before it touches memory).
+#include <cstdio>
+#include <cstdlib>
+#include <cstring>
+
+#include "grouped.cuh"
+
+namespace o64 {
+
+namespace {
+
+constexpr int kGrBufs = 4;  // accumulator buffers
+constexpr int kGrScaleSlots = 8;
+
+template <int NB, int TOK>
+struct RowsLayout {
+    static constexpr int kWBytes = NB * 128 * kRowBytes;
+    static constexpr int kXBytes = TOK * kRowBytes;
+    static constexpr int kStageBytes = kWBytes + kXBytes;
+    static constexpr int kXchBytes = NB == 2 ? TOK * 128 * 4 : 0;  // up values on their way to the gate warps
+    static constexpr int kRoom = 200 * 1024 - kXchBytes;
+    static constexpr int kStages = kRoom / kStageBytes > 12 ? 12 : kRoom / kStageBytes;
+    static constexpr int kRing = kStages * kStageBytes;
+    static constexpr int kXch = kRing;
+    static constexpr int kScales = kXch + kXchBytes;  // [slot][NB][TOK]
+    static constexpr int kAmax = kScales + kGrScaleSlots * NB * TOK * 4;  // [2][4][TOK]
+    static constexpr int kBars = kAmax + 2 * 4 * TOK * 4;
+    static constexpr int kNumBars = 2 * kStages + 2 * kGrBufs + 2 * kGrScaleSlots + 9;
+    static constexpr int kTmemPtr = kBars + 8 * kNumBars;
+    static constexpr int kAbort = kTmemPtr + 4;
+    static constexpr int kDynamic = kAbort + 4 + 1024;
+    static constexpr int kThreads = 128 + 128 * NB;
+    static constexpr uint32_t kTmemCols = kGrBufs * NB * TOK;
+    static_assert(kDynamic <= 227 * 1024, "shared memory");
+    static_assert(kStageBytes % 1024 == 0 && kWBytes % 1024 == 0, "swizzle atoms");
+    static_assert(kRing >= 128 * NB * TOK * 4, "the ring receives the partial sums");
+    static_assert(kTmemCols <= 512 && (kTmemCols & (kTmemCols - 1)) == 0 && kTmemCols >= 32, "TMEM columns");
+};
+
+struct RowsTile {
+    int g, begin, end;  // rows of this tile: [begin, end), at most TOK
+    int nb;
+};
+
+struct RowsWalk {
+    int g = 0;
+    int base = 0;
+};
+
+template <int TOK>
+__device__ __forceinline__ bool next_rows_tile(const GroupedParams &p, RowsWalk &w, int t, RowsTile &tile) {
+    for (; w.g < p.G; ++w.g) {
+        int begin, end;
+        group_rows(p, w.g, begin, end);
+        const int tt = (end - begin + TOK - 1) / TOK;
+        const int tiles = tt * p.num_n_tiles;
+        if (t < w.base + tiles) {
+            const int r = t - w.base;
+            tile.g = w.g;
+            tile.begin = begin + (r % tt) * TOK;
+            tile.end = min(tile.begin + TOK, end);
+            tile.nb = r / tt;
+            return true;
+        }
+        w.base += tiles;
+    }
+    return false;
+}
+
+__device__ __forceinline__ void st_cluster_f32(uint32_t addr, float v) {
+    asm volatile("st.shared::cluster.f32 [%0], %1;" ::"r"(addr), "f"(v) : "memory");
+}
+
+}  // namespace
+
+// p.num_n_tiles counts blocks of 128 columns of C; p.split: CTAs a cluster (> 1: one tile per cluster).
+template <int KIND, int EPI, int TOK>
+__global__ void __launch_bounds__(RowsLayout<gepi_swiglu(EPI) ? 2 : 1, TOK>::kThreads, 1)
+grouped_rows_kernel(const __grid_constant__ CUtensorMap tm_x, const __grid_constant__ CUtensorMap tm_w,
+                    const __grid_constant__ GroupedParams p) {
+    constexpr bool kSwiglu = gepi_swiglu(EPI);
+    constexpr int NB = kSwiglu ? 2 : 1;
+    using L = RowsLayout<NB, TOK>;
+    constexpr bool kScaled = KIND == MMA_F8F6F4;
+    constexpr int kBlockK = kRowBytes / (KIND == MMA_F16 ? 2 : 1);
+
+    extern __shared__ uint8_t smem_raw[];
+    const uint32_t smem_base = (smem_u32(smem_raw) + 1023u) & ~1023u;
+    uint8_t *smem_gen = smem_raw + (smem_base - smem_u32(smem_raw));
+    const uint32_t bar_base = smem_base + L::kBars;
+    auto full_bar = [&](int s) { return bar_base + 8u * s; };
+    auto empty_bar = [&](int s) { return bar_base + 8u * (L::kStages + s); };
+    auto acc_full_bar = [&](int b) { return bar_base + 8u * (2 * L::kStages + b); };
+    auto acc_empty_bar = [&](int b) { return bar_base + 8u * (2 * L::kStages + kGrBufs + b); };
+    auto scale_full_bar = [&](int s) { return bar_base + 8u * (2 * L::kStages + 2 * kGrBufs + s); };
+    auto scale_empty_bar = [&](int s) { return bar_base + 8u * (2 * L::kStages + 2 * kGrBufs + kGrScaleSlots + s); };
+    const uint32_t extra = bar_base + 8u * (2 * L::kStages + 2 * kGrBufs + 2 * kGrScaleSlots);
+    auto up_full_bar = [&](int q) { return extra + 8u * q; };
+    auto up_empty_bar = [&](int q) { return extra + 8u * (4 + q); };
+    const uint32_t amax_bar = extra + 8u * 8;
+    volatile uint32_t *tmem_ptr_smem = reinterpret_cast<volatile uint32_t *>(smem_gen + L::kTmemPtr);
+    volatile int *abort_flag = reinterpret_cast<volatile int *>(smem_gen + L::kAbort);
+
+    const int warp = threadIdx.x >> 5;
+    const int lane = threadIdx.x & 31;
+    const int S = p.split;
+    const int rank = S > 1 ? (int)cluster_ctarank() : 0;
+    const int first = S > 1 ? (int)(blockIdx.x / S) : (int)blockIdx.x;
+    const int step = S > 1 ? (int)(gridDim.x / S) : (int)gridDim.x;
+    const int kb_begin = (int)((long long)p.num_k_blocks * rank / S);
+    const int kb_end = (int)((long long)p.num_k_blocks * (rank + 1) / S);
+
+    griddep_launch_dependents();
+    if (threadIdx.x == 0) {
+        for (int s = 0; s < L::kStages; ++s) {
+            mbar_init(full_bar(s), 1);
+            mbar_init(empty_bar(s), 1);
+        }
+        for (int b = 0; b < kGrBufs; ++b) {
+            mbar_init(acc_full_bar(b), 1);
+            mbar_init(acc_empty_bar(b), 4 * NB);
+        }
+        for (int s = 0; s < kGrScaleSlots; ++s) {
+            mbar_init(scale_full_bar(s), 1);
+            mbar_init(scale_empty_bar(s), 4 * NB);
+        }
+        for (int q = 0; q < 4; ++q) {
+            mbar_init(up_full_bar(q), 1);
+            mbar_init(up_empty_bar(q), 1);
+        }
+        mbar_init(amax_bar, 4);
+        *abort_flag = 0;
+        fence_mbar_init();
+        tma_prefetch_desc(&tm_x);
+        tma_prefetch_desc(&tm_w);
+    }
+    if (warp == 1) {
+        tmem_alloc(smem_u32(smem_gen + L::kTmemPtr), L::kTmemCols);
+        tmem_relinquish();
+    }
+    tc_fence_before();
+    __syncthreads();
+    tc_fence_after();
+    const uint32_t tmem_base = *tmem_ptr_smem;
+    griddep_wait();
+    if (p.offsets && blockIdx.x == 0 && warp == 3) {  // offsets that are not ascending within 0 .. T are reported
+        for (int g = lane; g < p.G; g += 32) {
+            int b, e;
+            bool bad;
+            group_rows(p, g, b, e, &bad);
+            if (bad) atomicCAS(p.status, 0, kBadOffsets);
+        }
+    }
+
+    float2 acc[TOK / 2];
+    RowsTile last;  // split: the one tile of this cluster
+    bool have = false;
+
+    if (warp == 0) {
+        // ------------------------------ loads -------------------------------------------
+        const bool leader = elect_one();
+        int stage = 0;
+        uint32_t phase = 0;
+        bool ok = true;
+        RowsWalk walk;
+        RowsTile t;
+        for (int i = first; ok && next_rows_tile<TOK>(p, walk, i, t); i += step) {
+            for (int kb = kb_begin; kb < kb_end; ++kb) {
+                ok = mbar_wait_bounded(empty_bar(stage), phase ^ 1u, abort_flag, p.status, kWaitGroupProducer, p.wait_ns);
+                ok = __all_sync(0xffffffffu, ok);
+                if (!ok) break;
+                if (leader) {
+                    const uint32_t w_dst = smem_base + stage * L::kStageBytes;
+                    mbar_arrive_expect_tx(full_bar(stage), L::kStageBytes);
+#pragma unroll
+                    for (int b = 0; b < NB; ++b)
+                        tma_load_3d(w_dst + b * 128 * kRowBytes, &tm_w, kb * kBlockK, t.nb * 128 + b * p.N, t.g, full_bar(stage));
+                    tma_load_2d(w_dst + L::kWBytes, &tm_x, kb * kBlockK, t.begin, full_bar(stage));
+                }
+                __syncwarp();
+                if (++stage == L::kStages) {
+                    stage = 0;
+                    phase ^= 1u;
+                }
+            }
+        }
+        __syncwarp();
+    } else if (warp == 1) {
+        // ------------------------------ MMA ---------------------------------------------
+        const bool leader = elect_one();
+        constexpr uint32_t fmt = KIND == MMA_F8F6F4 ? 0u : 1u;
+        constexpr uint32_t idesc = make_idesc(1u, fmt, fmt, 0u, 128, TOK);
+        int stage = 0;
+        uint32_t phase = 0, uses = 0;
+        bool ok = true;
+        RowsWalk walk;
+        RowsTile t;
+        auto take = [&] {
+            ok = mbar_wait_bounded(acc_empty_bar(uses % kGrBufs), ((uses / kGrBufs) & 1) ^ 1u, abort_flag, p.status, kWaitGroupAccEmpty,
+                                   p.wait_ns);
+            ok = __all_sync(0xffffffffu, ok);
+            tc_fence_after();
+        };
+        for (int i = first; ok && next_rows_tile<TOK>(p, walk, i, t); i += step) {
+            if (kb_begin == kb_end) continue;
+            if (!kScaled) take();
+            for (int kb = kb_begin; ok && kb < kb_end; ++kb) {
+                if (kScaled) {
+                    take();
+                    if (!ok) break;
+                }
+                ok = mbar_wait_bounded(full_bar(stage), phase, abort_flag, p.status, kWaitGroupFull, p.wait_ns);
+                ok = __all_sync(0xffffffffu, ok);
+                if (!ok) break;
+                tc_fence_after();
+                const uint32_t w_addr = smem_base + stage * L::kStageBytes;
+                const uint64_t x_desc = make_smem_desc(w_addr + L::kWBytes, 16, 1024);
+                const uint32_t d = tmem_base + (uses % kGrBufs) * NB * TOK;
+                if (leader) {
+#pragma unroll
+                    for (int b = 0; b < NB; ++b) {
+                        const uint64_t w_desc = make_smem_desc(w_addr + b * 128 * kRowBytes, 16, 1024);
+#pragma unroll
+                        for (int k = 0; k < kRowBytes / 32; ++k)
+                            tc_mma<KIND>(d + b * TOK, w_desc + 2u * k, x_desc + 2u * k, idesc,
+                                         (kScaled ? k : ((kb - kb_begin) | k)) != 0 ? 1u : 0u);
+                    }
+                    tc_commit(empty_bar(stage));
+                    if (kScaled) tc_commit(acc_full_bar(uses % kGrBufs));
+                }
+                __syncwarp();
+                if (kScaled) ++uses;
+                if (++stage == L::kStages) {
+                    stage = 0;
+                    phase ^= 1u;
+                }
+            }
+            if (!kScaled) {
+                if (ok && leader) tc_commit(acc_full_bar(uses % kGrBufs));
+                __syncwarp();
+                ++uses;
+            }
+        }
+        __syncwarp();
+    } else if (kScaled && warp == 2) {
+        // ------------------------------ scales ------------------------------------------
+        float *ring = reinterpret_cast<float *>(smem_gen + L::kScales);
+        constexpr int kPer = (TOK + 31) / 32;  // rows a lane carries
+        int slot = 0;
+        uint32_t phase = 0;
+        bool ok = true;
+        RowsWalk walk;
+        RowsTile t;
+        for (int i = first; ok && next_rows_tile<TOK>(p, walk, i, t); i += step) {
+            const float *sa[kPer];
+#pragma unroll
+            for (int r = 0; r < kPer; ++r) sa[r] = p.scale_a + (long long)min(t.begin + r * 32 + lane, t.end - 1) * p.ldsa;
+            const float *sb = p.scale_b + (long long)t.g * p.stride_sb;
+            const float *sb0 = sb + t.nb * p.ldsb, *sb1 = sb + (long long)((p.N >> 7) + t.nb) * p.ldsb;
+            float next[kPer][4], b0[4], b1[4];
+            auto fetch = [&](int kb) __attribute__((always_inline)) {
+#pragma unroll
+                for (int u = 0; u < 4; ++u) {
+                    const bool in = kb + u < kb_end;
+#pragma unroll
+                    for (int r = 0; r < kPer; ++r) next[r][u] = in ? __ldg(sa[r] + kb + u) : 0.0f;
+                    b0[u] = in ? __ldg(sb0 + kb + u) : 0.0f;
+                    b1[u] = kSwiglu && in ? __ldg(sb1 + kb + u) : 0.0f;
+                }
+            };
+            if (kb_begin < kb_end) fetch(kb_begin);
+#pragma unroll 1
+            for (int kb0 = kb_begin; ok && kb0 < kb_end; kb0 += 4) {
+                float now[NB][kPer][4];
+#pragma unroll
+                for (int r = 0; r < kPer; ++r)
+#pragma unroll
+                    for (int u = 0; u < 4; ++u) {
+                        now[0][r][u] = next[r][u] * b0[u];
+                        if constexpr (kSwiglu) now[NB - 1][r][u] = next[r][u] * b1[u];
+                    }
+                fetch(kb0 + 4);
+#pragma unroll
+                for (int u = 0; u < 4; ++u) {
+                    if (kb0 + u >= kb_end) break;
+                    ok = mbar_wait_bounded(scale_empty_bar(slot), phase ^ 1u, abort_flag, p.status, kWaitGroupScales, p.wait_ns);
+                    ok = __all_sync(0xffffffffu, ok);
+                    if (!ok) break;
+#pragma unroll
+                    for (int b = 0; b < NB; ++b)
+#pragma unroll
+                        for (int r = 0; r < kPer; ++r)
+                            if (r * 32 + lane < TOK) ring[(slot * NB + b) * TOK + r * 32 + lane] = now[b][r][u];
+                    __syncwarp();
+                    if (lane == 0) mbar_arrive(scale_full_bar(slot));
+                    if (++slot == kGrScaleSlots) {
+                        slot = 0;
+                        phase ^= 1u;
+                    }
+                }
+            }
+        }
+        __syncwarp();
+    } else if (warp >= 4) {
+        // ------------------------------ sums and tails ----------------------------------
+        const int quarter = warp & 3;
+        const int blk = (warp - 4) >> 2;  // SwiGLU: 0 = gate, 1 = up
+        const int n_in = quarter * 32 + lane;
+        const uint32_t t_lane = tmem_base + (uint32_t(quarter * 32) << 16) + blk * TOK;
+        const float *ring = reinterpret_cast<const float *>(smem_gen + L::kScales);
+        uint32_t uses = 0, slot_phase = 0, tiles = 0;
+        int slot = 0;
+        bool ok = true;
+        RowsWalk walk;
+        RowsTile t;
+        auto load_add = [&](uint32_t taddr, const float *s) __attribute__((always_inline)) {
+            // acc += v (s == NULL), or acc += s[j] * v[j]; the buffer is released once everything is in registers
+            uint32_t v[TOK];
+            if constexpr (TOK == 16) {
+                tmem_ld_32x16(taddr, *reinterpret_cast<uint32_t(*)[16]>(&v[0]));
+            } else {
+#pragma unroll
+                for (int c = 0; c < TOK / 32; ++c) tmem_ld_32x32(taddr + 32 * c, *reinterpret_cast<uint32_t(*)[32]>(&v[32 * c]));
+            }
+            tmem_ld_wait();
+            tc_fence_before();
+            __syncwarp();
+            if (lane == 0) mbar_arrive(acc_empty_bar(uses % kGrBufs));
+#pragma unroll
+            for (int j = 0; j < TOK / 2; ++j) {
+                const float2 x = make_float2(__uint_as_float(v[2 * j]), __uint_as_float(v[2 * j + 1]));
+                if (s) {
+                    const float2 f = *reinterpret_cast<const float2 *>(s + 2 * j);
+                    acc[j] = __ffma2_rn(x, f, acc[j]);
+                } else {
+                    acc[j] = x;
+                }
+            }
+        };
+        for (int i = first; ok && next_rows_tile<TOK>(p, walk, i, t); i += step, ++tiles) {
+#pragma unroll
+            for (int j = 0; j < TOK / 2; ++j) acc[j] = make_float2(0.0f, 0.0f);
+            if constexpr (kScaled) {
+#pragma unroll 1
+                for (int kb = kb_begin; kb < kb_end; ++kb, ++uses) {
+                    if (lane == 0)
+                        ok = mbar_wait_bounded(scale_full_bar(slot), slot_phase, abort_flag, p.status, kWaitGroupScales, p.wait_ns) &&
+                             mbar_wait_bounded(acc_full_bar(uses % kGrBufs), (uses / kGrBufs) & 1, abort_flag, p.status, kWaitGroupAccFull,
+                                               p.wait_ns);
+                    ok = __shfl_sync(0xffffffffu, ok, 0);
+                    if (!ok) break;
+                    tc_fence_after();
+                    load_add(t_lane + (uses % kGrBufs) * NB * TOK, ring + (slot * NB + blk) * TOK);
+                    __syncwarp();
+                    if (lane == 0) mbar_arrive(scale_empty_bar(slot));
+                    if (++slot == kGrScaleSlots) {
+                        slot = 0;
+                        slot_phase ^= 1u;
+                    }
+                }
+            } else if (kb_begin < kb_end) {
+                if (lane == 0)
+                    ok = mbar_wait_bounded(acc_full_bar(uses % kGrBufs), (uses / kGrBufs) & 1, abort_flag, p.status, kWaitGroupAccFull,
+                                           p.wait_ns);
+                ok = __shfl_sync(0xffffffffu, ok, 0);
+                if (!ok) break;
+                tc_fence_after();
+                load_add(t_lane + (uses % kGrBufs) * NB * TOK, nullptr);
+                ++uses;
+            }
+            if (!ok) break;
+            last = t;
+            have = true;
+            if (S > 1) break;  // the partial sums meet below
+
+            const int rows = t.end - t.begin;
+            const int col = t.nb * 128 + n_in;
+            if constexpr (!kSwiglu) {
+                if (col < p.N) {
+                    __nv_bfloat16 *dst = static_cast<__nv_bfloat16 *>(p.C) + (long long)t.begin * p.ldc + col;
+#pragma unroll
+                    for (int j = 0; j < TOK; ++j)
+                        if (j < rows) dst[j * p.ldc] = __float2bfloat16_rn((j & 1) ? acc[j / 2].y : acc[j / 2].x);
+                }
+            } else {
+                float *xch = reinterpret_cast<float *>(smem_gen + L::kXch);
+                if (blk == 1) {
+                    // up: hand the sums to the gate warp of the same rows
+                    if (lane == 0)
+                        ok = mbar_wait_bounded(up_empty_bar(quarter), (tiles & 1) ^ 1u, abort_flag, p.status, kWaitGroupHalf, p.wait_ns);
+                    ok = __shfl_sync(0xffffffffu, ok, 0);
+                    if (!ok) break;
+#pragma unroll
+                    for (int j = 0; j < TOK; ++j) xch[j * 128 + n_in] = (j & 1) ? acc[j / 2].y : acc[j / 2].x;
+                    __syncwarp();
+                    if (lane == 0) mbar_arrive(up_full_bar(quarter));
+                } else {
+                    if (lane == 0)
+                        ok = mbar_wait_bounded(up_full_bar(quarter), tiles & 1, abort_flag, p.status, kWaitGroupHalf, p.wait_ns);
+                    ok = __shfl_sync(0xffffffffu, ok, 0);
+                    if (!ok) break;
+#pragma unroll
+                    for (int j = 0; j < TOK / 2; ++j) {
+                        acc[j].x = silu_mul(acc[j].x, xch[(2 * j) * 128 + n_in]);
+                        acc[j].y = silu_mul(acc[j].y, xch[(2 * j + 1) * 128 + n_in]);
+                    }
+                    __syncwarp();
+                    if (lane == 0) mbar_arrive(up_empty_bar(quarter));
+                    if constexpr (EPI == GEPI_SWIGLU_BF16) {
+                        __nv_bfloat16 *dst = static_cast<__nv_bfloat16 *>(p.C) + (long long)t.begin * p.ldc + col;
+#pragma unroll
+                        for (int j = 0; j < TOK; ++j)
+                            if (j < rows) dst[j * p.ldc] = __float2bfloat16_rn((j & 1) ? acc[j / 2].y : acc[j / 2].x);
+                    } else {
+                        // the largest magnitude of each row's 128 columns: as integers, whose order is the same and
+                        // where a NaN is above everything
+                        uint32_t *amax = reinterpret_cast<uint32_t *>(smem_gen + L::kAmax) + (tiles & 1) * 4 * TOK;
+#pragma unroll
+                        for (int j = 0; j < TOK; ++j) {
+                            const uint32_t m = __reduce_max_sync(0xffffffffu, __float_as_uint((j & 1) ? acc[j / 2].y : acc[j / 2].x) & 0x7fffffffu);
+                            if (lane == (j & 31)) amax[quarter * TOK + j] = m;
+                        }
+                        __syncwarp();
+                        if (lane == 0) {
+                            mbar_arrive(amax_bar);
+                            ok = mbar_wait_bounded(amax_bar, tiles & 1, abort_flag, p.status, kWaitGroupHalf, p.wait_ns);
+                        }
+                        ok = __shfl_sync(0xffffffffu, ok, 0);
+                        if (!ok) break;
+                        uint8_t *dst = static_cast<uint8_t *>(p.C) + (long long)t.begin * p.ldc + col;
+#pragma unroll
+                        for (int j = 0; j < TOK; ++j) {
+                            if (j >= rows) break;
+                            const uint32_t m = max(max(amax[j], amax[TOK + j]), max(amax[2 * TOK + j], amax[3 * TOK + j]));
+                            const float scale = block_scale_of(__uint_as_float(m));
+                            const float h = ((j & 1) ? acc[j / 2].y : acc[j / 2].x) * (1.0f / scale);
+                            dst[j * p.ldc] = (uint8_t)__nv_cvt_float_to_fp8(h, __NV_SATFINITE, __NV_E4M3);
+                            if (quarter == 0 && lane == 0) p.scale_c[(long long)(t.begin + j) * p.ldsc + t.nb] = scale;
+                        }
+                    }
+                }
+            }
+        }
+    }
+
+    if (S > 1) {
+        // ---- partial sums of one tile: rows r of it belong to CTA r / (TOK / S) of the cluster ----
+        __syncwarp();
+        cluster_sync_all();  // every ring is idle
+        const int per = TOK / S;
+        const uint32_t recv = smem_base;  // [rank][per][128]
+        if (warp >= 4 && have) {
+            const int n_in = (warp & 3) * 32 + lane;
+#pragma unroll
+            for (int j = 0; j < TOK; ++j) {
+                const int owner = j / per;
+                st_cluster_f32(map_to_cta(recv, owner) + ((rank * per + j % per) * 128 + n_in) * 4, (j & 1) ? acc[j / 2].y : acc[j / 2].x);
+            }
+        }
+        __syncwarp();
+        cluster_sync_all();
+        if (warp >= 4 && have) {
+            const int n_in = (warp & 3) * 32 + lane;
+            const int col = last.nb * 128 + n_in;
+            const float *got = reinterpret_cast<const float *>(smem_gen);
+            for (int j = 0; j < per; ++j) {
+                const int row = last.begin + rank * per + j;
+                if (row >= last.end || col >= p.N) break;
+                float sum = 0.0f;
+                for (int r = 0; r < S; ++r) sum += got[(r * per + j) * 128 + n_in];
+                static_cast<__nv_bfloat16 *>(p.C)[(long long)row * p.ldc + col] = __float2bfloat16_rn(sum);
+            }
+        }
+    }
+
+    // ------------------------------ teardown --------------------------------------------
+    tc_fence_before();
+    __syncthreads();
+    if (warp == 1) {
+        if (*abort_flag) {
+            const uint64_t t0 = globaltimer_ns();
+            while (globaltimer_ns() - t0 < 200000ull) __nanosleep(1000);
+        }
+        tc_fence_after();
+        tmem_dealloc(tmem_base, L::kTmemCols);
+    }
+}
+
+template <int KIND, int EPI, int TOK>
+static int launch_rows(const GroupedCall &c, GroupedParams p) {
+    constexpr int NB = gepi_swiglu(EPI) ? 2 : 1;
+    using L = RowsLayout<NB, TOK>;
+    constexpr int kElem = KIND == MMA_F16 ? 2 : 1;
+    constexpr int kBlockK = kRowBytes / kElem;
+    auto kern = grouped_rows_kernel<KIND, EPI, TOK>;
+    static KernelSetup ks;
+    int rc = ks.once(
+        [&](int *) {
+            return cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, L::kDynamic) == cudaSuccess
+                       ? (int)O64_OK
+                       : (int)O64_ERR_CUDA;
+        },
+        nullptr);
+    if (rc) return rc;
+    CUtensorMap tx, tw;
+    rc = encode_2d(&tx, c.kind, c.A, c.T, c.K, c.lda, kBlockK, TOK);
+    if (!rc) rc = encode_3d(&tw, kElem, c.B, c.K, NB * c.N, c.G, c.ldb, c.stride_b, kBlockK, 128, true);
+    if (rc) return rc;
+    p.num_n_tiles = (int)((c.N + 127) / 128);
+    // at most this many tiles (the groups' sizes are on the device)
+    const long long most = (c.T / TOK + (c.G < c.T ? c.G : c.T)) * p.num_n_tiles;
+    if (most > INT32_MAX - 4 * c.num_sms) return O64_ERR_RANK;
+    const long long tiles = c.offsets ? most : (c.T + TOK - 1) / TOK * p.num_n_tiles;
+    // Too few tiles for the GPU: the K blocks of each are divided over a cluster, as long as a CTA keeps four
+    // of them.  (SwiGLU tiles already carry two weight blocks.)
+    int S = 1;
+    if (NB == 1)
+        while (S < 8 && tiles * S * 2 <= c.num_sms && p.num_k_blocks >= 4 * S * 2) S *= 2;
+    p.split = S;
+    const int grid = (int)(S > 1 ? tiles * S : (tiles < c.num_sms ? tiles : c.num_sms));
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = dim3((unsigned)grid, 1, 1);
+    cfg.blockDim = dim3(L::kThreads, 1, 1);
+    cfg.dynamicSmemBytes = L::kDynamic;
+    cfg.stream = c.stream;
+    cudaLaunchAttribute at[2];
+    at[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    at[0].val.programmaticStreamSerializationAllowed = 1;
+    at[1].id = cudaLaunchAttributeClusterDimension;
+    at[1].val.clusterDim.x = (unsigned)S;
+    at[1].val.clusterDim.y = 1;
+    at[1].val.clusterDim.z = 1;
+    cfg.attrs = at;
+    cfg.numAttrs = 2;
+    if (cudaLaunchKernelEx(&cfg, kern, tx, tw, p) != cudaSuccess) {
+        (void)cudaGetLastError();
+        return O64_ERR_CUDA;
+    }
+    return O64_OK;
+}
+
+bool grouped_rows_fits(const GroupedCall &c) {
+    if (c.wgrad || c.b_kn || c.epi == GEPI_F32 || c.T <= 0) return false;
+    const int64_t groups = c.G < c.T ? c.G : c.T;
+    return c.T <= 64 * groups;
+}
+
+template <int KIND, int EPI>
+static int launch_rows_tok(const GroupedCall &c, const GroupedParams &p) {
+    const int64_t groups = c.G < c.T ? c.G : c.T;
+    const int64_t mean = (c.T + groups - 1) / groups;
+    if (mean <= 16) return launch_rows<KIND, EPI, 16>(c, p);
+    if (mean <= 32) return launch_rows<KIND, EPI, 32>(c, p);
+    return launch_rows<KIND, EPI, 64>(c, p);
+}
+
+int grouped_rows_launch(const GroupedCall &c, const GroupedParams &p) {
+    if (c.kind == O64_KIND_BF16) {
+        if (c.epi == GEPI_BF16) return launch_rows_tok<MMA_F16, GEPI_BF16>(c, p);
+    } else if (c.kind == O64_KIND_FP8) {
+        if (c.epi == GEPI_BF16) return launch_rows_tok<MMA_F8F6F4, GEPI_BF16>(c, p);
+        if (c.epi == GEPI_SWIGLU_BF16) return launch_rows_tok<MMA_F8F6F4, GEPI_SWIGLU_BF16>(c, p);
+        if (c.epi == GEPI_SWIGLU_E4M3) return launch_rows_tok<MMA_F8F6F4, GEPI_SWIGLU_E4M3>(c, p);
+    }
+    return O64_ERR_DTYPE;
+}
+
+}  // namespace o64
