@@ -823,7 +823,7 @@ extern "C" int o64_rmsnorm_bf16(o64_handle_t h, int64_t T, int64_t N, const void
     NormCall c;
     c.T = T, c.N = N, c.X = X, c.ldx = ldx, c.R = R, c.ldr = ldr, c.S = S, c.lds = lds, c.W = W, c.w_f32 = w_f32 != 0;
     c.eps = eps, c.out_kind = out_kind, c.row_scale = scale_block == 0, c.Y = Y, c.ldy = ldy, c.scales = scales;
-    c.ldscales = ldscales, c.rstd = rstd, c.stream = (cudaStream_t)stream;
+    c.ldscales = ldscales, c.rstd = rstd, c.status = h->status_word, c.wait_ns = h->wait_ns ? h->wait_ns : kDefaultWaitNs, c.stream = (cudaStream_t)stream;
     return norm_forward(c, h->num_sms);
 }
 
@@ -852,7 +852,8 @@ extern "C" int o64_rmsnorm_bf16_backward(o64_handle_t h, int64_t T, int64_t N, c
     NormBackwardCall c;
     c.T = T, c.N = N, c.dY = dY, c.lddy = lddy, c.S = S, c.lds = lds, c.W = W, c.w_f32 = w_f32 != 0, c.rstd = rstd;
     c.dR = dR, c.lddr = lddr, c.dX = dX, c.lddx = lddx, c.dW = dW, c.workspace = static_cast<float *>(workspace), c.stream = s;
-    return norm_backward(c);
+    c.status = h->status_word, c.wait_ns = h->wait_ns ? h->wait_ns : kDefaultWaitNs;
+    return norm_backward(c, h->num_sms);
 }
 
 // Checks what the grouped and block-scaled products have in common and launches.  Returns O64_ERR_* or O64_OK.

@@ -9,19 +9,29 @@
 // norm is taken of the sum in fp32; the stream s that goes on to the next layer is that sum rounded
 // to bf16 once.
 //
+// Bound by HBM.  Many rows run on a few blocks per SM that stay: rows come in by bulk copies, a ring of
+// three ahead, so that loads go on while a row is reduced, converted and stored, and a thread keeps its
+// columns of w.  Few rows, or rows that are not 16-byte aligned, run on a block per row that loads for
+// itself.
+//
 // Gradient, with n = s * rstd, g = dy * w:   dx = rstd * (g - n * mean(g n)) + dr   (x and r receive
 // the same one),   dw[j] = sum over rows of dy n.  The sum over rows runs in two fixed stages (a
 // partial row per thread group, then one addition per column), so that it does not depend on timing.
 #include <cuda_bf16.h>
 #include <cuda_fp8.h>
 
+#include <algorithm>
+
 #include "norm.cuh"
+#include "ptx_sm100.cuh"
+#include "umma_common.cuh"
 
 namespace o64 {
 
 namespace {
 
 constexpr int kNormMaxThreads = 512;
+constexpr int kRingCols = 2048;  // narrower rows run on the block-per-row kernel
 constexpr float kE4m3Max = 448.0f;
 constexpr float kMinNormal = 1.17549435e-38f;
 
@@ -102,6 +112,16 @@ __device__ __forceinline__ float row_reduce(float v, float *slot) {
     float r = mine[0];
     for (int i = 1; i < warps; ++i) r = MAX ? max_nan(r, mine[i]) : r + mine[i];
     return r;
+}
+
+__device__ __forceinline__ uint2 quant8(const float (&v)[8], float inv) {
+    uint32_t q[2] = {0, 0};
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+        const float2 two = make_float2(v[2 * e] * inv, v[2 * e + 1] * inv);
+        q[e >> 1] |= (uint32_t)__nv_cvt_float2_to_fp8x2(two, __NV_SATFINITE, __NV_E4M3) << (16 * (e & 1));
+    }
+    return make_uint2(q[0], q[1]);
 }
 
 struct FwdParams {
@@ -194,14 +214,10 @@ __global__ void __launch_bounds__(kNormMaxThreads) norm_forward_kernel(const Fwd
             // one reciprocal per block instead of a division per value: within an ulp of h / scale before
             // the rounding to four bits
             const float inv = 1.0f / scale;
-            uint32_t q[2] = {0, 0};
-#pragma unroll
-            for (int e = 0; e < 4; ++e) {
-                const float2 two = make_float2(v[i][2 * e] * inv, v[i][2 * e + 1] * inv);
-                q[e >> 1] |= (uint32_t)__nv_cvt_float2_to_fp8x2(two, __NV_SATFINITE, __NV_E4M3) << (16 * (e & 1));
-            }
+            const uint2 q2 = quant8(v[i], inv);
+            const uint32_t q[2] = {q2.x, q2.y};
             if constexpr (VEC) {
-                if (col < n) *reinterpret_cast<uint2 *>(y + col) = make_uint2(q[0], q[1]);
+                if (col < n) *reinterpret_cast<uint2 *>(y + col) = q2;
             } else {
 #pragma unroll
                 for (int e = 0; e < 8; ++e)
@@ -288,6 +304,252 @@ __global__ void __launch_bounds__(kNormMaxThreads) norm_backward_kernel(const Bw
     }
 }
 
+// ---- many rows: a ring of bulk copies -------------------------------------------------------------
+constexpr int kNormWait = 0x801;
+constexpr int kNormMaxStages = 3;
+
+__device__ __forceinline__ void bulk_load(uint32_t dst, const void *src, uint32_t bytes, uint32_t bar) {
+    asm volatile("cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];" ::"r"(dst), "l"(src),
+                 "r"(bytes), "r"(bar)
+                 : "memory");
+}
+
+// Eight values of a row in shared memory.
+__device__ __forceinline__ void smem8(const uint8_t *at, float (&v)[8]) {
+    const uint4 raw = *reinterpret_cast<const uint4 *>(at);
+    const uint32_t w[4] = {raw.x, raw.y, raw.z, raw.w};
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+        v[2 * i] = __uint_as_float(w[i] << 16);
+        v[2 * i + 1] = __uint_as_float(w[i] & 0xffff0000u);
+    }
+}
+
+// In both kernels a copy that does not arrive within the budget is reported and its rows are undefined; every
+// thread still walks to the end (the flag ends the remaining waits at once).
+template <int NV, bool E4M3>
+__global__ void __launch_bounds__(kNormMaxThreads) norm_forward_ring_kernel(const FwdParams p, int stages, int *status, unsigned long long wait_ns) {
+    extern __shared__ __align__(128) uint8_t smem[];
+    __shared__ float slots[2][16];
+    __shared__ __align__(8) uint64_t bars[kNormMaxStages];
+    __shared__ int abort_word;
+    const int n = p.N;
+    const uint32_t row_bytes = (uint32_t)n * 2, pitch = (row_bytes + 127) & ~127u;
+    const int operands = p.R ? 2 : 1;
+    const uint32_t stage_bytes = pitch * operands;
+    if (threadIdx.x == 0) {
+        for (int s = 0; s < stages; ++s) mbar_init(smem_u32(&bars[s]), 1);
+        abort_word = 0;
+        fence_mbar_init();
+    }
+    __syncthreads();
+    auto load = [&](long long row, int s) {
+        const uint32_t bar = smem_u32(&bars[s]), dst = smem_u32(smem) + s * stage_bytes;
+        mbar_arrive_expect_tx(bar, row_bytes * operands);
+        bulk_load(dst, p.X + row * p.ldx, row_bytes, bar);
+        if (p.R) bulk_load(dst + pitch, p.R + row * p.ldr, row_bytes, bar);
+    };
+    if (threadIdx.x == 0)
+        for (int s = 0; s < stages; ++s) {
+            const long long row = blockIdx.x + (long long)s * gridDim.x;
+            if (row < p.T) load(row, s);
+        }
+    float w[NV][8];
+#pragma unroll
+    for (int i = 0; i < NV; ++i) load_w8<true>(p.W, p.w_f32, (i * blockDim.x + threadIdx.x) * 8, n, w[i]);
+    int stage = 0, turn = 0;
+    uint32_t phase = 0;
+    for (long long row = blockIdx.x; row < p.T; row += gridDim.x, turn ^= 1) {
+        mbar_wait_bounded(smem_u32(&bars[stage]), phase, &abort_word, status, kNormWait, wait_ns);
+        const uint8_t *at = smem + stage * stage_bytes;
+        float v[NV][8];
+        float sq = 0.0f;
+#pragma unroll
+        for (int i = 0; i < NV; ++i) {
+            const int col = (i * blockDim.x + threadIdx.x) * 8;
+#pragma unroll
+            for (int e = 0; e < 8; ++e) v[i][e] = 0.0f;
+            if (col < n) {
+                smem8(at + col * 2, v[i]);
+                if (p.R) {
+                    float a[8];
+                    smem8(at + pitch + col * 2, a);
+#pragma unroll
+                    for (int e = 0; e < 8; ++e) v[i][e] += a[e];
+                }
+#pragma unroll
+                for (int e = 0; e < 8; ++e) sq = fmaf(v[i][e], v[i][e], sq);
+            }
+        }
+        // the block's sum; behind the barrier in it the stage's values are in registers and it is loaded again
+#pragma unroll
+        for (int o = 16; o > 0; o >>= 1) sq += __shfl_xor_sync(0xffffffffu, sq, o);
+        if ((threadIdx.x & 31) == 0) slots[turn][threadIdx.x >> 5] = sq;
+        __syncthreads();
+        if (threadIdx.x == 0 && row + (long long)stages * gridDim.x < p.T) {
+            fence_proxy_async_smem();
+            load(row + (long long)stages * gridDim.x, stage);
+        }
+        float sum = slots[turn][0];
+        for (int i = 1; i < (int)(blockDim.x >> 5); ++i) sum += slots[turn][i];
+        const float rstd = 1.0f / sqrtf(sum / (float)n + p.eps);
+        if (p.rstd && threadIdx.x == 0) p.rstd[row] = rstd;
+        if (p.S) {
+#pragma unroll
+            for (int i = 0; i < NV; ++i) store8<true>(p.S + row * p.lds, (i * blockDim.x + threadIdx.x) * 8, n, v[i]);
+        }
+#pragma unroll
+        for (int i = 0; i < NV; ++i) {
+            const int col = (i * blockDim.x + threadIdx.x) * 8;
+#pragma unroll
+            for (int e = 0; e < 8; ++e) v[i][e] = v[i][e] * rstd * w[i][e];
+            if constexpr (!E4M3) {
+                store8<true>(static_cast<__nv_bfloat16 *>(p.Y) + row * p.ldy, col, n, v[i]);
+            } else {
+                float m = 0.0f;
+                if (col < n) {
+#pragma unroll
+                    for (int e = 0; e < 8; ++e) m = max_nan(m, fabsf(v[i][e]));
+                }
+#pragma unroll
+                for (int o = 8; o > 0; o >>= 1) m = max_nan(m, __shfl_xor_sync(0xffffffffu, m, o));
+                const float scale = scale_of(m);
+                const float inv = 1.0f / scale;
+                if (col < n) {
+                    if ((threadIdx.x & 15) == 0) p.scales[row * p.ldscales + col / 128] = scale;
+                    *reinterpret_cast<uint2 *>(static_cast<uint8_t *>(p.Y) + row * p.ldy + col) = quant8(v[i], inv);
+                }
+            }
+        }
+        if (++stage == stages) {
+            stage = 0;
+            phase ^= 1u;
+        }
+    }
+    if (abort_word) {  // copies may still be in flight
+        const uint64_t t0 = globaltimer_ns();
+        while (globaltimer_ns() - t0 < 200000ull) __nanosleep(1000);
+    }
+}
+
+template <int NV>
+__global__ void __launch_bounds__(kNormMaxThreads) norm_backward_ring_kernel(const BwdParams p, int stages, int *status, unsigned long long wait_ns) {
+    extern __shared__ __align__(128) uint8_t smem[];
+    __shared__ float slots[2][16];
+    __shared__ __align__(8) uint64_t bars[kNormMaxStages];
+    __shared__ int abort_word;
+    const int n = p.N;
+    const uint32_t row_bytes = (uint32_t)n * 2, pitch = (row_bytes + 127) & ~127u;
+    const int operands = p.dR ? 3 : 2;
+    const uint32_t stage_bytes = pitch * operands;
+    float *w_smem = reinterpret_cast<float *>(smem + stages * stage_bytes);
+    if (threadIdx.x == 0) {
+        for (int s = 0; s < stages; ++s) mbar_init(smem_u32(&bars[s]), 1);
+        abort_word = 0;
+        fence_mbar_init();
+    }
+    __syncthreads();
+    auto load = [&](long long row, int s) {
+        const uint32_t bar = smem_u32(&bars[s]), dst = smem_u32(smem) + s * stage_bytes;
+        mbar_arrive_expect_tx(bar, row_bytes * operands);
+        bulk_load(dst, p.dY + row * p.lddy, row_bytes, bar);
+        bulk_load(dst + pitch, p.S + row * p.lds, row_bytes, bar);
+        if (p.dR) bulk_load(dst + 2 * pitch, p.dR + row * p.lddr, row_bytes, bar);
+    };
+    if (threadIdx.x == 0)
+        for (int s = 0; s < stages; ++s) {
+            const long long row = blockIdx.x + (long long)s * gridDim.x;
+            if (row < p.T) load(row, s);
+        }
+    float dw[NV][8];
+#pragma unroll
+    for (int i = 0; i < NV; ++i) {
+        const int col = (i * blockDim.x + threadIdx.x) * 8;
+        float w[8];
+        load_w8<true>(p.W, p.w_f32, col, n, w);
+#pragma unroll
+        for (int e = 0; e < 8; ++e) {
+            dw[i][e] = 0.0f;
+            if (col < n) w_smem[col + e] = w[e];  // read back by this thread only
+        }
+    }
+    int stage = 0, turn = 0, before = 0;
+    uint32_t phase = 0;
+    for (long long row = blockIdx.x; row < p.T; row += gridDim.x, turn ^= 1) {
+        const float rstd = p.rstd[row];
+        mbar_wait_bounded(smem_u32(&bars[stage]), phase, &abort_word, status, kNormWait, wait_ns);
+        const uint8_t *at = smem + stage * stage_bytes;
+        float dot = 0.0f;
+#pragma unroll
+        for (int i = 0; i < NV; ++i) {
+            const int col = (i * blockDim.x + threadIdx.x) * 8;
+            if (col < n) {
+                float g[8], nn[8], w[8];
+                smem8(at + col * 2, g);
+                smem8(at + pitch + col * 2, nn);
+                *reinterpret_cast<float4 *>(w) = *reinterpret_cast<const float4 *>(w_smem + col);
+                *reinterpret_cast<float4 *>(w + 4) = *reinterpret_cast<const float4 *>(w_smem + col + 4);
+#pragma unroll
+                for (int e = 0; e < 8; ++e) {
+                    const float x = nn[e] * rstd;
+                    dw[i][e] = fmaf(g[e], x, dw[i][e]);
+                    dot = fmaf(g[e] * w[e], x, dot);
+                }
+            }
+        }
+#pragma unroll
+        for (int o = 16; o > 0; o >>= 1) dot += __shfl_xor_sync(0xffffffffu, dot, o);
+        if ((threadIdx.x & 31) == 0) slots[turn][threadIdx.x >> 5] = dot;
+        __syncthreads();
+        // everyone is past the row before: its stage is free
+        if (threadIdx.x == 0 && row != blockIdx.x && row + (long long)(stages - 1) * gridDim.x < p.T) {
+            fence_proxy_async_smem();
+            load(row + (long long)(stages - 1) * gridDim.x, before);
+        }
+        float sum = slots[turn][0];
+        for (int i = 1; i < (int)(blockDim.x >> 5); ++i) sum += slots[turn][i];
+        const float mean = sum / (float)n;
+#pragma unroll
+        for (int i = 0; i < NV; ++i) {
+            const int col = (i * blockDim.x + threadIdx.x) * 8;
+            if (col < n) {
+                float g[8], nn[8], w[8], out[8], dr[8];
+                smem8(at + col * 2, g);
+                smem8(at + pitch + col * 2, nn);
+                if (p.dR) smem8(at + 2 * pitch + col * 2, dr);
+                *reinterpret_cast<float4 *>(w) = *reinterpret_cast<const float4 *>(w_smem + col);
+                *reinterpret_cast<float4 *>(w + 4) = *reinterpret_cast<const float4 *>(w_smem + col + 4);
+#pragma unroll
+                for (int e = 0; e < 8; ++e) {
+                    out[e] = rstd * (g[e] * w[e] - nn[e] * rstd * mean);
+                    if (p.dR) out[e] += dr[e];
+                }
+                store8<true>(p.dX + row * p.lddx, col, n, out);
+            }
+        }
+        before = stage;
+        if (++stage == stages) {
+            stage = 0;
+            phase ^= 1u;
+        }
+    }
+    if (p.partial) {
+        float *dst = p.partial + (long long)blockIdx.x * n;
+#pragma unroll
+        for (int i = 0; i < NV; ++i) {
+            const int col = (i * blockDim.x + threadIdx.x) * 8;
+            if (col < n) {
+                *reinterpret_cast<float4 *>(dst + col) = make_float4(dw[i][0], dw[i][1], dw[i][2], dw[i][3]);
+                *reinterpret_cast<float4 *>(dst + col + 4) = make_float4(dw[i][4], dw[i][5], dw[i][6], dw[i][7]);
+            }
+        }
+    }
+    if (abort_word) {
+        const uint64_t t0 = globaltimer_ns();
+        while (globaltimer_ns() - t0 < 200000ull) __nanosleep(1000);
+    }
+}
+
 // dW[j] = sum over the partial rows: 32 columns per block, 16 threads down the rows of each.
 __global__ void __launch_bounds__(512) norm_dw_kernel(const float *partial, long long rows, int N, float *dW) {
     __shared__ float part[16][33];
@@ -326,6 +588,37 @@ int launch_forward(const FwdParams &p, bool e4m3, dim3 grid, dim3 block, cudaStr
     return cudaGetLastError() == cudaSuccess ? O64_OK : O64_ERR_CUDA;
 }
 
+// Blocks that stay on an SM for rows of N columns with `operands` of them on their way, and the depth of their
+// rings: 512 threads and all shared memory of an SM, at most three blocks and three rows ahead.
+bool ring_shape(int64_t N, int operands, int extra_bytes_per_col, int *blocks_per_sm, int *stages, size_t *smem) {
+    const int tpr = threads_for(N, 4);
+    const size_t row = (size_t)((N * 2 + 127) / 128 * 128) * operands, extra = (size_t)N * extra_bytes_per_col;
+    if (tpr > kNormMaxThreads) return false;
+    for (int b = kNormMaxThreads / tpr < 3 ? kNormMaxThreads / tpr : 3; b >= 1; --b)
+        for (int s = 3; s >= 2; --s)
+            if ((row * s + extra + 1280) * b <= 227 * 1024 && row * s + extra <= 220 * 1024) {
+                *blocks_per_sm = b, *stages = s, *smem = row * s + extra;
+                return true;
+            }
+    return false;
+}
+
+template <typename F>
+int allow_smem(F kern, KernelSetup &ks) {
+    return ks.once([&](int *) { return cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, 220 * 1024) == cudaSuccess ? (int)O64_OK : (int)O64_ERR_CUDA; },
+                   nullptr);
+}
+
+template <bool E4M3>
+int launch_forward_ring(const FwdParams &p, int tpr, int grid, int stages, size_t smem, int *status, unsigned long long wait_ns, cudaStream_t s) {
+    static KernelSetup ks;
+    auto kern = norm_forward_ring_kernel<4, E4M3>;
+    const int rc = allow_smem(kern, ks);
+    if (rc) return rc;
+    kern<<<grid, tpr, smem, s>>>(p, stages, status, wait_ns);
+    return cudaGetLastError() == cudaSuccess ? O64_OK : O64_ERR_CUDA;
+}
+
 }  // namespace
 
 int norm_forward(const NormCall &c, int num_sms) {
@@ -339,6 +632,12 @@ int norm_forward(const NormCall &c, int num_sms) {
     p.S = static_cast<__nv_bfloat16 *>(c.S), p.lds = c.lds;
     p.W = c.W, p.w_f32 = c.w_f32, p.eps = c.eps;
     p.Y = c.Y, p.ldy = c.ldy, p.scales = c.scales, p.ldscales = c.ldscales, p.rstd = c.rstd, p.row_scale = c.row_scale;
+    int per_sm, stages;
+    size_t smem;
+    if (vec && !(e4m3 && c.row_scale) && c.N >= kRingCols && ring_shape(c.N, c.R ? 2 : 1, 0, &per_sm, &stages, &smem) &&
+        c.T >= (int64_t)2 * per_sm * num_sms)
+        return e4m3 ? launch_forward_ring<true>(p, threads_for(c.N, 4), per_sm * num_sms, stages, smem, c.status, c.wait_ns, c.stream)
+                    : launch_forward_ring<false>(p, threads_for(c.N, 4), per_sm * num_sms, stages, smem, c.status, c.wait_ns, c.stream);
     const int nv = pick_nv(c.N, c.T <= 2 * num_sms ? 1 : 4);
     const int tpr = threads_for(c.N, nv);
     const int rows = tpr >= 128 ? 1 : 128 / tpr;
@@ -368,7 +667,12 @@ int64_t norm_backward_partials(int64_t T, int64_t N) {
     return blocks * block.y;
 }
 
-int norm_backward(const NormBackwardCall &c) {
+static int add_partials(const NormBackwardCall &c, long long rows) {
+    norm_dw_kernel<<<(unsigned)((c.N + 31) / 32), dim3(32, 16), 0, c.stream>>>(c.workspace, rows, (int)c.N, c.dW);
+    return cudaGetLastError() == cudaSuccess ? O64_OK : O64_ERR_CUDA;
+}
+
+int norm_backward(const NormBackwardCall &c, int num_sms) {
     int nv;
     dim3 block;
     int64_t blocks;
@@ -382,6 +686,19 @@ int norm_backward(const NormBackwardCall &c) {
     p.dX = static_cast<__nv_bfloat16 *>(c.dX), p.lddx = c.lddx;
     p.W = c.W, p.w_f32 = c.w_f32, p.rstd = c.rstd;
     p.partial = c.dW ? c.workspace : nullptr;
+    int per_sm, stages;
+    size_t smem;
+    if (vec && c.N >= kRingCols && (reinterpret_cast<uintptr_t>(c.workspace) & 15u) == 0 && ring_shape(c.N, c.dR ? 3 : 2, 4, &per_sm, &stages, &smem) &&
+        c.T >= (int64_t)2 * per_sm * num_sms) {
+        static KernelSetup ks;
+        auto kern = norm_backward_ring_kernel<4>;
+        const int rc = allow_smem(kern, ks);
+        if (rc) return rc;
+        const int grid = (int)std::min<int64_t>((int64_t)per_sm * num_sms, blocks * block.y);  // no more partial rows than the workspace has
+        kern<<<grid, threads_for(c.N, 4), smem, c.stream>>>(p, stages, c.status, c.wait_ns);
+        if (cudaGetLastError() != cudaSuccess) return O64_ERR_CUDA;
+        return c.dW ? add_partials(c, grid) : O64_OK;
+    }
     const unsigned grid = (unsigned)blocks;
     switch (nv) {
     case 2: vec ? norm_backward_kernel<2, true><<<grid, block, 0, c.stream>>>(p) : norm_backward_kernel<2, false><<<grid, block, 0, c.stream>>>(p); break;
@@ -389,11 +706,7 @@ int norm_backward(const NormBackwardCall &c) {
     default: vec ? norm_backward_kernel<8, true><<<grid, block, 0, c.stream>>>(p) : norm_backward_kernel<8, false><<<grid, block, 0, c.stream>>>(p); break;
     }
     if (cudaGetLastError() != cudaSuccess) return O64_ERR_CUDA;
-    if (c.dW) {
-        norm_dw_kernel<<<(unsigned)((c.N + 31) / 32), dim3(32, 16), 0, c.stream>>>(c.workspace, blocks * block.y, (int)c.N, c.dW);
-        if (cudaGetLastError() != cudaSuccess) return O64_ERR_CUDA;
-    }
-    return O64_OK;
+    return c.dW ? add_partials(c, blocks * block.y) : O64_OK;
 }
 
 }  // namespace o64

@@ -28,6 +28,8 @@ struct NormCall {
     float *scales;
     int64_t ldscales;
     float *rstd;  // may be NULL
+    int *status;
+    unsigned long long wait_ns;
     cudaStream_t stream;
 };
 int norm_forward(const NormCall &c, int num_sms);
@@ -47,10 +49,12 @@ struct NormBackwardCall {
     int64_t lddx;
     float *dW;  // NULL: not wanted
     float *workspace;
+    int *status;
+    unsigned long long wait_ns;
     cudaStream_t stream;
 };
 // Rows of partial sums of dW (each N floats) that norm_backward leaves in the workspace.
 int64_t norm_backward_partials(int64_t T, int64_t N);
-int norm_backward(const NormBackwardCall &c);
+int norm_backward(const NormBackwardCall &c, int num_sms);
 
 }  // namespace o64

@@ -50,19 +50,34 @@ def _rowmajor(t, name):
     return t
 
 
-def _want(t, name, dtypes, shape=None):
+def _want(t, name, dtypes, shape):
     """An operand of the given element type(s) and shape (None: any extent), or the library's error."""
+    if t.dtype in dtypes and t.is_cuda and t.shape == shape:
+        return t
     if t.dtype not in dtypes:
         raise O64Error(_lib.ERR_DTYPE, f"{name}: {t.dtype}")
     if not t.is_cuda:
         raise O64Error(_lib.ERR_RANK, f"{name}: not device memory")
-    if shape is not None:
-        if t.dim() != len(shape):
-            raise O64Error(_lib.ERR_RANK, f"{name}: rank {t.dim()}")
-        for have, need in zip(t.shape, shape):
-            if need is not None and have != need:
-                raise O64Error(_lib.ERR_CONFORM, f"{name}: {tuple(t.shape)}")
+    if t.dim() != len(shape):
+        raise O64Error(_lib.ERR_RANK, f"{name}: rank {t.dim()}")
+    for have, need in zip(t.shape, shape):
+        if need is not None and have != need:
+            raise O64Error(_lib.ERR_CONFORM, f"{name}: {tuple(t.shape)}")
     return t
+
+
+def _matrix(t, name, dtype):
+    """An operand that is a matrix of any extents."""
+    if t.dtype is dtype and t.is_cuda and t.dim() == 2:
+        return t
+    return _want(t, name, (dtype,), (None, None))
+
+
+def _new(like, shape, dtype):
+    """A result on the device of `like` (empty_like costs the host half of what empty does)."""
+    if like.shape == shape and like.is_contiguous():
+        return torch.empty_like(like, dtype=dtype)
+    return like.new_empty(shape, dtype=dtype)
 
 
 def _ld(t):
@@ -72,6 +87,8 @@ def _ld(t):
 
 def _laid_out(t):
     """Contiguous columns, and rows (and matrices) that do not overlap."""
+    if t.is_contiguous():
+        return True
     rows, cols = t.shape[-2:]
     return ((cols <= 1 or t.stride(-1) == 1) and (rows <= 1 or t.stride(-2) >= cols) and
             (t.dim() < 3 or t.shape[0] <= 1 or t.stride(0) >= (rows - 1) * _ld(t) + cols))
@@ -93,7 +110,9 @@ def _tma(t):
     """`t` as TMA can read it (contiguous columns; base, pitch and matrix stride multiples of 16 bytes): itself,
     or a copy whose rows are padded."""
     t = _rows(t)
-    e = t.element_size()
+    e = 2 if t.dtype is _BF16 else 1
+    if t.data_ptr() % 16 == 0 and t.shape[-1] * e % 16 == 0 and t.is_contiguous():
+        return t
     if (t.data_ptr() % 16 == 0 and (_ld(t) * e) % 16 == 0 and
             (t.dim() < 3 or t.shape[0] <= 1 or (t.stride(0) * e) % 16 == 0)):
         return t
@@ -309,56 +328,55 @@ class Engine:
         (scale_block 0, one per row; None for bf16).  `summed` is x + residual in bf16 (x itself without a
         residual); pass summed=x or summed=residual to add in place.  rstd [T] is what rms_norm_backward
         needs."""
-        _want(x, "x", (_BF16,), (None, None))
-        T, N = x.shape
+        T, N = shape = _matrix(x, "x", _BF16).shape
         x = _rows(x)
-        _want(weight, "weight", (_BF16, _F32), (N,))
-        weight = weight.contiguous()
+        weight = _want(weight, "weight", (_BF16, _F32), (N,)).contiguous()
         if out_kind not in (_lib.OUT_BF16, _lib.OUT_E4M3) or scale_block not in (0, 128):
             raise O64Error(_lib.ERR_DTYPE, "rms_norm")
         if residual is None:
             if summed is not None:
                 raise O64Error(_lib.ERR_CONFORM, "rms_norm: summed without a residual")
         else:
-            _want(residual, "residual", (_BF16,), (T, N))
-            residual = _rows(residual)
-            summed = torch.empty((T, N), dtype=_BF16, device=x.device) if summed is None else _out(_want(summed, "summed", (_BF16,), (T, N)), "summed")
+            residual = _rows(_want(residual, "residual", (_BF16,), shape))
+            summed = _new(x, shape, _BF16) if summed is None else _out(_want(summed, "summed", (_BF16,), shape), "summed")
         dtype = _OUT_DTYPE[out_kind]
-        y = torch.empty((T, N), dtype=dtype, device=x.device) if out is None else _out(_want(out, "out", (dtype,), (T, N)), "out")
-        ldscales = 0
+        y = _new(x, shape, dtype) if out is None else _out(_want(out, "out", (dtype,), shape), "out")
+        p_scales, ldscales = None, 0
         if out_kind == _lib.OUT_E4M3:
-            shape = (T, -(-N // 128)) if scale_block else (T,)
-            scales = torch.empty(shape, dtype=_F32, device=x.device) if scales is None else _want(scales, "scales", (_F32,), shape)
+            scales_shape = (T, -(-N // 128)) if scale_block else (T,)
+            scales = x.new_empty(scales_shape, dtype=_F32) if scales is None else _want(scales, "scales", (_F32,), scales_shape)
             if scale_block:
                 ldscales = _ld(_out(scales, "scales"))
             else:
                 ldscales = scales.stride(0) if T > 1 else 1
+            p_scales = scales.data_ptr()
         elif scales is not None:
             raise O64Error(_lib.ERR_DTYPE, "rms_norm: scales of a bf16 result")
-        rstd = torch.empty((T,), dtype=_F32, device=x.device) if rstd is None else _want(rstd, "rstd", (_F32,), (T,))
+        rstd = x.new_empty((T,), dtype=_F32) if rstd is None else _want(rstd, "rstd", (_F32,), (T,))
         if T > 1 and rstd.stride(0) != 1:
             raise O64Error(_lib.ERR_CONFORM, "rms_norm: rstd is not contiguous")
-        check(self.lib.o64_rmsnorm_bf16(self._h, T, N, x.data_ptr(), _ld(x), None if residual is None else residual.data_ptr(),
-                                        0 if residual is None else _ld(residual), None if residual is None else summed.data_ptr(),
-                                        0 if residual is None else _ld(summed), weight.data_ptr(), 1 if weight.dtype == _F32 else 0, eps,
-                                        out_kind, scale_block, y.data_ptr(), _ld(y), None if scales is None else scales.data_ptr(),
-                                        ldscales, rstd.data_ptr(), _stream(x)), "o64_rmsnorm_bf16")
+        if residual is None:
+            add = (None, 0, None, 0)
+        else:
+            add = (residual.data_ptr(), _ld(residual), summed.data_ptr(), _ld(summed))
+        check(self.lib.o64_rmsnorm_bf16(self._h, T, N, x.data_ptr(), _ld(x), *add, weight.data_ptr(), 1 if weight.dtype is _F32 else 0, eps,
+                                        out_kind, scale_block, y.data_ptr(), _ld(y), p_scales, ldscales, rstd.data_ptr(), _stream(x)),
+              "o64_rmsnorm_bf16")
         return y, scales, (x if residual is None else summed), rstd
 
     def rms_norm_backward(self, dy, summed, weight, rstd, dresidual=None, dx=None):
         """Gradients of rms_norm: (dx, dweight).  dx [T,N] bf16 is the gradient of x and of the residual;
         `dresidual` is what arrives on the stream from beyond the norm (added to dx); dweight fp32."""
-        _want(dy, "dy", (_BF16,), (None, None))
-        T, N = dy.shape
-        _want(summed, "summed", (_BF16,), (T, N))
+        T, N = shape = _matrix(dy, "dy", _BF16).shape
+        _want(summed, "summed", (_BF16,), shape)
         _want(weight, "weight", (_BF16, _F32), (N,))
         _want(rstd, "rstd", (_F32,), (T,))
         dy, summed, weight, rstd = _rows(dy), _rows(summed), weight.contiguous(), rstd.contiguous()
         if dresidual is not None:
-            dresidual = _rows(_want(dresidual, "dresidual", (_BF16,), (T, N)))
-        dx = torch.empty((T, N), dtype=_BF16, device=dy.device) if dx is None else _out(_want(dx, "dx", (_BF16,), (T, N)), "dx")
-        dw = torch.empty((N,), dtype=_F32, device=dy.device)
-        ws = torch.empty((self.lib.o64_rmsnorm_bf16_backward_workspace(T, N) // 4,), dtype=_F32, device=dy.device)
+            dresidual = _rows(_want(dresidual, "dresidual", (_BF16,), shape))
+        dx = _new(dy, shape, _BF16) if dx is None else _out(_want(dx, "dx", (_BF16,), shape), "dx")
+        dw = dy.new_empty((N,), dtype=_F32)
+        ws = dy.new_empty((self.lib.o64_rmsnorm_bf16_backward_workspace(T, N) // 4,), dtype=_F32)
         check(self.lib.o64_rmsnorm_bf16_backward(self._h, T, N, dy.data_ptr(), _ld(dy), summed.data_ptr(), _ld(summed), weight.data_ptr(),
                                                  1 if weight.dtype == _F32 else 0, rstd.data_ptr(),
                                                  None if dresidual is None else dresidual.data_ptr(),
@@ -368,8 +386,7 @@ class Engine:
 
     def _block_operands(self, A8, scaleA, B8, scaleB, transB, swiglu, groups):
         """Checks an e4m3 product with block scales; returns (M, N, K, A8, scaleA, B8, scaleB) as the library reads them."""
-        _want(A8, "A8", (_E4M3,), (None, None))
-        M, K = A8.shape
+        M, K = _matrix(A8, "A8", _E4M3).shape
         lead = () if groups is None else (groups,)
         _want(B8, "B8", (_E4M3,), (*lead, None, K) if transB else (*lead, K, None))
         rows, cols = B8.shape[-2:]
@@ -393,8 +410,8 @@ class Engine:
         return out, scales
 
     @staticmethod
-    def _bf16_out(out, M, N, device):
-        return torch.empty((M, N), dtype=_BF16, device=device) if out is None else _out(_want(out, "out", (_BF16,), (M, N)), "out")
+    def _bf16_out(out, M, N, like):
+        return like.new_empty((M, N), dtype=_BF16) if out is None else _out(_want(out, "out", (_BF16,), (M, N)), "out")
 
     @staticmethod
     def _offsets(offsets, groups):
@@ -405,7 +422,7 @@ class Engine:
         """bf16 sum over blocks of 128 of K of scaleA[m,b] * scaleB[n/128,b] * (A8 @ B8^T in block b).  A8 [M,K],
         scaleA [M, ceil(K/128)]; B8 [N,K] (or [K,N]: transB False), scaleB one value per 128 x 128 of B8."""
         M, N, K, A8, scaleA, B8, scaleB = self._block_operands(A8, scaleA, B8, scaleB, transB, False, None)
-        out = self._bf16_out(out, M, N, A8.device)
+        out = self._bf16_out(out, M, N, A8)
         check(self.lib.o64_gemm_fp8_block(self._h, M, N, K, A8.data_ptr(), _ld(A8), scaleA.data_ptr(), _ld(scaleA), B8.data_ptr(), _ld(B8),
                                           1 if transB else 0, scaleB.data_ptr(), _ld(scaleB), out.data_ptr(), _ld(out), _stream(A8)),
               "o64_gemm_fp8_block")
@@ -425,21 +442,19 @@ class Engine:
     def gemm_grouped_bf16(self, A, offsets, B, transB=True, out=None):
         """A[rows of g] @ op(B[g]) for each group g: A [T,K] bf16 sorted by group, offsets int32 [G+1] on the
         device, B [G,N,K] (or [G,K,N]: transB False).  Rows outside offsets[0] .. offsets[G] are left as they are."""
-        _want(A, "A", (_BF16,), (None, None))
-        T, K = A.shape
+        T, K = _matrix(A, "A", _BF16).shape
         _want(B, "B", (_BF16,), (None, None, K) if transB else (None, K, None))
         G, N = B.shape[0], B.shape[1] if transB else B.shape[2]
         offsets = self._offsets(offsets, G)
         A, B = _tma(A), _tma(B)
-        out = self._bf16_out(out, T, N, A.device)
+        out = self._bf16_out(out, T, N, A)
         check(self.lib.o64_gemm_grouped_bf16(self._h, G, T, N, K, A.data_ptr(), _ld(A), offsets.data_ptr(), B.data_ptr(), _ld(B), _stride0(B),
                                              1 if transB else 0, out.data_ptr(), _ld(out), _stream(A)), "o64_gemm_grouped_bf16")
         return out
 
     def gemm_grouped_bf16_wgrad(self, dC, A, offsets, out_kind=_lib.OUT_BF16, out=None):
         """dC[rows of g]^T @ A[rows of g] for each group: dC [T,N], A [T,K] bf16 -> [G,N,K] bf16 or (OUT_F32) fp32."""
-        _want(dC, "dC", (_BF16,), (None, None))
-        T, N = dC.shape
+        T, N = _matrix(dC, "dC", _BF16).shape
         _want(A, "A", (_BF16,), (T, None))
         K = A.shape[1]
         if out_kind not in (_lib.OUT_BF16, _lib.OUT_F32):
@@ -463,7 +478,7 @@ class Engine:
             raise O64Error(_lib.ERR_RANK, f"B8: rank {B8.dim()}")
         T, N, K, A8, scaleA, B8, scaleB = self._block_operands(A8, scaleA, B8, scaleB, transB, False, B8.shape[0])
         offsets = self._offsets(offsets, B8.shape[0])
-        out = self._bf16_out(out, T, N, A8.device)
+        out = self._bf16_out(out, T, N, A8)
         check(self.lib.o64_gemm_grouped_fp8_block(self._h, B8.shape[0], T, N, K, A8.data_ptr(), _ld(A8), scaleA.data_ptr(), _ld(scaleA),
                                                   offsets.data_ptr(), B8.data_ptr(), _ld(B8), _stride0(B8), 1 if transB else 0,
                                                   scaleB.data_ptr(), _ld(scaleB), _stride0(scaleB), out.data_ptr(), _ld(out), _stream(A8)),

@@ -79,6 +79,29 @@ def test_e4m3(eng, T, N, block):
     check_e4m3(y, scales, h, size, block)
 
 
+MANY = [(1500, 2048), (1000, 4096), (1200, 5000), (601, 8192), (300, 16384), (890, 2056)]  # rows in a ring of bulk copies
+
+
+@pytest.mark.parametrize("T,N", MANY)
+@pytest.mark.parametrize("residual", [True, False], ids=["residual", "plain"])
+def test_many_rows(eng, T, N, residual):
+    x, r, w = data(T, N, T + N, residual, torch.bfloat16 if T % 3 else torch.float32)
+    x[17], w[5] = 0, 0
+    s, rstd, h, size = formula(x, r, w, 1e-6)
+    y, _, summed, got_rstd = eng.rms_norm(x, w, r)
+    assert ((y.double() - h).abs() <= BF16 * h.abs() + 2 * H * size).all()
+    assert ((got_rstd.double() - rstd).abs() <= H * rstd).all()
+    if residual:
+        assert torch.equal(summed, (x.float() + r.float()).to(torch.bfloat16))
+    y, scales, _, _ = eng.rms_norm(x, w, r, out_kind=o.OUT_E4M3)
+    check_e4m3(y, scales, h, size, 128)
+    if residual:  # in place, and rows apart
+        wide = torch.full((T, N + 8), 7.0, device="cuda", dtype=torch.bfloat16)
+        wide[:, :N] = r
+        y2, scales2, s2, _ = eng.rms_norm(x, w, wide[:, :N], out_kind=o.OUT_E4M3, summed=wide[:, :N])
+        assert torch.equal(y2.float(), y.float()) and torch.equal(scales2, scales) and torch.equal(s2, summed) and (wide[:, N:] == 7).all()
+
+
 def test_zero_rows_tiny_values_and_block_of_zeros(eng):
     x = torch.zeros((4, 300), device="cuda", dtype=torch.bfloat16)
     x[1] = 2.0 ** -120
@@ -135,7 +158,7 @@ def test_offsets_past_32_bits(eng):
 
 
 BACK = [(1, 1), (1, 4096), (3, 64), (5, 127), (130, 128), (64, 1000), (1000, 512), (445, 2141), (900, 4096), (50, 5000), (13, 8192), (3, 16392),
-        (2, 32768), (4, 32761)]
+        (2, 32768), (4, 32761), (2000, 2048), (1300, 5000), (601, 8192), (305, 16384), (888, 4104)]
 
 
 @pytest.mark.parametrize("T,N", BACK)
