@@ -59,6 +59,7 @@ struct GroupedParams {
     long long ldsc;
     const int *offsets;
     int vec_ok, tma_store;
+    int a_groups, b_groups;  // wgrad: the operands' columns are mapped in groups of 64
     int split;   // few rows: CTAs that share a tile's K blocks
     int sa_vec;  // the rows of scale_a are 16-byte aligned
     int *status;
@@ -86,7 +87,7 @@ int grouped_rows_launch(const GroupedCall &c, const GroupedParams &p);
 int grouped_zero_launch(const GroupedCall &c);
 
 int encode_3d(CUtensorMap *tm, int elem, const void *base, int64_t cols, int64_t rows, int64_t depth, int64_t ld, int64_t stride,
-              int box_cols, int box_rows, bool promote);
+              int box_cols, int box_rows, bool promote, int box_depth = 1);
 
 __device__ __forceinline__ void tma_load_3d_pair(uint32_t smem_dst, const void *tmap, int x, int y, int z, uint32_t bar) {
     asm volatile(
@@ -106,8 +107,9 @@ __device__ __forceinline__ void tma_store_3d(const void *tmap, uint32_t smem_src
                  : "memory");
 }
 
-// silu(g) * u
-__device__ __forceinline__ float silu_mul(float g, float u) { return g / (1.0f + __expf(-g)) * u; }
+// silu(g) * u.  exp and the division are the fast ones: together within 2^-20 of the value for |g| < 20, and
+// where exp(-g) passes 2^126 the result, below 1e-35 of u, is zero.
+__device__ __forceinline__ float silu_mul(float g, float u) { return __fdividef(g, 1.0f + __expf(-g)) * u; }
 
 // amax / 448, or 1 where that is no normal number (NaN stays NaN).
 __device__ __forceinline__ float block_scale_of(float amax) {

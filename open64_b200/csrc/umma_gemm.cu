@@ -355,14 +355,14 @@ int encode_c_bytes(CUtensorMap *tm, void *base, int64_t rows, int64_t cols, int6
 // 3-D tensor [depth][rows][cols] of `elem`-byte elements (1 or 2) with `ld` elements between rows and `stride`
 // between matrices; 128-byte swizzle; out-of-range elements read as zero and are not written.
 int encode_3d(CUtensorMap *tm, int elem, const void *base, int64_t cols, int64_t rows, int64_t depth, int64_t ld, int64_t stride,
-              int box_cols, int box_rows, bool promote) {
+              int box_cols, int box_rows, bool promote, int box_depth) {
     EncodeTiledFn fn = encode_tiled_fn();
     if (!fn) return O64_ERR_CUDA;
     const CUtensorMapDataType dt = elem == 2 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_UINT8;
-    if (depth <= 1) stride = rows * ld;  // never used
+    if (depth <= 1 && box_depth <= 1) stride = rows * ld;  // never used
     cuuint64_t dims[3] = {(cuuint64_t)cols, (cuuint64_t)rows, (cuuint64_t)depth};
     cuuint64_t strides[2] = {(cuuint64_t)ld * elem, (cuuint64_t)stride * elem};
-    cuuint32_t box[3] = {(cuuint32_t)box_cols, (cuuint32_t)box_rows, 1};
+    cuuint32_t box[3] = {(cuuint32_t)box_cols, (cuuint32_t)box_rows, (cuuint32_t)box_depth};
     cuuint32_t estr[3] = {1, 1, 1};
     CUresult r = fn(tm, dt, 3, const_cast<void *>(base), dims, strides, box, estr, CU_TENSOR_MAP_INTERLEAVE_NONE,
                     CU_TENSOR_MAP_SWIZZLE_128B, promote ? CU_TENSOR_MAP_L2_PROMOTION_L2_256B : CU_TENSOR_MAP_L2_PROMOTION_NONE,

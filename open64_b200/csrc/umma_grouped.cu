@@ -218,10 +218,20 @@ grouped_pair_kernel(const __grid_constant__ CUtensorMap tm_a, const __grid_const
                             mbar_arrive_expect_tx(full_bar(stage), 2 * kGpStageBytes);
                         else
                             mbar_arrive_cluster(full0);
+                        // (the maps count the columns in groups of 64 or, where the last group is not whole, one by one;
+                        // two boxes a stage instead of four: the issuing thread needs about 120 cycles for each)
+                        if (p.a_groups) {
+                            tma_load_3d_pair(a_dst, &tm_a, 0, row, m0 / kKnCols, bar);
+                        } else {
 #pragma unroll
-                        for (int c = 0; c < kKnGroups; ++c) {
-                            tma_load_2d_pair(a_dst + c * kKnGroupBytes, &tm_a, m0 + c * kKnCols, row, bar);
-                            tma_load_2d_pair(b_dst + c * kKnGroupBytes, &tm_b, n0 + (int)rank * 128 + c * kKnCols, row, bar);
+                            for (int c = 0; c < kKnGroups; ++c) tma_load_3d_pair(a_dst + c * kKnGroupBytes, &tm_a, m0 + c * kKnCols, row, 0, bar);
+                        }
+                        if (p.b_groups) {
+                            tma_load_3d_pair(b_dst, &tm_b, 0, row, (n0 + (int)rank * 128) / kKnCols, bar);
+                        } else {
+#pragma unroll
+                            for (int c = 0; c < kKnGroups; ++c)
+                                tma_load_3d_pair(b_dst + c * kKnGroupBytes, &tm_b, n0 + (int)rank * 128 + c * kKnCols, row, 0, bar);
                         }
                     }
                     __syncwarp();
@@ -337,57 +347,69 @@ grouped_pair_kernel(const __grid_constant__ CUtensorMap tm_a, const __grid_const
         bool ok = true;
         TileWalk walk;
         GroupTile t;
-        for (int i = pair_id; ok && next_tile<WGRAD>(p, walk, i, kBlockK, t); i += num_pairs) {
-            // lane l carries rows l, l + 32, l + 64, l + 96 and, for l < 2, one of the two runs of columns
+        // lane l carries rows l, l + 32, l + 64, l + 96 and, for l < 2, one of the two runs of columns; four K
+        // blocks at a time, the next four (of this tile or of the next one) always on their way
+        const float *sa[4], *sb = nullptr;
+        const long long sb_step = B_KN ? p.ldsb : 1;
+        float next[5][4];
+        int tile = pair_id, kb0 = 0;
+        auto fetch = [&]() __attribute__((always_inline)) {
+#pragma unroll
+            for (int r = 0; r < 4; ++r) {
+                if (p.sa_vec && kb0 + 4 <= t.kbs) {
+                    const float4 x = __ldg(reinterpret_cast<const float4 *>(sa[r] + kb0));
+                    next[r][0] = x.x, next[r][1] = x.y, next[r][2] = x.z, next[r][3] = x.w;
+                } else {
+#pragma unroll
+                    for (int u = 0; u < 4; ++u) next[r][u] = kb0 + u < t.kbs ? __ldg(sa[r] + kb0 + u) : 0.0f;
+                }
+            }
+#pragma unroll
+            for (int u = 0; u < 4; ++u) next[4][u] = lane < 2 && kb0 + u < t.kbs ? __ldg(sb + (kb0 + u) * sb_step) : 0.0f;
+        };
+        auto begin_tile = [&]() __attribute__((always_inline)) {
+            if (!next_tile<WGRAD>(p, walk, tile, kBlockK, t)) return false;
             const int n0 = t.nb * kOutN;
-            const float *sa[4];
 #pragma unroll
             for (int r = 0; r < 4; ++r)
                 sa[r] = p.scale_a + (long long)min(t.begin + t.mb * kGpTileM + (int)rank * kBlockM + r * 32 + lane, t.end - 1) * p.ldsa;
             // the block of 128 columns of C (SwiGLU: of gate, or of up) behind run `lane`
             const int blk = kSwiglu ? ((lane & 1 ? p.N + n0 : n0) >> 7) : min((n0 >> 7) + (lane & 1), (p.N - 1) >> 7);
-            const float *sb = p.scale_b + (long long)t.g * p.stride_sb + (B_KN ? (long long)blk : blk * p.ldsb);
-            const long long sb_step = B_KN ? p.ldsb : 1;
-            float next[5][4];
-            auto fetch = [&](int kb) __attribute__((always_inline)) {
+            sb = p.scale_b + (long long)t.g * p.stride_sb + (B_KN ? (long long)blk : blk * p.ldsb);
+            kb0 = 0;
+            fetch();
+            return true;
+        };
+        bool more = begin_tile();
+        while (ok && more) {
+            float now[5][4];
+            const int have = min(4, t.kbs - kb0);
 #pragma unroll
-                for (int r = 0; r < 4; ++r) {
-                    if (p.sa_vec && kb + 4 <= t.kbs) {
-                        const float4 x = __ldg(reinterpret_cast<const float4 *>(sa[r] + kb));
-                        next[r][0] = x.x, next[r][1] = x.y, next[r][2] = x.z, next[r][3] = x.w;
-                    } else {
+            for (int r = 0; r < 5; ++r)
 #pragma unroll
-                        for (int u = 0; u < 4; ++u) next[r][u] = kb + u < t.kbs ? __ldg(sa[r] + kb + u) : 0.0f;
-                    }
-                }
+                for (int u = 0; u < 4; ++u) now[r][u] = next[r][u];
+            kb0 += 4;
+            if (kb0 < t.kbs) {
+                fetch();
+            } else {
+                tile += num_pairs;
+                more = begin_tile();
+            }
 #pragma unroll
-                for (int u = 0; u < 4; ++u) next[4][u] = lane < 2 && kb + u < t.kbs ? __ldg(sb + (kb + u) * sb_step) : 0.0f;
-            };
-            fetch(0);
-#pragma unroll 1
-            for (int kb0 = 0; ok && kb0 < t.kbs; kb0 += 4) {
-                float now[5][4];
+            for (int u = 0; u < 4; ++u) {
+                if (u >= have) break;
+                ok = mbar_wait_bounded(scale_empty_bar(slot), phase ^ 1u, abort_flag, p.status, kWaitGroupScales, p.wait_ns);
+                ok = __all_sync(0xffffffffu, ok);
+                if (!ok) break;
+                float *dst = ring + slot * kGpScaleFloats;
 #pragma unroll
-                for (int r = 0; r < 5; ++r)
-#pragma unroll
-                    for (int u = 0; u < 4; ++u) now[r][u] = next[r][u];
-                fetch(kb0 + 4);
-#pragma unroll
-                for (int u = 0; u < 4; ++u) {
-                    if (kb0 + u >= t.kbs) break;
-                    ok = mbar_wait_bounded(scale_empty_bar(slot), phase ^ 1u, abort_flag, p.status, kWaitGroupScales, p.wait_ns);
-                    ok = __all_sync(0xffffffffu, ok);
-                    if (!ok) break;
-                    float *dst = ring + slot * kGpScaleFloats;
-#pragma unroll
-                    for (int r = 0; r < 4; ++r) dst[r * 32 + lane] = now[r][u];
-                    if (lane < 2) dst[128 + lane] = now[4][u];
-                    __syncwarp();
-                    if (lane == 0) mbar_arrive(scale_full_bar(slot));
-                    if (++slot == kGpScaleSlots) {
-                        slot = 0;
-                        phase ^= 1u;
-                    }
+                for (int r = 0; r < 4; ++r) dst[r * 32 + lane] = now[r][u];
+                if (lane < 2) dst[128 + lane] = now[4][u];
+                __syncwarp();
+                if (lane == 0) mbar_arrive(scale_full_bar(slot));
+                if (++slot == kGpScaleSlots) {
+                    slot = 0;
+                    phase ^= 1u;
                 }
             }
         }
@@ -421,11 +443,14 @@ grouped_pair_kernel(const __grid_constant__ CUtensorMap tm_a, const __grid_const
                 const float *ring = reinterpret_cast<const float *>(smem_gen + kGpScales);
 #pragma unroll 1
                 for (int kb = 0; kb < t.kbs; ++kb, ++uses) {
-                    if (lane == 0)
-                        ok = mbar_wait_bounded(scale_full_bar(slot), slot_phase, abort_flag, p.status, kWaitGroupScales, p.wait_ns) &&
-                             mbar_wait_bounded(acc_full_bar(uses & 1), (uint32_t)((uses >> 1) & 1), abort_flag, p.status,
-                                               kWaitGroupAccFull, p.wait_ns);
-                    ok = __shfl_sync(0xffffffffu, ok, 0);
+                    // the block's scales first: they are there long before its products are
+                    ok = mbar_wait_bounded(scale_full_bar(slot), slot_phase, abort_flag, p.status, kWaitGroupScales, p.wait_ns);
+                    const float s = ring[slot * kGpScaleFloats + quarter * 32 + lane];
+                    const float2 sb = *reinterpret_cast<const float2 *>(ring + slot * kGpScaleFloats + 128);
+                    const float f0 = s * sb.x, f1 = s * sb.y;
+                    ok = mbar_wait_bounded(acc_full_bar(uses & 1), (uint32_t)((uses >> 1) & 1), abort_flag, p.status, kWaitGroupAccFull,
+                                           p.wait_ns) && ok;
+                    ok = __all_sync(0xffffffffu, ok);
                     if (!ok) break;
                     tc_fence_after();
                     const uint32_t t_row = t_lane + (uint32_t)(uses & 1) * kGpTileN;
@@ -433,8 +458,6 @@ grouped_pair_kernel(const __grid_constant__ CUtensorMap tm_a, const __grid_const
                     uint32_t va[32], vb[32];
                     tmem_ld_32x32(t_row, va);
                     tmem_ld_32x32(t_row + 32, vb);
-                    const float s = ring[slot * kGpScaleFloats + quarter * 32 + lane];
-                    const float2 sb = *reinterpret_cast<const float2 *>(ring + slot * kGpScaleFloats + 128);
                     auto add = [&](const uint32_t(&v)[32], float2(&sum)[32], int at, float f) __attribute__((always_inline)) {
 #pragma unroll
                         for (int j = 0; j < 16; ++j)
@@ -442,9 +465,9 @@ grouped_pair_kernel(const __grid_constant__ CUtensorMap tm_a, const __grid_const
                                                      make_float2(f, f), sum[at + j]);
                     };
                     tmem_ld_wait();
-                    add(va, acc[0], 0, s * sb.x);
+                    add(va, acc[0], 0, f0);
                     tmem_ld_32x32(t_row + 128, va);
-                    add(vb, acc[0], 16, s * sb.x);
+                    add(vb, acc[0], 16, f0);
                     tmem_ld_32x32(t_row + 160, vb);
                     tmem_ld_wait();
                     tc_fence_before();  // everything of this buffer is in registers
@@ -453,8 +476,8 @@ grouped_pair_kernel(const __grid_constant__ CUtensorMap tm_a, const __grid_const
                         mbar_arrive_cluster(map_to_cta(acc_empty_bar(uses & 1), 0));
                         mbar_arrive(scale_empty_bar(slot));
                     }
-                    add(va, acc[1], 0, s * sb.y);
-                    add(vb, acc[1], 16, s * sb.y);
+                    add(va, acc[1], 0, f1);
+                    add(vb, acc[1], 16, f1);
                     if (++slot == kGpScaleSlots) {
                         slot = 0;
                         slot_phase ^= 1u;
@@ -662,6 +685,7 @@ static GroupedParams grouped_params(const GroupedCall &c) {
     p.vec_ok = (reinterpret_cast<uintptr_t>(c.C) & 15u) == 0 && (c.ldc * elem) % 16 == 0 && (c.stride_c * elem) % 16 == 0;
     p.tma_store = 0;
     p.split = 1;
+    p.a_groups = p.b_groups = 0;
     p.sa_vec = (reinterpret_cast<uintptr_t>(c.scale_a) & 15u) == 0 && c.ldsa % 4 == 0;
     p.num_m_tiles = (int)((c.N + kGpTileM - 1) / kGpTileM);
     const int out_n = gepi_swiglu(c.epi) ? kGpTileN / 2 : kGpTileN;
@@ -708,8 +732,15 @@ int grouped_launch(const GroupedCall &c) {
     CUtensorMap ta, tb, tc;
     int rc;
     if (c.wgrad) {
-        rc = encode_2d(&ta, c.kind, c.A, c.T, c.N, c.lda, 64, 64);
-        if (!rc) rc = encode_2d(&tb, c.kind, c.B, c.T, c.K, c.ldb, 64, 64);
+        // an operand whose columns come in whole groups of 64 as [group][row][64]: a box of two groups is what a
+        // CTA holds of it.  (A last group that is not whole would be read past the rows' ends.)
+        auto encode = [&](CUtensorMap *tm, const void *base, int64_t cols, int64_t ld, int *groups) {
+            *groups = cols % 64 == 0;
+            return *groups ? encode_3d(tm, 2, base, 64, c.T, cols / 64, ld, 64, 64, 64, true, 2)
+                           : encode_3d(tm, 2, base, cols, c.T, 1, ld, 0, 64, 64, true);
+        };
+        rc = encode(&ta, c.A, c.N, c.lda, &p.a_groups);
+        if (!rc) rc = encode(&tb, c.B, c.K, c.ldb, &p.b_groups);
     } else {
         const int64_t b_out = gepi_swiglu(c.epi) ? 2 * c.N : c.N;
         rc = encode_2d(&ta, c.kind, c.A, c.T, c.K, c.lda, block_k, kBlockM);

@@ -265,52 +265,65 @@ grouped_rows_kernel(const __grid_constant__ CUtensorMap tm_x, const __grid_const
         bool ok = true;
         RowsWalk walk;
         RowsTile t;
-        for (int i = first; ok && next_rows_tile<TOK>(p, walk, i, t); i += step) {
-            const float *sa[kPer];
+        // four K blocks at a time, the next four (of this tile or of the next one) always on their way
+        const float *sa[kPer], *sb0 = nullptr, *sb1 = nullptr;
+        float next[kPer][4], b0[4], b1[4];
+        int tile = first, kb0 = kb_begin;
+        auto fetch = [&]() __attribute__((always_inline)) {
+#pragma unroll
+            for (int u = 0; u < 4; ++u) {
+                const bool in = kb0 + u < kb_end;
+#pragma unroll
+                for (int r = 0; r < kPer; ++r) next[r][u] = in ? __ldg(sa[r] + kb0 + u) : 0.0f;
+                b0[u] = in ? __ldg(sb0 + kb0 + u) : 0.0f;
+                b1[u] = kSwiglu && in ? __ldg(sb1 + kb0 + u) : 0.0f;
+            }
+        };
+        auto begin_tile = [&]() __attribute__((always_inline)) {
+            if (!next_rows_tile<TOK>(p, walk, tile, t)) return false;
 #pragma unroll
             for (int r = 0; r < kPer; ++r) sa[r] = p.scale_a + (long long)min(t.begin + r * 32 + lane, t.end - 1) * p.ldsa;
             const float *sb = p.scale_b + (long long)t.g * p.stride_sb;
-            const float *sb0 = sb + t.nb * p.ldsb, *sb1 = sb + (long long)((p.N >> 7) + t.nb) * p.ldsb;
-            float next[kPer][4], b0[4], b1[4];
-            auto fetch = [&](int kb) __attribute__((always_inline)) {
+            sb0 = sb + t.nb * p.ldsb;
+            sb1 = sb + (long long)((p.N >> 7) + t.nb) * p.ldsb;
+            kb0 = kb_begin;
+            fetch();
+            return true;
+        };
+        bool more = kb_begin < kb_end && begin_tile();
+        while (ok && more) {
+            float now[NB][kPer][4];
+            const int got = min(4, kb_end - kb0);
+#pragma unroll
+            for (int r = 0; r < kPer; ++r)
 #pragma unroll
                 for (int u = 0; u < 4; ++u) {
-                    const bool in = kb + u < kb_end;
-#pragma unroll
-                    for (int r = 0; r < kPer; ++r) next[r][u] = in ? __ldg(sa[r] + kb + u) : 0.0f;
-                    b0[u] = in ? __ldg(sb0 + kb + u) : 0.0f;
-                    b1[u] = kSwiglu && in ? __ldg(sb1 + kb + u) : 0.0f;
+                    now[0][r][u] = next[r][u] * b0[u];
+                    if constexpr (kSwiglu) now[NB - 1][r][u] = next[r][u] * b1[u];
                 }
-            };
-            if (kb_begin < kb_end) fetch(kb_begin);
-#pragma unroll 1
-            for (int kb0 = kb_begin; ok && kb0 < kb_end; kb0 += 4) {
-                float now[NB][kPer][4];
+            kb0 += 4;
+            if (kb0 < kb_end) {
+                fetch();
+            } else {
+                tile += step;
+                more = begin_tile();
+            }
 #pragma unroll
-                for (int r = 0; r < kPer; ++r)
+            for (int u = 0; u < 4; ++u) {
+                if (u >= got) break;
+                ok = mbar_wait_bounded(scale_empty_bar(slot), phase ^ 1u, abort_flag, p.status, kWaitGroupScales, p.wait_ns);
+                ok = __all_sync(0xffffffffu, ok);
+                if (!ok) break;
 #pragma unroll
-                    for (int u = 0; u < 4; ++u) {
-                        now[0][r][u] = next[r][u] * b0[u];
-                        if constexpr (kSwiglu) now[NB - 1][r][u] = next[r][u] * b1[u];
-                    }
-                fetch(kb0 + 4);
+                for (int b = 0; b < NB; ++b)
 #pragma unroll
-                for (int u = 0; u < 4; ++u) {
-                    if (kb0 + u >= kb_end) break;
-                    ok = mbar_wait_bounded(scale_empty_bar(slot), phase ^ 1u, abort_flag, p.status, kWaitGroupScales, p.wait_ns);
-                    ok = __all_sync(0xffffffffu, ok);
-                    if (!ok) break;
-#pragma unroll
-                    for (int b = 0; b < NB; ++b)
-#pragma unroll
-                        for (int r = 0; r < kPer; ++r)
-                            if (r * 32 + lane < TOK) ring[(slot * NB + b) * TOK + r * 32 + lane] = now[b][r][u];
-                    __syncwarp();
-                    if (lane == 0) mbar_arrive(scale_full_bar(slot));
-                    if (++slot == kGrScaleSlots) {
-                        slot = 0;
-                        phase ^= 1u;
-                    }
+                    for (int r = 0; r < kPer; ++r)
+                        if (r * 32 + lane < TOK) ring[(slot * NB + b) * TOK + r * 32 + lane] = now[b][r][u];
+                __syncwarp();
+                if (lane == 0) mbar_arrive(scale_full_bar(slot));
+                if (++slot == kGrScaleSlots) {
+                    slot = 0;
+                    phase ^= 1u;
                 }
             }
         }
