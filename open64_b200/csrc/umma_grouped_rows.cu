@@ -47,7 +47,7 @@ struct RowsLayout {
     static constexpr uint32_t kTmemCols = kGrBufs * NB * TOK;
     static_assert(kDynamic <= 227 * 1024, "shared memory");
     static_assert(kStageBytes % 1024 == 0 && kWBytes % 1024 == 0, "swizzle atoms");
-    static_assert(kRing >= 128 * NB * TOK * 4, "the ring receives the partial sums");
+    static_assert(kRing >= 128 * (NB + 1) * TOK * 4, "the ring receives the partial sums");
     static_assert(kTmemCols <= 512 && (kTmemCols & (kTmemCols - 1)) == 0 && kTmemCols >= 32, "TMEM columns");
 };
 
@@ -340,29 +340,20 @@ grouped_rows_kernel(const __grid_constant__ CUtensorMap tm_x, const __grid_const
         bool ok = true;
         RowsWalk walk;
         RowsTile t;
-        auto load_add = [&](uint32_t taddr, const float *s) __attribute__((always_inline)) {
-            // acc += v (s == NULL), or acc += s[j] * v[j]; the buffer is released once everything is in registers
-            uint32_t v[TOK];
+        constexpr int kCols = TOK < 64 ? TOK : 64;  // accumulator columns in flight
+        auto fetch = [&](uint32_t (&v)[kCols], int half) __attribute__((always_inline)) {
+            const uint32_t taddr = t_lane + (uses % kGrBufs) * NB * TOK + half * kCols;
             if constexpr (TOK == 16) {
-                tmem_ld_32x16(taddr, *reinterpret_cast<uint32_t(*)[16]>(&v[0]));
+                tmem_ld_32x16(taddr, v);
             } else {
 #pragma unroll
-                for (int c = 0; c < TOK / 32; ++c) tmem_ld_32x32(taddr + 32 * c, *reinterpret_cast<uint32_t(*)[32]>(&v[32 * c]));
+                for (int c = 0; c < kCols / 32; ++c) tmem_ld_32x32(taddr + 32 * c, *reinterpret_cast<uint32_t(*)[32]>(&v[32 * c]));
             }
-            tmem_ld_wait();
+        };
+        auto release = [&]() __attribute__((always_inline)) {
             tc_fence_before();
             __syncwarp();
             if (lane == 0) mbar_arrive(acc_empty_bar(uses % kGrBufs));
-#pragma unroll
-            for (int j = 0; j < TOK / 2; ++j) {
-                const float2 x = make_float2(__uint_as_float(v[2 * j]), __uint_as_float(v[2 * j + 1]));
-                if (s) {
-                    const float2 f = *reinterpret_cast<const float2 *>(s + 2 * j);
-                    acc[j] = __ffma2_rn(x, f, acc[j]);
-                } else {
-                    acc[j] = x;
-                }
-            }
         };
         for (int i = first; ok && next_rows_tile<TOK>(p, walk, i, t); i += step, ++tiles) {
 #pragma unroll
@@ -370,14 +361,36 @@ grouped_rows_kernel(const __grid_constant__ CUtensorMap tm_x, const __grid_const
             if constexpr (kScaled) {
 #pragma unroll 1
                 for (int kb = kb_begin; kb < kb_end; ++kb, ++uses) {
-                    if (lane == 0)
-                        ok = mbar_wait_bounded(scale_full_bar(slot), slot_phase, abort_flag, p.status, kWaitGroupScales, p.wait_ns) &&
-                             mbar_wait_bounded(acc_full_bar(uses % kGrBufs), (uses / kGrBufs) & 1, abort_flag, p.status, kWaitGroupAccFull,
-                                               p.wait_ns);
-                    ok = __shfl_sync(0xffffffffu, ok, 0);
+                    // the block's scales are there long before its products are
+                    ok = mbar_wait_bounded(scale_full_bar(slot), slot_phase, abort_flag, p.status, kWaitGroupScales, p.wait_ns);
+                    ok = mbar_wait_bounded(acc_full_bar(uses % kGrBufs), (uses / kGrBufs) & 1, abort_flag, p.status, kWaitGroupAccFull,
+                                           p.wait_ns) && ok;
+                    ok = __all_sync(0xffffffffu, ok);
                     if (!ok) break;
                     tc_fence_after();
-                    load_add(t_lane + (uses % kGrBufs) * NB * TOK, ring + (slot * NB + blk) * TOK);
+#pragma unroll
+                    for (int half = 0; half < TOK / kCols; ++half) {
+                        uint32_t v[kCols];
+                        fetch(v, half);
+                        // 16 rows' scales at a time (all of them at once would not fit the registers)
+                        const float4 *s = reinterpret_cast<const float4 *>(ring + (slot * NB + blk) * TOK + half * kCols);
+                        float4 f[4];
+#pragma unroll
+                        for (int q = 0; q < 4; ++q) f[q] = s[q];
+                        tmem_ld_wait();
+                        if (half == TOK / kCols - 1) release();
+#pragma unroll
+                        for (int c = 0; c < kCols / 16; ++c) {
+#pragma unroll
+                            for (int q = 0; q < 4; ++q) {
+                                const int x = c * 16 + 4 * q;
+                                float2 *sum = acc + (half * kCols + x) / 2;
+                                sum[0] = __ffma2_rn(make_float2(__uint_as_float(v[x]), __uint_as_float(v[x + 1])), make_float2(f[q].x, f[q].y), sum[0]);
+                                sum[1] = __ffma2_rn(make_float2(__uint_as_float(v[x + 2]), __uint_as_float(v[x + 3])), make_float2(f[q].z, f[q].w), sum[1]);
+                                if (c + 1 < kCols / 16) f[q] = s[(c + 1) * 4 + q];
+                            }
+                        }
+                    }
                     __syncwarp();
                     if (lane == 0) mbar_arrive(scale_empty_bar(slot));
                     if (++slot == kGrScaleSlots) {
@@ -386,13 +399,20 @@ grouped_rows_kernel(const __grid_constant__ CUtensorMap tm_x, const __grid_const
                     }
                 }
             } else if (kb_begin < kb_end) {
-                if (lane == 0)
-                    ok = mbar_wait_bounded(acc_full_bar(uses % kGrBufs), (uses / kGrBufs) & 1, abort_flag, p.status, kWaitGroupAccFull,
-                                           p.wait_ns);
-                ok = __shfl_sync(0xffffffffu, ok, 0);
+                ok = mbar_wait_bounded(acc_full_bar(uses % kGrBufs), (uses / kGrBufs) & 1, abort_flag, p.status, kWaitGroupAccFull, p.wait_ns);
+                ok = __all_sync(0xffffffffu, ok);
                 if (!ok) break;
                 tc_fence_after();
-                load_add(t_lane + (uses % kGrBufs) * NB * TOK, nullptr);
+#pragma unroll
+                for (int half = 0; half < TOK / kCols; ++half) {
+                    uint32_t v[kCols];
+                    fetch(v, half);
+                    tmem_ld_wait();
+                    if (half == TOK / kCols - 1) release();
+#pragma unroll
+                    for (int j = 0; j < kCols / 2; ++j)
+                        acc[half * kCols / 2 + j] = make_float2(__uint_as_float(v[2 * j]), __uint_as_float(v[2 * j + 1]));
+                }
                 ++uses;
             }
             if (!ok) break;
@@ -474,29 +494,50 @@ grouped_rows_kernel(const __grid_constant__ CUtensorMap tm_x, const __grid_const
         // ---- partial sums of one tile: rows r of it belong to CTA r / (TOK / S) of the cluster ----
         __syncwarp();
         cluster_sync_all();  // every ring is idle
-        const int per = TOK / S;
-        const uint32_t recv = smem_base;  // [rank][per][128]
+        const int shift = __ffs(TOK / S) - 1, per = 1 << shift;  // S and TOK are powers of two
+        const uint32_t recv = smem_base;  // [rank][per][NB * 128]
+        const int n_in = (warp & 3) * 32 + lane;
         if (warp >= 4 && have) {
-            const int n_in = (warp & 3) * 32 + lane;
+            const int at = (warp - 4) / 4 * 128 + n_in;
 #pragma unroll
-            for (int j = 0; j < TOK; ++j) {
-                const int owner = j / per;
-                st_cluster_f32(map_to_cta(recv, owner) + ((rank * per + j % per) * 128 + n_in) * 4, (j & 1) ? acc[j / 2].y : acc[j / 2].x);
-            }
+            for (int j = 0; j < TOK; ++j)
+                st_cluster_f32(map_to_cta(recv, j >> shift) + (((rank << shift) + (j & (per - 1))) * (NB * 128) + at) * 4,
+                               (j & 1) ? acc[j / 2].y : acc[j / 2].x);
         }
         __syncwarp();
         cluster_sync_all();
-        if (warp >= 4 && have) {
-            const int n_in = (warp & 3) * 32 + lane;
-            const int col = last.nb * 128 + n_in;
-            const float *got = reinterpret_cast<const float *>(smem_gen);
-            for (int j = 0; j < per; ++j) {
-                const int row = last.begin + rank * per + j;
-                if (row >= last.end || col >= p.N) break;
-                float sum = 0.0f;
-                for (int r = 0; r < S; ++r) sum += got[(r * per + j) * 128 + n_in];
-                static_cast<__nv_bfloat16 *>(p.C)[(long long)row * p.ldc + col] = __float2bfloat16_rn(sum);
+        const bool mine = warp >= 4 && warp < 8 && have;
+        const int col = mine ? last.nb * 128 + n_in : 0;
+        const int row0 = mine ? last.begin + (rank << shift) : 0;
+        const int rows = mine ? min(per, last.end - row0) : 0;
+        const float *got = reinterpret_cast<const float *>(smem_gen) + n_in;
+        float *h_buf = reinterpret_cast<float *>(smem_gen) + TOK * NB * 128 + n_in;  // [per][128]
+        auto total = [&](int j, int blk) {
+            float sum = 0.0f;
+            for (int r = 0; r < S; ++r) sum += got[((r << shift) + j) * (NB * 128) + blk * 128];
+            return sum;
+        };
+        if constexpr (EPI == GEPI_SWIGLU_E4M3) {
+            uint32_t *amax = reinterpret_cast<uint32_t *>(smem_gen + L::kAmax);  // [4][TOK]
+            for (int j = 0; j < rows; ++j) {
+                const float h = silu_mul(total(j, 0), total(j, 1));
+                h_buf[j * 128] = h;
+                const uint32_t m = __reduce_max_sync(0xffffffffu, __float_as_uint(h) & 0x7fffffffu);
+                if (lane == 0) amax[(warp & 3) * TOK + j] = m;
             }
+            __syncthreads();
+            for (int j = 0; j < rows; ++j) {
+                const uint32_t m = max(max(amax[j], amax[TOK + j]), max(amax[2 * TOK + j], amax[3 * TOK + j]));
+                const float scale = block_scale_of(__uint_as_float(m));
+                static_cast<uint8_t *>(p.C)[(long long)(row0 + j) * p.ldc + col] =
+                    (uint8_t)__nv_cvt_float_to_fp8(h_buf[j * 128] * (1.0f / scale), __NV_SATFINITE, __NV_E4M3);
+                if (warp == 4 && lane == 0) p.scale_c[(long long)(row0 + j) * p.ldsc + last.nb] = scale;
+            }
+        } else if (col < p.N) {
+            __nv_bfloat16 *dst = static_cast<__nv_bfloat16 *>(p.C) + (long long)row0 * p.ldc + col;
+#pragma unroll 4
+            for (int j = 0; j < rows; ++j)
+                dst[j * p.ldc] = __float2bfloat16_rn(kSwiglu ? silu_mul(total(j, 0), total(j, 1)) : total(j, 0));
         }
     }
 
@@ -539,10 +580,9 @@ static int launch_rows(const GroupedCall &c, GroupedParams p) {
     if (most > INT32_MAX - 4 * c.num_sms) return O64_ERR_RANK;
     const long long tiles = c.offsets ? most : (c.T + TOK - 1) / TOK * p.num_n_tiles;
     // Too few tiles for the GPU: the K blocks of each are divided over a cluster, as long as a CTA keeps four
-    // of them.  (SwiGLU tiles already carry two weight blocks.)
+    // of them.
     int S = 1;
-    if (NB == 1)
-        while (S < 8 && tiles * S * 2 <= c.num_sms && p.num_k_blocks >= 4 * S * 2) S *= 2;
+    while (S < 8 && tiles * S * 2 <= c.num_sms && p.num_k_blocks >= 4 * S * 2) S *= 2;
     p.split = S;
     const int grid = (int)(S > 1 ? tiles * S : (tiles < c.num_sms ? tiles : c.num_sms));
     cudaLaunchConfig_t cfg = {};
@@ -578,6 +618,8 @@ static int launch_rows_tok(const GroupedCall &c, const GroupedParams &p) {
     const int64_t mean = (c.T + groups - 1) / groups;
     if (mean <= 16) return launch_rows<KIND, EPI, 16>(c, p);
     if (mean <= 32) return launch_rows<KIND, EPI, 32>(c, p);
+    if constexpr (KIND == MMA_F8F6F4 && !gepi_swiglu(EPI))
+        if (mean > 64) return launch_rows<KIND, EPI, 128>(c, p);
     return launch_rows<KIND, EPI, 64>(c, p);
 }
 
