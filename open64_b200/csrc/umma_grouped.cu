@@ -287,7 +287,9 @@ grouped_pair_kernel(const __grid_constant__ CUtensorMap tm_a, const __grid_const
             uint32_t ready = mbar_test_wait(full_bar(0), 0);
             TileWalk walk;
             GroupTile t;
+            uint32_t acc_ready = 0;
             auto take = [&] {
+                if (!acc_ready)
                 ok = mbar_wait_bounded(acc_empty_bar(uses & 1), (uint32_t)((uses >> 1) & 1) ^ 1u, abort_flag, p.status,
                                        kWaitGroupAccEmpty, p.wait_ns);
                 ok = __all_sync(0xffffffffu, ok);
@@ -308,6 +310,7 @@ grouped_pair_kernel(const __grid_constant__ CUtensorMap tm_a, const __grid_const
                     const int next_stage = (stage + 1 == kGpStages) ? 0 : stage + 1;
                     const uint32_t next_phase = (stage + 1 == kGpStages) ? (phase ^ 1u) : phase;
                     const uint32_t next_ready = mbar_test_wait(full_bar(next_stage), next_phase);
+                    if (kScaled) acc_ready = mbar_test_wait(acc_empty_bar((uses + 1) & 1), (uint32_t)(((uses + 1) >> 1) & 1) ^ 1u);
                     tc_fence_after();
                     const uint32_t a_addr = smem_base + stage * kGpStageBytes;
                     const uint32_t b_addr = a_addr + kABytes;
@@ -441,10 +444,11 @@ grouped_pair_kernel(const __grid_constant__ CUtensorMap tm_a, const __grid_const
 
             if constexpr (kScaled) {
                 const float *ring = reinterpret_cast<const float *>(smem_gen + kGpScales);
+                uint32_t scale_ready = 0;  // the next block's scales, probed while this one is added
 #pragma unroll 1
                 for (int kb = 0; kb < t.kbs; ++kb, ++uses) {
                     // the block's scales first: they are there long before its products are
-                    ok = mbar_wait_bounded(scale_full_bar(slot), slot_phase, abort_flag, p.status, kWaitGroupScales, p.wait_ns);
+                    if (!scale_ready) ok = mbar_wait_bounded(scale_full_bar(slot), slot_phase, abort_flag, p.status, kWaitGroupScales, p.wait_ns);
                     const float s = ring[slot * kGpScaleFloats + quarter * 32 + lane];
                     const float2 sb = *reinterpret_cast<const float2 *>(ring + slot * kGpScaleFloats + 128);
                     const float f0 = s * sb.x, f1 = s * sb.y;
@@ -476,12 +480,13 @@ grouped_pair_kernel(const __grid_constant__ CUtensorMap tm_a, const __grid_const
                         mbar_arrive_cluster(map_to_cta(acc_empty_bar(uses & 1), 0));
                         mbar_arrive(scale_empty_bar(slot));
                     }
-                    add(va, acc[1], 0, f1);
-                    add(vb, acc[1], 16, f1);
                     if (++slot == kGpScaleSlots) {
                         slot = 0;
                         slot_phase ^= 1u;
                     }
+                    scale_ready = mbar_test_wait(scale_full_bar(slot), slot_phase);
+                    add(va, acc[1], 0, f1);
+                    add(vb, acc[1], 16, f1);
                 }
             } else if (t.kbs > 0) {
                 if (lane == 0)

@@ -16,6 +16,7 @@
 #include <cstdio>
 #include <cstdlib>
 #include <cstring>
+#include <type_traits>
 
 #include "grouped.cuh"
 
@@ -209,23 +210,30 @@ grouped_rows_kernel(const __grid_constant__ CUtensorMap tm_x, const __grid_const
         bool ok = true;
         RowsWalk walk;
         RowsTile t;
-        auto take = [&] {
-            ok = mbar_wait_bounded(acc_empty_bar(uses % kGrBufs), ((uses / kGrBufs) & 1) ^ 1u, abort_flag, p.status, kWaitGroupAccEmpty,
-                                   p.wait_ns);
-            ok = __all_sync(0xffffffffu, ok);
-            tc_fence_after();
+        // the barriers of the next K block are probed before this one's MMAs are issued: a probe takes about 100
+        // cycles, and a loop that waits for its two in turn took 590 a block, 260 of them for the issue
+        uint32_t acc_ready = 1, full_ready = mbar_test_wait(full_bar(0), 0);
+        auto take = [&]() __attribute__((always_inline)) {
+            if (!acc_ready)
+                ok = mbar_wait_bounded(acc_empty_bar(uses % kGrBufs), ((uses / kGrBufs) & 1) ^ 1u, abort_flag, p.status, kWaitGroupAccEmpty,
+                                       p.wait_ns);
         };
         for (int i = first; ok && next_rows_tile<TOK>(p, walk, i, t); i += step) {
             if (kb_begin == kb_end) continue;
-            if (!kScaled) take();
+            if (!kScaled) {
+                acc_ready = 0;
+                take();
+            }
             for (int kb = kb_begin; ok && kb < kb_end; ++kb) {
-                if (kScaled) {
-                    take();
-                    if (!ok) break;
-                }
-                ok = mbar_wait_bounded(full_bar(stage), phase, abort_flag, p.status, kWaitGroupFull, p.wait_ns);
+                if (kScaled) take();
+                if (!full_ready)
+                    ok = mbar_wait_bounded(full_bar(stage), phase, abort_flag, p.status, kWaitGroupFull, p.wait_ns) && ok;
                 ok = __all_sync(0xffffffffu, ok);
                 if (!ok) break;
+                const int next_stage = stage + 1 == L::kStages ? 0 : stage + 1;
+                const uint32_t next_phase = stage + 1 == L::kStages ? phase ^ 1u : phase;
+                if (kScaled) acc_ready = mbar_test_wait(acc_empty_bar((uses + 1) % kGrBufs), (((uses + 1) / kGrBufs) & 1) ^ 1u);
+                full_ready = mbar_test_wait(full_bar(next_stage), next_phase);
                 tc_fence_after();
                 const uint32_t w_addr = smem_base + stage * L::kStageBytes;
                 const uint64_t x_desc = make_smem_desc(w_addr + L::kWBytes, 16, 1024);
@@ -244,10 +252,8 @@ grouped_rows_kernel(const __grid_constant__ CUtensorMap tm_x, const __grid_const
                 }
                 __syncwarp();
                 if (kScaled) ++uses;
-                if (++stage == L::kStages) {
-                    stage = 0;
-                    phase ^= 1u;
-                }
+                stage = next_stage;
+                phase = next_phase;
             }
             if (!kScaled) {
                 if (ok && leader) tc_commit(acc_full_bar(uses % kGrBufs));
@@ -341,8 +347,8 @@ grouped_rows_kernel(const __grid_constant__ CUtensorMap tm_x, const __grid_const
         RowsWalk walk;
         RowsTile t;
         constexpr int kCols = TOK < 64 ? TOK : 64;  // accumulator columns in flight
-        auto fetch = [&](uint32_t (&v)[kCols], int half) __attribute__((always_inline)) {
-            const uint32_t taddr = t_lane + (uses % kGrBufs) * NB * TOK + half * kCols;
+        auto fetch = [&](uint32_t (&v)[kCols], uint32_t use, int half) __attribute__((always_inline)) {
+            const uint32_t taddr = t_lane + (use % kGrBufs) * NB * TOK + half * kCols;
             if constexpr (TOK == 16) {
                 tmem_ld_32x16(taddr, v);
             } else {
@@ -359,45 +365,85 @@ grouped_rows_kernel(const __grid_constant__ CUtensorMap tm_x, const __grid_const
 #pragma unroll
             for (int j = 0; j < TOK / 2; ++j) acc[j] = make_float2(0.0f, 0.0f);
             if constexpr (kScaled) {
-#pragma unroll 1
-                for (int kb = kb_begin; kb < kb_end; ++kb, ++uses) {
-                    // the block's scales are there long before its products are
-                    ok = mbar_wait_bounded(scale_full_bar(slot), slot_phase, abort_flag, p.status, kWaitGroupScales, p.wait_ns);
-                    ok = mbar_wait_bounded(acc_full_bar(uses % kGrBufs), (uses / kGrBufs) & 1, abort_flag, p.status, kWaitGroupAccFull,
-                                           p.wait_ns) && ok;
+                // U K blocks at a time: their waits and their way out of tensor memory overlap.  The barriers of the
+                // next ones are probed while these are added.
+                auto scales_there = [&](int u) __attribute__((always_inline)) {
+                    return mbar_test_wait(scale_full_bar((slot + u) % kGrScaleSlots), slot + u < kGrScaleSlots ? slot_phase : slot_phase ^ 1u);
+                };
+                auto sums_there = [&](int u) __attribute__((always_inline)) {
+                    return mbar_test_wait(acc_full_bar((uses + u) % kGrBufs), ((uses + u) / kGrBufs) & 1);
+                };
+                uint32_t ready_s = 0, ready_a = 0;  // (of the first of the next blocks)
+                auto blocks = [&](auto count) __attribute__((always_inline)) {
+                    constexpr int U = decltype(count)::value;
+#pragma unroll
+                    for (int u = 0; u < U; ++u) {
+                        const int sl = (slot + u) % kGrScaleSlots;
+                        if (u > 0 || !ready_s)
+                            ok = mbar_wait_bounded(scale_full_bar(sl), slot + u < kGrScaleSlots ? slot_phase : slot_phase ^ 1u, abort_flag, p.status,
+                                                   kWaitGroupScales, p.wait_ns) && ok;
+                        if (u > 0 || !ready_a)
+                            ok = mbar_wait_bounded(acc_full_bar((uses + u) % kGrBufs), ((uses + u) / kGrBufs) & 1, abort_flag, p.status,
+                                                   kWaitGroupAccFull, p.wait_ns) && ok;
+                    }
                     ok = __all_sync(0xffffffffu, ok);
-                    if (!ok) break;
+                    if (!ok) return;
                     tc_fence_after();
 #pragma unroll
                     for (int half = 0; half < TOK / kCols; ++half) {
-                        uint32_t v[kCols];
-                        fetch(v, half);
-                        // 16 rows' scales at a time (all of them at once would not fit the registers)
-                        const float4 *s = reinterpret_cast<const float4 *>(ring + (slot * NB + blk) * TOK + half * kCols);
-                        float4 f[4];
+                        uint32_t v[U][kCols];
 #pragma unroll
-                        for (int q = 0; q < 4; ++q) f[q] = s[q];
+                        for (int u = 0; u < U; ++u) fetch(v[u], uses + u, half);
+                        // the first 16 rows' scales of each block set out with the sums
+                        const float4 *s[U];
+                        float4 f[U][4];
+#pragma unroll
+                        for (int u = 0; u < U; ++u) {
+                            s[u] = reinterpret_cast<const float4 *>(ring + (((slot + u) % kGrScaleSlots) * NB + blk) * TOK + half * kCols);
+#pragma unroll
+                            for (int q = 0; q < 4; ++q) f[u][q] = s[u][q];
+                        }
                         tmem_ld_wait();
-                        if (half == TOK / kCols - 1) release();
+                        if (half == TOK / kCols - 1) {
+                            tc_fence_before();
+                            __syncwarp();
+                            if (lane == 0) {
 #pragma unroll
-                        for (int c = 0; c < kCols / 16; ++c) {
+                                for (int u = 0; u < U; ++u) mbar_arrive(acc_empty_bar((uses + u) % kGrBufs));
+                            }
+                            ready_s = scales_there(U);
+                            ready_a = sums_there(U);
+                        }
 #pragma unroll
-                            for (int q = 0; q < 4; ++q) {
-                                const int x = c * 16 + 4 * q;
-                                float2 *sum = acc + (half * kCols + x) / 2;
-                                sum[0] = __ffma2_rn(make_float2(__uint_as_float(v[x]), __uint_as_float(v[x + 1])), make_float2(f[q].x, f[q].y), sum[0]);
-                                sum[1] = __ffma2_rn(make_float2(__uint_as_float(v[x + 2]), __uint_as_float(v[x + 3])), make_float2(f[q].z, f[q].w), sum[1]);
-                                if (c + 1 < kCols / 16) f[q] = s[(c + 1) * 4 + q];
+                        for (int u = 0; u < U; ++u) {
+#pragma unroll
+                            for (int q = 0; q < kCols / 4; ++q) {
+                                const float4 x = f[u][q & 3];
+                                if (q + 4 < kCols / 4) f[u][q & 3] = s[u][q + 4];
+                                float2 *sum = acc + (half * kCols + 4 * q) / 2;
+                                sum[0] = __ffma2_rn(make_float2(__uint_as_float(v[u][4 * q]), __uint_as_float(v[u][4 * q + 1])), make_float2(x.x, x.y), sum[0]);
+                                sum[1] = __ffma2_rn(make_float2(__uint_as_float(v[u][4 * q + 2]), __uint_as_float(v[u][4 * q + 3])), make_float2(x.z, x.w), sum[1]);
                             }
                         }
                     }
                     __syncwarp();
-                    if (lane == 0) mbar_arrive(scale_empty_bar(slot));
-                    if (++slot == kGrScaleSlots) {
-                        slot = 0;
+                    if (lane == 0) {
+#pragma unroll
+                        for (int u = 0; u < U; ++u) mbar_arrive(scale_empty_bar((slot + u) % kGrScaleSlots));
+                    }
+                    uses += U;
+                    slot += U;
+                    if (slot >= kGrScaleSlots) {
+                        slot -= kGrScaleSlots;
                         slot_phase ^= 1u;
                     }
-                }
+                };
+                constexpr int kAtOnce = (NB == 1 && TOK <= 64) || TOK <= 32 ? 2 : 1;  // what the registers hold
+                int kb = kb_begin;
+#pragma unroll 1
+                for (; ok && kb + kAtOnce <= kb_end; kb += kAtOnce) blocks(std::integral_constant<int, kAtOnce>());
+                if (ok && kb < kb_end) blocks(std::integral_constant<int, 1>());
+                if (!ok) break;
             } else if (kb_begin < kb_end) {
                 ok = mbar_wait_bounded(acc_full_bar(uses % kGrBufs), (uses / kGrBufs) & 1, abort_flag, p.status, kWaitGroupAccFull, p.wait_ns);
                 ok = __all_sync(0xffffffffu, ok);
@@ -406,7 +452,7 @@ grouped_rows_kernel(const __grid_constant__ CUtensorMap tm_x, const __grid_const
 #pragma unroll
                 for (int half = 0; half < TOK / kCols; ++half) {
                     uint32_t v[kCols];
-                    fetch(v, half);
+                    fetch(v, uses, half);
                     tmem_ld_wait();
                     if (half == TOK / kCols - 1) release();
 #pragma unroll
@@ -561,14 +607,33 @@ static int launch_rows(const GroupedCall &c, GroupedParams p) {
     constexpr int kElem = KIND == MMA_F16 ? 2 : 1;
     constexpr int kBlockK = kRowBytes / kElem;
     auto kern = grouped_rows_kernel<KIND, EPI, TOK>;
-    static KernelSetup ks;
-    int rc = ks.once(
-        [&](int *) {
-            return cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, L::kDynamic) == cudaSuccess
-                       ? (int)O64_OK
-                       : (int)O64_ERR_CUDA;
-        },
-        nullptr);
+    // per size of cluster: how many the device holds at once (the SMs of a GPC do not divide by every size)
+    static KernelSetup ks[4];
+    int most_clusters[4] = {c.num_sms, 0, 0, 0};
+    int rc = O64_OK;
+    for (int i = 0; i < 4 && !rc; ++i)
+        rc = ks[i].once(
+            [&](int *clusters) {
+                if (cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, L::kDynamic) != cudaSuccess) return (int)O64_ERR_CUDA;
+                cudaLaunchConfig_t q = {};
+                q.gridDim = dim3(1u << i, 1, 1);
+                q.blockDim = dim3(L::kThreads, 1, 1);
+                q.dynamicSmemBytes = L::kDynamic;
+                cudaLaunchAttribute a;
+                a.id = cudaLaunchAttributeClusterDimension;
+                a.val.clusterDim.x = 1u << i;
+                a.val.clusterDim.y = a.val.clusterDim.z = 1;
+                q.attrs = &a;
+                q.numAttrs = 1;
+                int n = 0;
+                if (cudaOccupancyMaxActiveClusters(&n, kern, &q) != cudaSuccess) {
+                    (void)cudaGetLastError();
+                    n = 0;
+                }
+                *clusters = n;
+                return (int)O64_OK;
+            },
+            &most_clusters[i]);
     if (rc) return rc;
     CUtensorMap tx, tw;
     rc = encode_2d(&tx, c.kind, c.A, c.T, c.K, c.lda, kBlockK, TOK);
@@ -582,7 +647,8 @@ static int launch_rows(const GroupedCall &c, GroupedParams p) {
     // Too few tiles for the GPU: the K blocks of each are divided over a cluster, as long as a CTA keeps four
     // of them.
     int S = 1;
-    while (S < 8 && tiles * S * 2 <= c.num_sms && p.num_k_blocks >= 4 * S * 2) S *= 2;
+    for (int i = 1; i < 4; ++i)
+        if (tiles <= most_clusters[i] && p.num_k_blocks >= 4 << i) S = 1 << i;
     p.split = S;
     const int grid = (int)(S > 1 ? tiles * S : (tiles < c.num_sms ? tiles : c.num_sms));
     cudaLaunchConfig_t cfg = {};
