@@ -731,7 +731,7 @@ static int launch_grouped(const CUtensorMap &ta, const CUtensorMap &tb, const CU
 
 int grouped_launch(const GroupedCall &c) {
     GroupedParams p = grouped_params(c);
-    if (grouped_rows_fits(c)) return grouped_rows_launch(c, p);
+    if (const int tok = grouped_rows_tile(c)) return grouped_rows_launch(c, p, tok);
     const int elem = c.kind == O64_KIND_BF16 ? 2 : 1;
     const int block_k = kRowBytes / elem;
     CUtensorMap ta, tb, tc;

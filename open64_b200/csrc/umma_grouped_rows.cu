@@ -48,7 +48,7 @@ struct RowsLayout {
     static constexpr uint32_t kTmemCols = kGrBufs * NB * TOK;
     static_assert(kDynamic <= 227 * 1024, "shared memory");
     static_assert(kStageBytes % 1024 == 0 && kWBytes % 1024 == 0, "swizzle atoms");
-    static_assert(kRing >= 128 * (NB + 1) * TOK * 4, "the ring receives the partial sums");
+    static_assert(kRing >= 128 * NB * 8 * 16 && kRing >= 128 * NB * TOK * 4, "the ring receives the partial sums");
     static_assert(kTmemCols <= 512 && (kTmemCols & (kTmemCols - 1)) == 0 && kTmemCols >= 32, "TMEM columns");
 };
 
@@ -82,8 +82,38 @@ __device__ __forceinline__ bool next_rows_tile(const GroupedParams &p, RowsWalk 
     return false;
 }
 
-__device__ __forceinline__ void st_cluster_f32(uint32_t addr, float v) {
-    asm volatile("st.shared::cluster.f32 [%0], %1;" ::"r"(addr), "f"(v) : "memory");
+// The e4m3 tail of a warp's 32 columns: `amax` holds the four warps' largest magnitudes of each row ([4][TOK],
+// as integers).  Lane l works out the scales of rows l and l + 32, for all columns of the warp.
+template <int TOK, int ROWS>
+__device__ __forceinline__ void store_e4m3_rows(const uint32_t *amax, const float (&h)[ROWS], int rows, uint8_t *dst, long long ld, float *scales,
+                                                long long ld_scales, bool write_scales) {
+    const int lane = threadIdx.x & 31;
+    constexpr int kPer = (ROWS + 31) / 32;
+    float inv[kPer];
+#pragma unroll
+    for (int i = 0; i < kPer; ++i) {
+        const int j = i * 32 + lane;
+        inv[i] = 1.0f;
+        if (j < rows) {
+            const uint32_t m = max(max(amax[j], amax[TOK + j]), max(amax[2 * TOK + j], amax[3 * TOK + j]));
+            const float scale = block_scale_of(__uint_as_float(m));
+            if (write_scales) scales[j * ld_scales] = scale;
+            inv[i] = 1.0f / scale;
+        }
+    }
+#pragma unroll
+    for (int j = 0; j < ROWS; ++j) {
+        if (j >= rows) break;
+        const float f = __shfl_sync(0xffffffffu, inv[j / 32], j % 32);
+        dst[j * ld] = (uint8_t)__nv_cvt_float_to_fp8(h[j] * f, __NV_SATFINITE, __NV_E4M3);
+    }
+}
+
+__device__ __forceinline__ void st_cluster_f32x4(uint32_t addr, float2 a, float2 b) {
+    asm volatile("st.shared::cluster.v4.f32 [%0], {%1, %2, %3, %4};" ::"r"(addr), "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y) : "memory");
+}
+__device__ __forceinline__ void st_cluster_f32x2(uint32_t addr, float2 a) {
+    asm volatile("st.shared::cluster.v2.f32 [%0], {%1, %2};" ::"r"(addr), "f"(a.x), "f"(a.y) : "memory");
 }
 
 }  // namespace
@@ -520,16 +550,11 @@ grouped_rows_kernel(const __grid_constant__ CUtensorMap tm_x, const __grid_const
                         }
                         ok = __shfl_sync(0xffffffffu, ok, 0);
                         if (!ok) break;
-                        uint8_t *dst = static_cast<uint8_t *>(p.C) + (long long)t.begin * p.ldc + col;
+                        float h[TOK];
 #pragma unroll
-                        for (int j = 0; j < TOK; ++j) {
-                            if (j >= rows) break;
-                            const uint32_t m = max(max(amax[j], amax[TOK + j]), max(amax[2 * TOK + j], amax[3 * TOK + j]));
-                            const float scale = block_scale_of(__uint_as_float(m));
-                            const float h = ((j & 1) ? acc[j / 2].y : acc[j / 2].x) * (1.0f / scale);
-                            dst[j * p.ldc] = (uint8_t)__nv_cvt_float_to_fp8(h, __NV_SATFINITE, __NV_E4M3);
-                            if (quarter == 0 && lane == 0) p.scale_c[(long long)(t.begin + j) * p.ldsc + t.nb] = scale;
-                        }
+                        for (int j = 0; j < TOK; ++j) h[j] = (j & 1) ? acc[j / 2].y : acc[j / 2].x;
+                        store_e4m3_rows<TOK>(amax, h, rows, static_cast<uint8_t *>(p.C) + (long long)t.begin * p.ldc + col, p.ldc,
+                                             p.scale_c + (long long)t.begin * p.ldsc + t.nb, p.ldsc, quarter == 0);
                     }
                 }
             }
@@ -541,14 +566,25 @@ grouped_rows_kernel(const __grid_constant__ CUtensorMap tm_x, const __grid_const
         __syncwarp();
         cluster_sync_all();  // every ring is idle
         const int shift = __ffs(TOK / S) - 1, per = 1 << shift;  // S and TOK are powers of two
-        const uint32_t recv = smem_base;  // [rank][per][NB * 128]
+        // what a CTA receives: [rank][four rows at a time][NB * 128 columns], 16 bytes a column, so that a warp's
+        // store and its loads are 512 contiguous bytes (with a column's rows side by side the exchange of 64 rows
+        // took 10000 cycles)
+        const int chunks = per >= 4 ? per >> 2 : 1;
+        constexpr uint32_t kChunkBytes = NB * 128 * 16;
         const int n_in = (warp & 3) * 32 + lane;
         if (warp >= 4 && have) {
-            const int at = (warp - 4) / 4 * 128 + n_in;
+            const uint32_t base = smem_base + rank * chunks * kChunkBytes + ((warp - 4) / 4 * 128 + n_in) * 16;
+            if (per >= 4) {
 #pragma unroll
-            for (int j = 0; j < TOK; ++j)
-                st_cluster_f32(map_to_cta(recv, j >> shift) + (((rank << shift) + (j & (per - 1))) * (NB * 128) + at) * 4,
-                               (j & 1) ? acc[j / 2].y : acc[j / 2].x);
+                for (int j = 0; j < TOK; j += 4)
+                    if (j < last.end - last.begin)
+                        st_cluster_f32x4(map_to_cta(base + ((j & (per - 1)) >> 2) * kChunkBytes, j >> shift), acc[j / 2], acc[j / 2 + 1]);
+            } else {
+#pragma unroll
+                for (int j = 0; j < TOK; j += 2)  // per == 2
+                    if (j < last.end - last.begin)
+                        st_cluster_f32x2(map_to_cta(base, j >> shift), acc[j / 2]);
+            }
         }
         __syncwarp();
         cluster_sync_all();
@@ -556,34 +592,50 @@ grouped_rows_kernel(const __grid_constant__ CUtensorMap tm_x, const __grid_const
         const int col = mine ? last.nb * 128 + n_in : 0;
         const int row0 = mine ? last.begin + (rank << shift) : 0;
         const int rows = mine ? min(per, last.end - row0) : 0;
-        const float *got = reinterpret_cast<const float *>(smem_gen) + n_in;
-        float *h_buf = reinterpret_cast<float *>(smem_gen) + TOK * NB * 128 + n_in;  // [per][128]
-        auto total = [&](int j, int blk) {
-            float sum = 0.0f;
-            for (int r = 0; r < S; ++r) sum += got[((r << shift) + j) * (NB * 128) + blk * 128];
+        // this column's sums of four rows, over all ranks in their order
+        auto total4 = [&](int chunk, int blk) __attribute__((always_inline)) {
+            const uint8_t *src = smem_gen + chunk * kChunkBytes + (blk * 128 + n_in) * 16;
+            float4 sum = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+#pragma unroll
+            for (int r = 0; r < 8; ++r) {
+                if (r >= S) break;
+                const float4 x = *reinterpret_cast<const float4 *>(src + r * chunks * kChunkBytes);
+                sum.x += x.x, sum.y += x.y, sum.z += x.z, sum.w += x.w;
+            }
             return sum;
         };
+        constexpr int kMostChunks = TOK / 2 / 4;
+        float h[kMostChunks * 4];
+#pragma unroll
+        for (int c = 0; c < kMostChunks; ++c) {
+            if (c >= chunks || c * 4 >= rows) break;
+            float4 x = total4(c, 0);
+            if constexpr (kSwiglu) {
+                const float4 u = total4(c, 1);
+                x = make_float4(silu_mul(x.x, u.x), silu_mul(x.y, u.y), silu_mul(x.z, u.z), silu_mul(x.w, u.w));
+            }
+            h[4 * c] = x.x, h[4 * c + 1] = x.y, h[4 * c + 2] = x.z, h[4 * c + 3] = x.w;
+        }
         if constexpr (EPI == GEPI_SWIGLU_E4M3) {
             uint32_t *amax = reinterpret_cast<uint32_t *>(smem_gen + L::kAmax);  // [4][TOK]
-            for (int j = 0; j < rows; ++j) {
-                const float h = silu_mul(total(j, 0), total(j, 1));
-                h_buf[j * 128] = h;
-                const uint32_t m = __reduce_max_sync(0xffffffffu, __float_as_uint(h) & 0x7fffffffu);
-                if (lane == 0) amax[(warp & 3) * TOK + j] = m;
+#pragma unroll
+            for (int c = 0; c < kMostChunks; ++c) {
+                if (c * 4 >= rows) break;
+                uint32_t m[4];
+#pragma unroll
+                for (int e = 0; e < 4; ++e) m[e] = __reduce_max_sync(0xffffffffu, __float_as_uint(h[4 * c + e]) & 0x7fffffffu);
+                if (lane == 0) *reinterpret_cast<uint4 *>(amax + (warp & 3) * TOK + 4 * c) = make_uint4(m[0], m[1], m[2], m[3]);
             }
             __syncthreads();
-            for (int j = 0; j < rows; ++j) {
-                const uint32_t m = max(max(amax[j], amax[TOK + j]), max(amax[2 * TOK + j], amax[3 * TOK + j]));
-                const float scale = block_scale_of(__uint_as_float(m));
-                static_cast<uint8_t *>(p.C)[(long long)(row0 + j) * p.ldc + col] =
-                    (uint8_t)__nv_cvt_float_to_fp8(h_buf[j * 128] * (1.0f / scale), __NV_SATFINITE, __NV_E4M3);
-                if (warp == 4 && lane == 0) p.scale_c[(long long)(row0 + j) * p.ldsc + last.nb] = scale;
-            }
+            store_e4m3_rows<TOK>(amax, h, rows, static_cast<uint8_t *>(p.C) + (long long)row0 * p.ldc + col, p.ldc,
+                                 p.scale_c + (long long)row0 * p.ldsc + (mine ? last.nb : 0), p.ldsc, warp == 4);
         } else if (col < p.N) {
             __nv_bfloat16 *dst = static_cast<__nv_bfloat16 *>(p.C) + (long long)row0 * p.ldc + col;
-#pragma unroll 4
-            for (int j = 0; j < rows; ++j)
-                dst[j * p.ldc] = __float2bfloat16_rn(kSwiglu ? silu_mul(total(j, 0), total(j, 1)) : total(j, 0));
+#pragma unroll
+            for (int j = 0; j < kMostChunks * 4; ++j) {
+                if (j >= rows) break;
+                dst[j * p.ldc] = __float2bfloat16_rn(h[j]);
+            }
         }
     }
 
@@ -672,30 +724,53 @@ static int launch_rows(const GroupedCall &c, GroupedParams p) {
     return O64_OK;
 }
 
-bool grouped_rows_fits(const GroupedCall &c) {
-    if (c.wgrad || c.b_kn || c.epi == GEPI_F32 || c.T <= 0) return false;
+// Which kernel, and how many rows of A a tile: the cheaper of  waves * K blocks / S * (time of a K block)  over the
+// tiles that the groups' mean size makes (their sizes are on the device).  Microseconds a K block of 128 bytes,
+// measured with one to eight waves of tiles at N, K of 2048 to 8192:
+//   e4m3 128 x 16 / 32 / 64 / 128 rows: 0.30 / 0.33 / 0.42 / 0.55    two weight blocks (SwiGLU): 0.42 / 0.45 / 0.60
+//   bf16 128 x 16 ... 64 rows: 0.26                                   CTA pairs, 256 x 256: e4m3 0.48, bf16 0.46
+// e.g. 128 x 8192 x 8192 e4m3: 24 us here on clusters of two, 35 us on pairs; 256 rows: 38 and 36.
+int grouped_rows_tile(const GroupedCall &c) {
+    if (c.wgrad || c.b_kn || c.epi == GEPI_F32 || c.T <= 0) return 0;
+    const bool fp8 = c.kind == O64_KIND_FP8, swiglu = gepi_swiglu(c.epi);
     const int64_t groups = c.G < c.T ? c.G : c.T;
-    return c.T <= 64 * groups;
+    const int64_t mean = (c.T + groups - 1) / groups;
+    const int64_t kbs = (c.K * (fp8 ? 1 : 2) + kRowBytes - 1) / kRowBytes;
+    const int64_t pair_cols = swiglu ? 128 : 256;
+    const int64_t pair_tiles = groups * ((mean + 255) / 256) * ((c.N + pair_cols - 1) / pair_cols);
+    const int pairs = c.num_sms / 2;
+    double best = (double)((pair_tiles + pairs - 1) / pairs) * kbs * (fp8 ? 0.48 : 0.46);
+    static const double us[3][4] = {{0.30, 0.33, 0.42, 0.55}, {0.42, 0.45, 0.60, 0}, {0.26, 0.26, 0.26, 0}};
+    int tok = 0;
+    for (int i = 0; i < (fp8 && !swiglu ? 4 : 3); ++i) {
+        const int64_t tiles = groups * ((mean + (16 << i) - 1) / (16 << i)) * ((c.N + 127) / 128);
+        int S = 1;
+        while (S < 8 && tiles * S * 2 <= c.num_sms * 9 / 10 && kbs >= 8 * S) S *= 2;
+        const double cost = (double)((tiles * S + c.num_sms - 1) / c.num_sms) * kbs / S * us[fp8 ? (swiglu ? 1 : 0) : 2][i];
+        if (cost < best) {
+            best = cost;
+            tok = 16 << i;
+        }
+    }
+    return tok;
 }
 
 template <int KIND, int EPI>
-static int launch_rows_tok(const GroupedCall &c, const GroupedParams &p) {
-    const int64_t groups = c.G < c.T ? c.G : c.T;
-    const int64_t mean = (c.T + groups - 1) / groups;
-    if (mean <= 16) return launch_rows<KIND, EPI, 16>(c, p);
-    if (mean <= 32) return launch_rows<KIND, EPI, 32>(c, p);
+static int launch_rows_tok(const GroupedCall &c, const GroupedParams &p, int tok) {
     if constexpr (KIND == MMA_F8F6F4 && !gepi_swiglu(EPI))
-        if (mean > 64) return launch_rows<KIND, EPI, 128>(c, p);
+        if (tok == 128) return launch_rows<KIND, EPI, 128>(c, p);
+    if (tok == 16) return launch_rows<KIND, EPI, 16>(c, p);
+    if (tok == 32) return launch_rows<KIND, EPI, 32>(c, p);
     return launch_rows<KIND, EPI, 64>(c, p);
 }
 
-int grouped_rows_launch(const GroupedCall &c, const GroupedParams &p) {
+int grouped_rows_launch(const GroupedCall &c, const GroupedParams &p, int tok) {
     if (c.kind == O64_KIND_BF16) {
-        if (c.epi == GEPI_BF16) return launch_rows_tok<MMA_F16, GEPI_BF16>(c, p);
+        if (c.epi == GEPI_BF16) return launch_rows_tok<MMA_F16, GEPI_BF16>(c, p, tok);
     } else if (c.kind == O64_KIND_FP8) {
-        if (c.epi == GEPI_BF16) return launch_rows_tok<MMA_F8F6F4, GEPI_BF16>(c, p);
-        if (c.epi == GEPI_SWIGLU_BF16) return launch_rows_tok<MMA_F8F6F4, GEPI_SWIGLU_BF16>(c, p);
-        if (c.epi == GEPI_SWIGLU_E4M3) return launch_rows_tok<MMA_F8F6F4, GEPI_SWIGLU_E4M3>(c, p);
+        if (c.epi == GEPI_BF16) return launch_rows_tok<MMA_F8F6F4, GEPI_BF16>(c, p, tok);
+        if (c.epi == GEPI_SWIGLU_BF16) return launch_rows_tok<MMA_F8F6F4, GEPI_SWIGLU_BF16>(c, p, tok);
+        if (c.epi == GEPI_SWIGLU_E4M3) return launch_rows_tok<MMA_F8F6F4, GEPI_SWIGLU_E4M3>(c, p, tok);
     }
     return O64_ERR_DTYPE;
 }
