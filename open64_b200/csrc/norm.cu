@@ -328,7 +328,7 @@ __device__ __forceinline__ void smem8(const uint8_t *at, float (&v)[8]) {
 // In both kernels a copy that does not arrive within the budget is reported and its rows are undefined; every
 // thread still walks to the end (the flag ends the remaining waits at once).
 template <int NV, bool E4M3>
-__global__ void __launch_bounds__(kNormMaxThreads) norm_forward_ring_kernel(const FwdParams p, int stages, int *status, unsigned long long wait_ns) {
+__global__ void __launch_bounds__(kNormMaxThreads, NV == 2 ? 2 : 1) norm_forward_ring_kernel(const FwdParams p, int stages, int *status, unsigned long long wait_ns) {
     extern __shared__ __align__(128) uint8_t smem[];
     __shared__ float slots[2][16];
     __shared__ __align__(8) uint64_t bars[kNormMaxStages];
@@ -433,7 +433,7 @@ __global__ void __launch_bounds__(kNormMaxThreads) norm_forward_ring_kernel(cons
 }
 
 template <int NV>
-__global__ void __launch_bounds__(kNormMaxThreads) norm_backward_ring_kernel(const BwdParams p, int stages, int *status, unsigned long long wait_ns) {
+__global__ void __launch_bounds__(kNormMaxThreads, NV == 2 ? 2 : 1) norm_backward_ring_kernel(const BwdParams p, int stages, int *status, unsigned long long wait_ns) {
     extern __shared__ __align__(128) uint8_t smem[];
     __shared__ float slots[2][16];
     __shared__ __align__(8) uint64_t bars[kNormMaxStages];
@@ -589,15 +589,22 @@ int launch_forward(const FwdParams &p, bool e4m3, dim3 grid, dim3 block, cudaStr
 }
 
 // Blocks that stay on an SM for rows of N columns with `operands` of them on their way, and the depth of their
-// rings: 512 threads and all shared memory of an SM, at most three blocks and three rows ahead.
-bool ring_shape(int64_t N, int operands, int extra_bytes_per_col, int *blocks_per_sm, int *stages, size_t *smem) {
-    const int tpr = threads_for(N, 4);
+// rings: two vectors a thread where 512 threads hold a row so (8191 rows of 5000, backward: 75 us with four vectors
+// and 160 threads a row, RING_BWD with two and 320), 1024 threads and all shared memory of an SM, at most three rows ahead.
+struct RingShape {
+    int nv, threads, blocks_per_sm, stages;
+    size_t smem;
+};
+bool ring_shape(int64_t N, int operands, int extra_bytes_per_col, RingShape *r) {
+    r->nv = threads_for(N, 2) <= kNormMaxThreads ? 2 : 4;
+    r->threads = threads_for(N, r->nv);
+    if (r->threads > kNormMaxThreads) return false;
     const size_t row = (size_t)((N * 2 + 127) / 128 * 128) * operands, extra = (size_t)N * extra_bytes_per_col;
-    if (tpr > kNormMaxThreads) return false;
-    for (int b = kNormMaxThreads / tpr < 3 ? kNormMaxThreads / tpr : 3; b >= 1; --b)
+    const int most = std::min(3, (r->nv == 2 ? 1024 : 512) / r->threads);
+    for (int b = most; b >= 1; --b)
         for (int s = 3; s >= 2; --s)
             if ((row * s + extra + 1280) * b <= 227 * 1024 && row * s + extra <= 220 * 1024) {
-                *blocks_per_sm = b, *stages = s, *smem = row * s + extra;
+                r->blocks_per_sm = b, r->stages = s, r->smem = row * s + extra;
                 return true;
             }
     return false;
@@ -609,13 +616,23 @@ int allow_smem(F kern, KernelSetup &ks) {
                    nullptr);
 }
 
-template <bool E4M3>
-int launch_forward_ring(const FwdParams &p, int tpr, int grid, int stages, size_t smem, int *status, unsigned long long wait_ns, cudaStream_t s) {
+template <int NV, bool E4M3>
+int launch_forward_ring(const FwdParams &p, const RingShape &r, const NormCall &c, int num_sms) {
     static KernelSetup ks;
-    auto kern = norm_forward_ring_kernel<4, E4M3>;
+    auto kern = norm_forward_ring_kernel<NV, E4M3>;
     const int rc = allow_smem(kern, ks);
     if (rc) return rc;
-    kern<<<grid, tpr, smem, s>>>(p, stages, status, wait_ns);
+    kern<<<r.blocks_per_sm * num_sms, r.threads, r.smem, c.stream>>>(p, r.stages, c.status, c.wait_ns);
+    return cudaGetLastError() == cudaSuccess ? O64_OK : O64_ERR_CUDA;
+}
+
+template <int NV>
+int launch_backward_ring(const BwdParams &p, const RingShape &r, const NormBackwardCall &c, int grid) {
+    static KernelSetup ks;
+    auto kern = norm_backward_ring_kernel<NV>;
+    const int rc = allow_smem(kern, ks);
+    if (rc) return rc;
+    kern<<<grid, r.threads, r.smem, c.stream>>>(p, r.stages, c.status, c.wait_ns);
     return cudaGetLastError() == cudaSuccess ? O64_OK : O64_ERR_CUDA;
 }
 
@@ -632,12 +649,11 @@ int norm_forward(const NormCall &c, int num_sms) {
     p.S = static_cast<__nv_bfloat16 *>(c.S), p.lds = c.lds;
     p.W = c.W, p.w_f32 = c.w_f32, p.eps = c.eps;
     p.Y = c.Y, p.ldy = c.ldy, p.scales = c.scales, p.ldscales = c.ldscales, p.rstd = c.rstd, p.row_scale = c.row_scale;
-    int per_sm, stages;
-    size_t smem;
-    if (vec && !(e4m3 && c.row_scale) && c.N >= kRingCols && ring_shape(c.N, c.R ? 2 : 1, 0, &per_sm, &stages, &smem) &&
-        c.T >= (int64_t)2 * per_sm * num_sms)
-        return e4m3 ? launch_forward_ring<true>(p, threads_for(c.N, 4), per_sm * num_sms, stages, smem, c.status, c.wait_ns, c.stream)
-                    : launch_forward_ring<false>(p, threads_for(c.N, 4), per_sm * num_sms, stages, smem, c.status, c.wait_ns, c.stream);
+    RingShape r;
+    if (vec && !(e4m3 && c.row_scale) && c.N >= kRingCols && ring_shape(c.N, c.R ? 2 : 1, 0, &r) && c.T >= (int64_t)2 * r.blocks_per_sm * num_sms) {
+        if (r.nv == 2) return e4m3 ? launch_forward_ring<2, true>(p, r, c, num_sms) : launch_forward_ring<2, false>(p, r, c, num_sms);
+        return e4m3 ? launch_forward_ring<4, true>(p, r, c, num_sms) : launch_forward_ring<4, false>(p, r, c, num_sms);
+    }
     const int nv = pick_nv(c.N, c.T <= 2 * num_sms ? 1 : 4);
     const int tpr = threads_for(c.N, nv);
     const int rows = tpr >= 128 ? 1 : 128 / tpr;
@@ -686,17 +702,12 @@ int norm_backward(const NormBackwardCall &c, int num_sms) {
     p.dX = static_cast<__nv_bfloat16 *>(c.dX), p.lddx = c.lddx;
     p.W = c.W, p.w_f32 = c.w_f32, p.rstd = c.rstd;
     p.partial = c.dW ? c.workspace : nullptr;
-    int per_sm, stages;
-    size_t smem;
-    if (vec && c.N >= kRingCols && (reinterpret_cast<uintptr_t>(c.workspace) & 15u) == 0 && ring_shape(c.N, c.dR ? 3 : 2, 4, &per_sm, &stages, &smem) &&
-        c.T >= (int64_t)2 * per_sm * num_sms) {
-        static KernelSetup ks;
-        auto kern = norm_backward_ring_kernel<4>;
-        const int rc = allow_smem(kern, ks);
+    RingShape r;
+    if (vec && c.N >= kRingCols && (reinterpret_cast<uintptr_t>(c.workspace) & 15u) == 0 && ring_shape(c.N, c.dR ? 3 : 2, 4, &r) &&
+        c.T >= (int64_t)2 * r.blocks_per_sm * num_sms) {
+        const int grid = (int)std::min<int64_t>((int64_t)r.blocks_per_sm * num_sms, blocks * block.y);  // no more partial rows than the workspace has
+        const int rc = r.nv == 2 ? launch_backward_ring<2>(p, r, c, grid) : launch_backward_ring<4>(p, r, c, grid);
         if (rc) return rc;
-        const int grid = (int)std::min<int64_t>((int64_t)per_sm * num_sms, blocks * block.y);  // no more partial rows than the workspace has
-        kern<<<grid, threads_for(c.N, 4), smem, c.stream>>>(p, stages, c.status, c.wait_ns);
-        if (cudaGetLastError() != cudaSuccess) return O64_ERR_CUDA;
         return c.dW ? add_partials(c, grid) : O64_OK;
     }
     const unsigned grid = (unsigned)blocks;

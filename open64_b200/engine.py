@@ -52,7 +52,7 @@ def _rowmajor(t, name):
 
 def _want(t, name, dtypes, shape):
     """An operand of the given element type(s) and shape (None: any extent), or the library's error."""
-    if t.dtype in dtypes and t.is_cuda and t.shape == shape:
+    if t.dtype in dtypes and t.shape == shape and t.is_cuda:
         return t
     if t.dtype not in dtypes:
         raise O64Error(_lib.ERR_DTYPE, f"{name}: {t.dtype}")
@@ -82,7 +82,8 @@ def _new(like, shape, dtype):
 
 def _ld(t):
     """Elements between rows of a matrix whose columns are contiguous (a single row: any pitch, here one that TMA takes)."""
-    return t.stride(-2) if t.shape[-2] > 1 else t.shape[-1] + -t.shape[-1] % 16
+    rows, cols = t.shape[-2:]
+    return t.stride(-2) if rows > 1 else cols + -cols % 16
 
 
 def _laid_out(t):
@@ -96,7 +97,7 @@ def _laid_out(t):
 
 def _rows(t):
     """`t` as the library reads a matrix: itself, or a copy."""
-    return t if _laid_out(t) else t.contiguous()
+    return t if t.is_contiguous() or _laid_out(t) else t.contiguous()
 
 
 def _out(t, name):
@@ -329,39 +330,47 @@ class Engine:
         residual); pass summed=x or summed=residual to add in place.  rstd [T] is what rms_norm_backward
         needs."""
         T, N = shape = _matrix(x, "x", _BF16).shape
-        x = _rows(x)
-        weight = _want(weight, "weight", (_BF16, _F32), (N,)).contiguous()
-        if out_kind not in (_lib.OUT_BF16, _lib.OUT_E4M3) or scale_block not in (0, 128):
+        if not x.is_contiguous():
+            x = _rows(x)
+        _want(weight, "weight", (_BF16, _F32), (N,))
+        if not weight.is_contiguous():
+            weight = weight.contiguous()
+        quantized = out_kind == _lib.OUT_E4M3
+        if not (quantized or out_kind == _lib.OUT_BF16) or scale_block not in (0, 128):
             raise O64Error(_lib.ERR_DTYPE, "rms_norm")
-        if residual is None:
-            if summed is not None:
-                raise O64Error(_lib.ERR_CONFORM, "rms_norm: summed without a residual")
-        else:
-            residual = _rows(_want(residual, "residual", (_BF16,), shape))
+        p_residual = p_summed = None
+        ldr = lds = 0
+        if residual is not None:
+            _want(residual, "residual", (_BF16,), shape)
+            if not residual.is_contiguous():
+                residual = _rows(residual)
             summed = _new(x, shape, _BF16) if summed is None else _out(_want(summed, "summed", (_BF16,), shape), "summed")
-        dtype = _OUT_DTYPE[out_kind]
+            p_residual, ldr, p_summed, lds = residual.data_ptr(), _ld(residual), summed.data_ptr(), _ld(summed)
+        elif summed is not None:
+            raise O64Error(_lib.ERR_CONFORM, "rms_norm: summed without a residual")
+        dtype = _E4M3 if quantized else _BF16
         y = _new(x, shape, dtype) if out is None else _out(_want(out, "out", (dtype,), shape), "out")
         p_scales, ldscales = None, 0
-        if out_kind == _lib.OUT_E4M3:
-            scales_shape = (T, -(-N // 128)) if scale_block else (T,)
-            scales = x.new_empty(scales_shape, dtype=_F32) if scales is None else _want(scales, "scales", (_F32,), scales_shape)
-            if scale_block:
-                ldscales = _ld(_out(scales, "scales"))
+        if quantized:
+            blocks = (N + 127) // 128
+            scales_shape = (T, blocks) if scale_block else (T,)
+            if scales is None:
+                scales, ldscales = x.new_empty(scales_shape, dtype=_F32), blocks if scale_block else 1
             else:
-                ldscales = scales.stride(0) if T > 1 else 1
+                _want(scales, "scales", (_F32,), scales_shape)
+                ldscales = _ld(_out(scales, "scales")) if scale_block else scales.stride(0) if T > 1 else 1
             p_scales = scales.data_ptr()
         elif scales is not None:
             raise O64Error(_lib.ERR_DTYPE, "rms_norm: scales of a bf16 result")
-        rstd = x.new_empty((T,), dtype=_F32) if rstd is None else _want(rstd, "rstd", (_F32,), (T,))
-        if T > 1 and rstd.stride(0) != 1:
+        if rstd is None:
+            rstd = x.new_empty((T,), dtype=_F32)
+        elif T > 1 and _want(rstd, "rstd", (_F32,), (T,)).stride(0) != 1:
             raise O64Error(_lib.ERR_CONFORM, "rms_norm: rstd is not contiguous")
-        if residual is None:
-            add = (None, 0, None, 0)
-        else:
-            add = (residual.data_ptr(), _ld(residual), summed.data_ptr(), _ld(summed))
-        check(self.lib.o64_rmsnorm_bf16(self._h, T, N, x.data_ptr(), _ld(x), *add, weight.data_ptr(), 1 if weight.dtype is _F32 else 0, eps,
-                                        out_kind, scale_block, y.data_ptr(), _ld(y), p_scales, ldscales, rstd.data_ptr(), _stream(x)),
-              "o64_rmsnorm_bf16")
+        rc = self.lib.o64_rmsnorm_bf16(self._h, T, N, x.data_ptr(), _ld(x), p_residual, ldr, p_summed, lds, weight.data_ptr(),
+                                       weight.dtype is _F32, eps, out_kind, scale_block, y.data_ptr(), _ld(y), p_scales, ldscales,
+                                       rstd.data_ptr(), _stream(x))
+        if rc:
+            check(rc, "o64_rmsnorm_bf16")
         return y, scales, (x if residual is None else summed), rstd
 
     def rms_norm_backward(self, dy, summed, weight, rstd, dresidual=None, dx=None):
@@ -387,6 +396,14 @@ class Engine:
     def _block_operands(self, A8, scaleA, B8, scaleB, transB, swiglu, groups):
         """Checks an e4m3 product with block scales; returns (M, N, K, A8, scaleA, B8, scaleB) as the library reads them."""
         M, K = _matrix(A8, "A8", _E4M3).shape
+        if groups is None and B8.dim() == 2:
+            rows, cols = B8.shape  # the common case, checked in one go
+            n = rows if transB else cols
+            if (B8.dtype is _E4M3 and (cols if transB else rows) == K and not (swiglu and n % 256) and (K | cols) % 16 == 0 and
+                    scaleA.dtype is _F32 and scaleB.dtype is _F32 and scaleA.shape == (M, (K + 127) // 128) and
+                    scaleB.shape == ((rows + 127) // 128, (cols + 127) // 128) and A8.is_contiguous() and B8.is_contiguous() and
+                    scaleA.is_contiguous() and scaleB.is_contiguous() and (A8.data_ptr() | B8.data_ptr()) % 16 == 0):
+                return M, n // 2 if swiglu else n, K, A8, scaleA, B8, scaleB
         lead = () if groups is None else (groups,)
         _want(B8, "B8", (_E4M3,), (*lead, None, K) if transB else (*lead, K, None))
         rows, cols = B8.shape[-2:]
