@@ -814,8 +814,9 @@ extern "C" int o64_rmsnorm_bf16(o64_handle_t h, int64_t T, int64_t N, const void
     if (out_kind != O64_OUT_BF16 && out_kind != O64_OUT_E4M3) return O64_ERR_DTYPE;
     const bool e4m3 = out_kind == O64_OUT_E4M3;
     if (e4m3 && scale_block != 0 && scale_block != 128) return O64_ERR_DTYPE;
-    if (T == 0 || N == 0) return O64_OK;
-    if (N > kNormMaxCols || T > INT32_MAX || !X || !W || !Y || (e4m3 && !scales)) return O64_ERR_RANK;
+    if (N < 1 || N > kNormMaxCols || T > INT32_MAX) return O64_ERR_RANK;
+    if (T == 0) return O64_OK;
+    if (!X || !W || !Y || (e4m3 && !scales)) return O64_ERR_RANK;
     if (ldx < N || ldy < N || (R && ldr < N) || (S && lds < N)) return O64_ERR_CONFORM;
     if (e4m3 && ldscales < (scale_block ? (N + 127) / 128 : 1)) return O64_ERR_CONFORM;
     if (!device_operands(h, {X, R, S, W, Y, scales, rstd})) return O64_ERR_RANK;
@@ -836,8 +837,7 @@ extern "C" int o64_rmsnorm_bf16_backward(o64_handle_t h, int64_t T, int64_t N, c
                                          int64_t lds, const void *W, int w_f32, const float *rstd, const void *dR, int64_t lddr,
                                          void *dX, int64_t lddx, float *dW, void *workspace, void *stream) {
     if (!h || T < 0 || N < 0) return O64_ERR_RANK;
-    if (N == 0) return O64_OK;
-    if (N > kNormMaxCols || T > INT32_MAX) return O64_ERR_RANK;
+    if (N < 1 || N > kNormMaxCols || T > INT32_MAX) return O64_ERR_RANK;
     DeviceGuard g(h->device);
     cudaStream_t s = (cudaStream_t)stream;
     if (T == 0) {  // the sum over no rows
@@ -861,7 +861,8 @@ static int grouped_entry(o64_handle_t h, GroupedCall c, void *stream) {
     if (!h || c.G < 0 || c.T < 0 || c.N < 0 || c.K < 0) return O64_ERR_RANK;
     const bool swiglu = gepi_swiglu(c.epi);
     const bool scaled = c.kind == O64_KIND_FP8;
-    if (c.G > INT32_MAX || c.T > INT32_MAX || c.N > INT32_MAX / 2 || c.K > INT32_MAX) return O64_ERR_RANK;
+    constexpr int64_t kMost = INT32_MAX - 1024;  // coordinates count past the last tile's end in 32 bits
+    if (c.G > kMost || c.T > kMost || c.N > kMost / 2 || c.K > kMost) return O64_ERR_RANK;
     if (c.G == 0 || c.N == 0 || (c.wgrad ? c.K == 0 : c.T == 0)) return O64_OK;
     if (swiglu && c.N % 128) return O64_ERR_CONFORM;
     const int64_t c_rows = c.wgrad ? c.N : c.T, c_cols = c.wgrad ? c.K : c.N;

@@ -31,7 +31,7 @@ namespace o64 {
 namespace {
 
 constexpr int kNormMaxThreads = 512;
-constexpr int kRingCols = 2048;  // narrower rows run on the block-per-row kernel
+constexpr int kRingCols = 256;  // narrower rows run on the block-per-row kernel
 constexpr float kE4m3Max = 448.0f;
 constexpr float kMinNormal = 1.17549435e-38f;
 
@@ -433,7 +433,7 @@ __global__ void __launch_bounds__(kNormMaxThreads, NV == 2 ? 2 : 1) norm_forward
 }
 
 template <int NV>
-__global__ void __launch_bounds__(kNormMaxThreads, NV == 2 ? 2 : 1) norm_backward_ring_kernel(const BwdParams p, int stages, int *status, unsigned long long wait_ns) {
+__global__ void __launch_bounds__(kNormMaxThreads, NV == 2 ? 2 : 1) norm_backward_ring_kernel(const BwdParams p, int stages, int w_in_smem, int *status, unsigned long long wait_ns) {
     extern __shared__ __align__(128) uint8_t smem[];
     __shared__ float slots[2][16];
     __shared__ __align__(8) uint64_t bars[kNormMaxStages];
@@ -466,13 +466,21 @@ __global__ void __launch_bounds__(kNormMaxThreads, NV == 2 ? 2 : 1) norm_backwar
     for (int i = 0; i < NV; ++i) {
         const int col = (i * blockDim.x + threadIdx.x) * 8;
         float w[8];
-        load_w8<true>(p.W, p.w_f32, col, n, w);
+        if (w_in_smem) load_w8<true>(p.W, p.w_f32, col, n, w);
 #pragma unroll
         for (int e = 0; e < 8; ++e) {
             dw[i][e] = 0.0f;
-            if (col < n) w_smem[col + e] = w[e];  // read back by this thread only
+            if (w_in_smem && col < n) w_smem[col + e] = w[e];  // read back by this thread only
         }
     }
+    auto weight8 = [&](int col, float (&w)[8]) __attribute__((always_inline)) {
+        if (w_in_smem) {
+            *reinterpret_cast<float4 *>(w) = *reinterpret_cast<const float4 *>(w_smem + col);
+            *reinterpret_cast<float4 *>(w + 4) = *reinterpret_cast<const float4 *>(w_smem + col + 4);
+        } else {  // wide rows leave no room for it
+            load_w8<true>(p.W, p.w_f32, col, n, w);
+        }
+    };
     int stage = 0, turn = 0, before = 0;
     uint32_t phase = 0;
     for (long long row = blockIdx.x; row < p.T; row += gridDim.x, turn ^= 1) {
@@ -487,8 +495,7 @@ __global__ void __launch_bounds__(kNormMaxThreads, NV == 2 ? 2 : 1) norm_backwar
                 float g[8], nn[8], w[8];
                 smem8(at + col * 2, g);
                 smem8(at + pitch + col * 2, nn);
-                *reinterpret_cast<float4 *>(w) = *reinterpret_cast<const float4 *>(w_smem + col);
-                *reinterpret_cast<float4 *>(w + 4) = *reinterpret_cast<const float4 *>(w_smem + col + 4);
+                weight8(col, w);
 #pragma unroll
                 for (int e = 0; e < 8; ++e) {
                     const float x = nn[e] * rstd;
@@ -517,8 +524,7 @@ __global__ void __launch_bounds__(kNormMaxThreads, NV == 2 ? 2 : 1) norm_backwar
                 smem8(at + col * 2, g);
                 smem8(at + pitch + col * 2, nn);
                 if (p.dR) smem8(at + 2 * pitch + col * 2, dr);
-                *reinterpret_cast<float4 *>(w) = *reinterpret_cast<const float4 *>(w_smem + col);
-                *reinterpret_cast<float4 *>(w + 4) = *reinterpret_cast<const float4 *>(w_smem + col + 4);
+                weight8(col, w);
 #pragma unroll
                 for (int e = 0; e < 8; ++e) {
                     out[e] = rstd * (g[e] * w[e] - nn[e] * rstd * mean);
@@ -550,19 +556,25 @@ __global__ void __launch_bounds__(kNormMaxThreads, NV == 2 ? 2 : 1) norm_backwar
     }
 }
 
-// dW[j] = sum over the partial rows: 32 columns per block, 16 threads down the rows of each.
-__global__ void __launch_bounds__(512) norm_dw_kernel(const float *partial, long long rows, int N, float *dW) {
-    __shared__ float part[16][33];
-    const int col = blockIdx.x * 32 + threadIdx.x;
+// dW[j] = sum over the partial rows: eight columns (one sector of each row) per block, 128 threads down the rows.
+__global__ void __launch_bounds__(1024) norm_dw_kernel(const float *partial, int rows, int N, float *dW) {
+    __shared__ float part[32][8];
+    const int c = threadIdx.x & 7, col = blockIdx.x * 8 + c;
     float s = 0.0f;
-    if (col < N)
-        for (long long r = threadIdx.y; r < rows; r += 16) s += partial[r * N + col];
-    part[threadIdx.y][threadIdx.x] = s;
+    if (col < N) {
+#pragma unroll 4
+        for (int r = threadIdx.x >> 3; r < rows; r += 128) s += partial[(long long)r * N + col];
+    }
+    s += __shfl_xor_sync(0xffffffffu, s, 8);
+    s += __shfl_xor_sync(0xffffffffu, s, 16);
+    if ((threadIdx.x & 31) < 8) part[threadIdx.x >> 5][c] = s;
     __syncthreads();
-    if (threadIdx.y == 0 && col < N) {
+    if (threadIdx.x < 256) {  // warp w adds column w
+        const int w = threadIdx.x >> 5, lane = threadIdx.x & 31;
+        s = part[lane][w];
 #pragma unroll
-        for (int i = 1; i < 16; ++i) s += part[i][threadIdx.x];
-        dW[col] = s;
+        for (int o = 16; o > 0; o >>= 1) s += __shfl_xor_sync(0xffffffffu, s, o);
+        if (lane == 0 && blockIdx.x * 8 + w < N) dW[blockIdx.x * 8 + w] = s;
     }
 }
 
@@ -590,7 +602,7 @@ int launch_forward(const FwdParams &p, bool e4m3, dim3 grid, dim3 block, cudaStr
 
 // Blocks that stay on an SM for rows of N columns with `operands` of them on their way, and the depth of their
 // rings: two vectors a thread where 512 threads hold a row so (8191 rows of 5000, backward: 75 us with four vectors
-// and 160 threads a row, RING_BWD with two and 320), 1024 threads and all shared memory of an SM, at most three rows ahead.
+// and 160 threads a row, 70 us with two and 320), 1024 threads and all shared memory of an SM, at most three rows ahead.
 struct RingShape {
     int nv, threads, blocks_per_sm, stages;
     size_t smem;
@@ -600,7 +612,7 @@ bool ring_shape(int64_t N, int operands, int extra_bytes_per_col, RingShape *r) 
     r->threads = threads_for(N, r->nv);
     if (r->threads > kNormMaxThreads) return false;
     const size_t row = (size_t)((N * 2 + 127) / 128 * 128) * operands, extra = (size_t)N * extra_bytes_per_col;
-    const int most = std::min(3, (r->nv == 2 ? 1024 : 512) / r->threads);
+    const int most = std::min(16, (r->nv == 2 ? 1024 : 512) / r->threads);
     for (int b = most; b >= 1; --b)
         for (int s = 3; s >= 2; --s)
             if ((row * s + extra + 1280) * b <= 227 * 1024 && row * s + extra <= 220 * 1024) {
@@ -627,12 +639,12 @@ int launch_forward_ring(const FwdParams &p, const RingShape &r, const NormCall &
 }
 
 template <int NV>
-int launch_backward_ring(const BwdParams &p, const RingShape &r, const NormBackwardCall &c, int grid) {
+int launch_backward_ring(const BwdParams &p, const RingShape &r, const NormBackwardCall &c, int grid, int w_in_smem) {
     static KernelSetup ks;
     auto kern = norm_backward_ring_kernel<NV>;
     const int rc = allow_smem(kern, ks);
     if (rc) return rc;
-    kern<<<grid, r.threads, r.smem, c.stream>>>(p, r.stages, c.status, c.wait_ns);
+    kern<<<grid, r.threads, r.smem, c.stream>>>(p, r.stages, w_in_smem, c.status, c.wait_ns);
     return cudaGetLastError() == cudaSuccess ? O64_OK : O64_ERR_CUDA;
 }
 
@@ -672,7 +684,9 @@ static void backward_shape(int64_t T, int64_t N, int *nv, dim3 *block, int64_t *
     const int rows = tpr >= 128 ? 1 : 128 / tpr;
     *block = dim3(tpr, rows);
     const int64_t want = (T + rows - 1) / rows;
-    *blocks = want < 444 ? want : 444;  // three blocks per SM
+    // three blocks per SM, and more of narrow rows: the partial rows then stay under 10 MB
+    const int64_t most = std::min<int64_t>(2368, std::max<int64_t>(444, (int64_t)2400000 / N / rows / 148 * 148));
+    *blocks = want < most ? want : most;
 }
 
 int64_t norm_backward_partials(int64_t T, int64_t N) {
@@ -683,8 +697,8 @@ int64_t norm_backward_partials(int64_t T, int64_t N) {
     return blocks * block.y;
 }
 
-static int add_partials(const NormBackwardCall &c, long long rows) {
-    norm_dw_kernel<<<(unsigned)((c.N + 31) / 32), dim3(32, 16), 0, c.stream>>>(c.workspace, rows, (int)c.N, c.dW);
+static int add_partials(const NormBackwardCall &c, int64_t rows) {
+    norm_dw_kernel<<<(unsigned)((c.N + 7) / 8), 1024, 0, c.stream>>>(c.workspace, (int)rows, (int)c.N, c.dW);
     return cudaGetLastError() == cudaSuccess ? O64_OK : O64_ERR_CUDA;
 }
 
@@ -703,10 +717,11 @@ int norm_backward(const NormBackwardCall &c, int num_sms) {
     p.W = c.W, p.w_f32 = c.w_f32, p.rstd = c.rstd;
     p.partial = c.dW ? c.workspace : nullptr;
     RingShape r;
-    if (vec && c.N >= kRingCols && (reinterpret_cast<uintptr_t>(c.workspace) & 15u) == 0 && ring_shape(c.N, c.dR ? 3 : 2, 4, &r) &&
-        c.T >= (int64_t)2 * r.blocks_per_sm * num_sms) {
+    int w_in_smem = 1;
+    if (vec && c.N >= kRingCols && (reinterpret_cast<uintptr_t>(c.workspace) & 15u) == 0 &&
+        (ring_shape(c.N, c.dR ? 3 : 2, 4, &r) || ring_shape(c.N, c.dR ? 3 : 2, w_in_smem = 0, &r)) && c.T >= (int64_t)2 * r.blocks_per_sm * num_sms) {
         const int grid = (int)std::min<int64_t>((int64_t)r.blocks_per_sm * num_sms, blocks * block.y);  // no more partial rows than the workspace has
-        const int rc = r.nv == 2 ? launch_backward_ring<2>(p, r, c, grid) : launch_backward_ring<4>(p, r, c, grid);
+        const int rc = r.nv == 2 ? launch_backward_ring<2>(p, r, c, grid, w_in_smem) : launch_backward_ring<4>(p, r, c, grid, w_in_smem);
         if (rc) return rc;
         return c.dW ? add_partials(c, grid) : O64_OK;
     }

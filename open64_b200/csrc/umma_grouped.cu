@@ -76,7 +76,8 @@ __device__ __forceinline__ bool next_tile(const GroupedParams &p, TileWalk &w, i
         group_rows(p, w.g, tile.begin, tile.end);
         const int rows = tile.end - tile.begin;
         const int mt = WGRAD ? p.num_m_tiles : (rows + kGpTileM - 1) / kGpTileM;
-        const int tiles = mt * p.num_n_tiles;  // (the host has checked that all of them fit an int)
+        // (the host has checked that all of them fit an int; groups that overlap, from bad offsets, may not)
+        const int tiles = (int)min((long long)mt * p.num_n_tiles, (long long)(INT32_MAX - w.base));
         if (t < w.base + tiles) {
             // bands of eight row tiles, rows fastest: a band's rows of A and one column block of B stay in L2
             const int r = t - w.base;

@@ -68,7 +68,7 @@ __device__ __forceinline__ bool next_rows_tile(const GroupedParams &p, RowsWalk 
         int begin, end;
         group_rows(p, w.g, begin, end);
         const int tt = (end - begin + TOK - 1) / TOK;
-        const int tiles = tt * p.num_n_tiles;
+        const int tiles = (int)min((long long)tt * p.num_n_tiles, (long long)(INT32_MAX - w.base));
         if (t < w.base + tiles) {
             const int r = t - w.base;
             tile.g = w.g;

@@ -107,6 +107,19 @@ def _out(t, name):
     return t
 
 
+_WORDS = ((8, torch.int64), (4, torch.int32), (2, torch.int16))
+
+
+def _copy_rows(to, t):
+    """to.copy_(t) in the widest words that both sides' rows are made of (byte by byte a 17 MB weight took 25 us)."""
+    e = t.element_size()
+    for width, word in _WORDS:
+        if width > e and not any(v % width for v in (t.shape[-1] * e, t.data_ptr(), to.data_ptr(),
+                                                     *(s * e for s in t.stride()[:-1]), *(s * e for s in to.stride()[:-1]))):
+            return to.view(word).copy_(t.view(word))
+    return to.copy_(t)
+
+
 def _tma(t):
     """`t` as TMA can read it (contiguous columns; base, pitch and matrix stride multiples of 16 bytes): itself,
     or a copy whose rows are padded."""
@@ -122,7 +135,7 @@ def _tma(t):
     cols = t.shape[-1]
     padded = torch.empty((*t.shape[:-1], cols + -cols % (16 // e)), dtype=t.dtype, device=t.device)
     padded = padded[..., :cols]
-    padded.copy_(t)
+    _copy_rows(padded, t)
     return padded
 
 

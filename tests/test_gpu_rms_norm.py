@@ -134,11 +134,13 @@ def test_nan_and_infinity_stay_in_their_row_and_block(eng):
 def test_in_place_strides_and_what_lies_between(eng):
     T, N = 37, 1000
     x, r, w = data(T, N, 11)
-    want = eng.rms_norm(x, w, r, out_kind=o.OUT_E4M3)
-    for pad in (8, 3):  # vector path, and rows that start anywhere
+    _, _, h, size = formula(x, r, w, 1e-6)
+    for pad in (8, 3):  # vector path, and rows that start anywhere (another order of the sum: its own values to compare with)
         bx = torch.full((T, N + pad), 7.0, device="cuda", dtype=torch.bfloat16)
         br = bx.clone()
         bx[:, :N], br[:, :N] = x, r
+        want = eng.rms_norm(bx[:, :N], w, br[:, :N], out_kind=o.OUT_E4M3)
+        check_e4m3(want[0], want[1], h, size, 128)
         by = torch.zeros((T, N + pad), device="cuda", dtype=torch.float8_e4m3fn)
         bs = torch.full((T, 11), -1.0, device="cuda")
         y, scales, summed, _ = eng.rms_norm(bx[:, :N], w, br[:, :N], out_kind=o.OUT_E4M3, out=by[:, :N], scales=bs[:, :8], summed=br[:, :N])
@@ -278,6 +280,7 @@ def test_refusals(eng):
     refused(o.ERR_RANK, lambda: eng.rms_norm(x, w.cpu()))
     wide = torch.zeros((1, 32769), device="cuda", dtype=torch.bfloat16)
     refused(o.ERR_RANK, lambda: eng.rms_norm(wide, wide[0].float()))
+    refused(o.ERR_RANK, lambda: eng.rms_norm(x[:, :0], w[:0]))
     L, P = eng.lib, lambda t: t.data_ptr()
     s = torch.cuda.current_stream().cuda_stream
     call = lambda **k: L.o64_rmsnorm_bf16(*{**dict(h=eng._h, T=4, N=256, X=P(x), ldx=256, R=None, ldr=0, S=None, lds=0, W=P(w), f=1, eps=1e-6,
