@@ -442,7 +442,6 @@ __global__ void __launch_bounds__(kNormMaxThreads, NV == 2 ? 2 : 1) norm_backwar
     const uint32_t row_bytes = (uint32_t)n * 2, pitch = (row_bytes + 127) & ~127u;
     const int operands = p.dR ? 3 : 2;
     const uint32_t stage_bytes = pitch * operands;
-    float *w_smem = reinterpret_cast<float *>(smem + stages * stage_bytes);
     if (threadIdx.x == 0) {
         for (int s = 0; s < stages; ++s) mbar_init(smem_u32(&bars[s]), 1);
         abort_word = 0;
@@ -465,20 +464,34 @@ __global__ void __launch_bounds__(kNormMaxThreads, NV == 2 ? 2 : 1) norm_backwar
 #pragma unroll
     for (int i = 0; i < NV; ++i) {
         const int col = (i * blockDim.x + threadIdx.x) * 8;
-        float w[8];
-        if (w_in_smem) load_w8<true>(p.W, p.w_f32, col, n, w);
 #pragma unroll
         for (int e = 0; e < 8; ++e) {
             dw[i][e] = 0.0f;
-            if (w_in_smem && col < n) w_smem[col + e] = w[e];  // read back by this thread only
+        }
+    }
+    // a thread's columns of w lie behind the ring as they came (wide rows leave no room for them); nobody else reads them
+    uint8_t *w_smem = smem + stages * stage_bytes;
+    const int w_elem = p.w_f32 ? 4 : 2;
+    if (w_in_smem) {
+#pragma unroll
+        for (int i = 0; i < NV; ++i) {
+            const int col = (i * blockDim.x + threadIdx.x) * 8;
+            if (col < n) {
+                const uint4 *src = reinterpret_cast<const uint4 *>(static_cast<const uint8_t *>(p.W) + (size_t)col * w_elem);
+                uint4 *dst = reinterpret_cast<uint4 *>(w_smem + (size_t)col * w_elem);
+                dst[0] = __ldg(src);
+                if (p.w_f32) dst[1] = __ldg(src + 1);
+            }
         }
     }
     auto weight8 = [&](int col, float (&w)[8]) __attribute__((always_inline)) {
-        if (w_in_smem) {
-            *reinterpret_cast<float4 *>(w) = *reinterpret_cast<const float4 *>(w_smem + col);
-            *reinterpret_cast<float4 *>(w + 4) = *reinterpret_cast<const float4 *>(w_smem + col + 4);
-        } else {  // wide rows leave no room for it
+        if (!w_in_smem) {
             load_w8<true>(p.W, p.w_f32, col, n, w);
+        } else if (p.w_f32) {
+            *reinterpret_cast<float4 *>(w) = *reinterpret_cast<const float4 *>(w_smem + col * 4);
+            *reinterpret_cast<float4 *>(w + 4) = *reinterpret_cast<const float4 *>(w_smem + col * 4 + 16);
+        } else {
+            smem8(w_smem + col * 2, w);
         }
     };
     int stage = 0, turn = 0, before = 0;
@@ -539,6 +552,7 @@ __global__ void __launch_bounds__(kNormMaxThreads, NV == 2 ? 2 : 1) norm_backwar
             phase ^= 1u;
         }
     }
+    griddep_launch_dependents();
     if (p.partial) {
         float *dst = p.partial + (long long)blockIdx.x * n;
 #pragma unroll
@@ -556,14 +570,17 @@ __global__ void __launch_bounds__(kNormMaxThreads, NV == 2 ? 2 : 1) norm_backwar
     }
 }
 
-// dW[j] = sum over the partial rows: eight columns (one sector of each row) per block, 128 threads down the rows.
-__global__ void __launch_bounds__(1024) norm_dw_kernel(const float *partial, int rows, int N, float *dW) {
-    __shared__ float part[32][8];
+// dW[j] = sum over the partial rows: eight columns (one sector of each row) per block, THREADS / 8 down the rows.
+// Launched so that its set-up overlaps the kernel that writes them.
+template <int THREADS>
+__global__ void __launch_bounds__(THREADS) norm_dw_kernel(const float *partial, int rows, int N, float *dW) {
+    __shared__ float part[THREADS / 32][8];
     const int c = threadIdx.x & 7, col = blockIdx.x * 8 + c;
+    griddep_wait();
     float s = 0.0f;
     if (col < N) {
-#pragma unroll 4
-        for (int r = threadIdx.x >> 3; r < rows; r += 128) s += partial[(long long)r * N + col];
+#pragma unroll 8
+        for (int r = threadIdx.x >> 3; r < rows; r += THREADS / 8) s += partial[(long long)r * N + col];
     }
     s += __shfl_xor_sync(0xffffffffu, s, 8);
     s += __shfl_xor_sync(0xffffffffu, s, 16);
@@ -571,7 +588,7 @@ __global__ void __launch_bounds__(1024) norm_dw_kernel(const float *partial, int
     __syncthreads();
     if (threadIdx.x < 256) {  // warp w adds column w
         const int w = threadIdx.x >> 5, lane = threadIdx.x & 31;
-        s = part[lane][w];
+        s = lane < THREADS / 32 ? part[lane][w] : 0.0f;
 #pragma unroll
         for (int o = 16; o > 0; o >>= 1) s += __shfl_xor_sync(0xffffffffu, s, o);
         if (lane == 0 && blockIdx.x * 8 + w < N) dW[blockIdx.x * 8 + w] = s;
@@ -698,8 +715,20 @@ int64_t norm_backward_partials(int64_t T, int64_t N) {
 }
 
 static int add_partials(const NormBackwardCall &c, int64_t rows) {
-    norm_dw_kernel<<<(unsigned)((c.N + 7) / 8), 1024, 0, c.stream>>>(c.workspace, (int)rows, (int)c.N, c.dW);
-    return cudaGetLastError() == cudaSuccess ? O64_OK : O64_ERR_CUDA;
+    cudaLaunchConfig_t cfg = {};
+    const bool many = rows > 800;
+    cfg.gridDim = dim3((unsigned)((c.N + 7) / 8));
+    cfg.blockDim = dim3(many ? 1024 : 256);
+    cfg.stream = c.stream;
+    cudaLaunchAttribute at;
+    at.id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    at.val.programmaticStreamSerializationAllowed = 1;
+    cfg.attrs = &at;
+    cfg.numAttrs = 1;
+    const float *partial = c.workspace;
+    const cudaError_t e = cudaLaunchKernelEx(&cfg, many ? norm_dw_kernel<1024> : norm_dw_kernel<256>, partial, (int)rows, (int)c.N, c.dW);
+    if (e != cudaSuccess) (void)cudaGetLastError();
+    return e == cudaSuccess ? O64_OK : O64_ERR_CUDA;
 }
 
 int norm_backward(const NormBackwardCall &c, int num_sms) {
@@ -717,9 +746,13 @@ int norm_backward(const NormBackwardCall &c, int num_sms) {
     p.W = c.W, p.w_f32 = c.w_f32, p.rstd = c.rstd;
     p.partial = c.dW ? c.workspace : nullptr;
     RingShape r;
-    int w_in_smem = 1;
-    if (vec && c.N >= kRingCols && (reinterpret_cast<uintptr_t>(c.workspace) & 15u) == 0 &&
-        (ring_shape(c.N, c.dR ? 3 : 2, 4, &r) || ring_shape(c.N, c.dR ? 3 : 2, w_in_smem = 0, &r)) && c.T >= (int64_t)2 * r.blocks_per_sm * num_sms) {
+    // w stays in shared memory (4096 columns: 53 us with it and three blocks an SM, 59 without and four) unless only
+    // one block fits then (8192 rows of 8192, fp32 w: 119 us with it, 99 from L2 and two blocks)
+    RingShape with_w;
+    bool fits = vec && c.N >= kRingCols && (reinterpret_cast<uintptr_t>(c.workspace) & 15u) == 0 && ring_shape(c.N, c.dR ? 3 : 2, 0, &r);
+    const int w_in_smem = fits && ring_shape(c.N, c.dR ? 3 : 2, c.w_f32 ? 4 : 2, &with_w) && (with_w.blocks_per_sm > 1 || r.blocks_per_sm == 1);
+    if (w_in_smem) r = with_w;
+    if (fits && c.T >= (int64_t)2 * r.blocks_per_sm * num_sms) {
         const int grid = (int)std::min<int64_t>((int64_t)r.blocks_per_sm * num_sms, blocks * block.y);  // no more partial rows than the workspace has
         const int rc = r.nv == 2 ? launch_backward_ring<2>(p, r, c, grid, w_in_smem) : launch_backward_ring<4>(p, r, c, grid, w_in_smem);
         if (rc) return rc;
