@@ -80,7 +80,7 @@ __device__ __forceinline__ void group_rows(const GroupedParams &p, int g, int &b
 }
 
 int grouped_launch(const GroupedCall &c);
-// Few rows a group (weights [N,K]): the kernel that reads every weight once for them.
+// Few rows a group: the kernel that reads every weight once for them.
 // grouped_rows_tile: the rows of A of its tiles (16 ... 128), or 0 where CTA pairs are the faster choice.
 int grouped_rows_tile(const GroupedCall &c);
 int grouped_rows_launch(const GroupedCall &c, const GroupedParams &p, int tok);

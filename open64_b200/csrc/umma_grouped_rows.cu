@@ -119,7 +119,8 @@ __device__ __forceinline__ void st_cluster_f32x2(uint32_t addr, float2 a) {
 }  // namespace
 
 // p.num_n_tiles counts blocks of 128 columns of C; p.split: CTAs a cluster (> 1: one tile per cluster).
-template <int KIND, int EPI, int TOK>
+// KN: the weight lies [K,N], the first operand with M contiguous.
+template <int KIND, int EPI, int TOK, bool KN>
 __global__ void __launch_bounds__(RowsLayout<gepi_swiglu(EPI) ? 2 : 1, TOK>::kThreads, 1)
 grouped_rows_kernel(const __grid_constant__ CUtensorMap tm_x, const __grid_constant__ CUtensorMap tm_w,
                     const __grid_constant__ GroupedParams p) {
@@ -127,7 +128,11 @@ grouped_rows_kernel(const __grid_constant__ CUtensorMap tm_x, const __grid_const
     constexpr int NB = kSwiglu ? 2 : 1;
     using L = RowsLayout<NB, TOK>;
     constexpr bool kScaled = KIND == MMA_F8F6F4;
-    constexpr int kBlockK = kRowBytes / (KIND == MMA_F16 ? 2 : 1);
+    constexpr int kElem = KIND == MMA_F16 ? 2 : 1;
+    constexpr int kBlockK = kRowBytes / kElem;
+    constexpr int kKnCols = kRowBytes / kElem;          // columns in a 128-byte row of a [K,N] weight
+    constexpr int kKnGroupBytes = kBlockK * kRowBytes;  // kBlockK such rows
+    static_assert(!KN || !kSwiglu, "gate and up weights are [N,K]");
 
     extern __shared__ uint8_t smem_raw[];
     const uint32_t smem_base = (smem_u32(smem_raw) + 1023u) & ~1023u;
@@ -217,9 +222,15 @@ grouped_rows_kernel(const __grid_constant__ CUtensorMap tm_x, const __grid_const
                 if (leader) {
                     const uint32_t w_dst = smem_base + stage * L::kStageBytes;
                     mbar_arrive_expect_tx(full_bar(stage), L::kStageBytes);
+                    if constexpr (KN) {
 #pragma unroll
-                    for (int b = 0; b < NB; ++b)
-                        tma_load_3d(w_dst + b * 128 * kRowBytes, &tm_w, kb * kBlockK, t.nb * 128 + b * p.N, t.g, full_bar(stage));
+                        for (int c = 0; c < 128 / kKnCols; ++c)
+                            tma_load_3d(w_dst + c * kKnGroupBytes, &tm_w, t.nb * 128 + c * kKnCols, kb * kBlockK, t.g, full_bar(stage));
+                    } else {
+#pragma unroll
+                        for (int b = 0; b < NB; ++b)
+                            tma_load_3d(w_dst + b * 128 * kRowBytes, &tm_w, kb * kBlockK, t.nb * 128 + b * p.N, t.g, full_bar(stage));
+                    }
                     tma_load_2d(w_dst + L::kWBytes, &tm_x, kb * kBlockK, t.begin, full_bar(stage));
                 }
                 __syncwarp();
@@ -234,7 +245,8 @@ grouped_rows_kernel(const __grid_constant__ CUtensorMap tm_x, const __grid_const
         // ------------------------------ MMA ---------------------------------------------
         const bool leader = elect_one();
         constexpr uint32_t fmt = KIND == MMA_F8F6F4 ? 0u : 1u;
-        constexpr uint32_t idesc = make_idesc(1u, fmt, fmt, 0u, 128, TOK);
+        constexpr uint32_t idesc = make_idesc(1u, fmt, fmt, 0u, 128, TOK) | (KN ? 1u << 15 : 0u);
+        constexpr uint32_t kWAdvance = KN ? (32 / kElem * kRowBytes) >> 4 : 2;
         int stage = 0;
         uint32_t phase = 0, uses = 0;
         bool ok = true;
@@ -271,10 +283,10 @@ grouped_rows_kernel(const __grid_constant__ CUtensorMap tm_x, const __grid_const
                 if (leader) {
 #pragma unroll
                     for (int b = 0; b < NB; ++b) {
-                        const uint64_t w_desc = make_smem_desc(w_addr + b * 128 * kRowBytes, 16, 1024);
+                        const uint64_t w_desc = make_smem_desc(w_addr + b * 128 * kRowBytes, KN ? kKnGroupBytes : 16, 1024);
 #pragma unroll
                         for (int k = 0; k < kRowBytes / 32; ++k)
-                            tc_mma<KIND>(d + b * TOK, w_desc + 2u * k, x_desc + 2u * k, idesc,
+                            tc_mma<KIND>(d + b * TOK, w_desc + kWAdvance * k, x_desc + 2u * k, idesc,
                                          (kScaled ? k : ((kb - kb_begin) | k)) != 0 ? 1u : 0u);
                     }
                     tc_commit(empty_bar(stage));
@@ -303,6 +315,7 @@ grouped_rows_kernel(const __grid_constant__ CUtensorMap tm_x, const __grid_const
         RowsTile t;
         // four K blocks at a time, the next four (of this tile or of the next one) always on their way
         const float *sa[kPer], *sb0 = nullptr, *sb1 = nullptr;
+        const long long sb_step = KN ? p.ldsb : 1;
         float next[kPer][4], b0[4], b1[4];
         int tile = first, kb0 = kb_begin;
         auto fetch = [&]() __attribute__((always_inline)) {
@@ -311,7 +324,7 @@ grouped_rows_kernel(const __grid_constant__ CUtensorMap tm_x, const __grid_const
                 const bool in = kb0 + u < kb_end;
 #pragma unroll
                 for (int r = 0; r < kPer; ++r) next[r][u] = in ? __ldg(sa[r] + kb0 + u) : 0.0f;
-                b0[u] = in ? __ldg(sb0 + kb0 + u) : 0.0f;
+                b0[u] = in ? __ldg(sb0 + (kb0 + u) * sb_step) : 0.0f;
                 b1[u] = kSwiglu && in ? __ldg(sb1 + kb0 + u) : 0.0f;
             }
         };
@@ -320,7 +333,7 @@ grouped_rows_kernel(const __grid_constant__ CUtensorMap tm_x, const __grid_const
 #pragma unroll
             for (int r = 0; r < kPer; ++r) sa[r] = p.scale_a + (long long)min(t.begin + r * 32 + lane, t.end - 1) * p.ldsa;
             const float *sb = p.scale_b + (long long)t.g * p.stride_sb;
-            sb0 = sb + t.nb * p.ldsb;
+            sb0 = KN ? sb + t.nb : sb + t.nb * p.ldsb;
             sb1 = sb + (long long)((p.N >> 7) + t.nb) * p.ldsb;
             kb0 = kb_begin;
             fetch();
@@ -652,13 +665,13 @@ grouped_rows_kernel(const __grid_constant__ CUtensorMap tm_x, const __grid_const
     }
 }
 
-template <int KIND, int EPI, int TOK>
+template <int KIND, int EPI, int TOK, bool KN>
 static int launch_rows(const GroupedCall &c, GroupedParams p) {
     constexpr int NB = gepi_swiglu(EPI) ? 2 : 1;
     using L = RowsLayout<NB, TOK>;
     constexpr int kElem = KIND == MMA_F16 ? 2 : 1;
     constexpr int kBlockK = kRowBytes / kElem;
-    auto kern = grouped_rows_kernel<KIND, EPI, TOK>;
+    auto kern = grouped_rows_kernel<KIND, EPI, TOK, KN>;
     // per size of cluster: how many the device holds at once (the SMs of a GPC do not divide by every size)
     static KernelSetup ks[4];
     int most_clusters[4] = {c.num_sms, 0, 0, 0};
@@ -689,7 +702,9 @@ static int launch_rows(const GroupedCall &c, GroupedParams p) {
     if (rc) return rc;
     CUtensorMap tx, tw;
     rc = encode_2d(&tx, c.kind, c.A, c.T, c.K, c.lda, kBlockK, TOK);
-    if (!rc) rc = encode_3d(&tw, kElem, c.B, c.K, NB * c.N, c.G, c.ldb, c.stride_b, kBlockK, 128, true);
+    if (!rc)
+        rc = KN ? encode_3d(&tw, kElem, c.B, c.N, c.K, c.G, c.ldb, c.stride_b, kRowBytes / kElem, kBlockK, true)
+                : encode_3d(&tw, kElem, c.B, c.K, NB * c.N, c.G, c.ldb, c.stride_b, kBlockK, 128, true);
     if (rc) return rc;
     p.num_n_tiles = (int)((c.N + 127) / 128);
     // at most this many tiles (the groups' sizes are on the device)
@@ -731,7 +746,7 @@ static int launch_rows(const GroupedCall &c, GroupedParams p) {
 //   bf16 128 x 16 ... 64 rows: 0.26                                   CTA pairs, 256 x 256: e4m3 0.48, bf16 0.46
 // e.g. 128 x 8192 x 8192 e4m3: 24 us here on clusters of two, 35 us on pairs; 256 rows: 38 and 36.
 int grouped_rows_tile(const GroupedCall &c) {
-    if (c.wgrad || c.b_kn || c.epi == GEPI_F32 || c.T <= 0) return 0;
+    if (c.wgrad || c.epi == GEPI_F32 || c.T <= 0) return 0;
     const bool fp8 = c.kind == O64_KIND_FP8, swiglu = gepi_swiglu(c.epi);
     const int64_t groups = c.G < c.T ? c.G : c.T;
     const int64_t mean = (c.T + groups - 1) / groups;
@@ -755,20 +770,20 @@ int grouped_rows_tile(const GroupedCall &c) {
     return tok;
 }
 
-template <int KIND, int EPI>
+template <int KIND, int EPI, bool KN = false>
 static int launch_rows_tok(const GroupedCall &c, const GroupedParams &p, int tok) {
     if constexpr (KIND == MMA_F8F6F4 && !gepi_swiglu(EPI))
-        if (tok == 128) return launch_rows<KIND, EPI, 128>(c, p);
-    if (tok == 16) return launch_rows<KIND, EPI, 16>(c, p);
-    if (tok == 32) return launch_rows<KIND, EPI, 32>(c, p);
-    return launch_rows<KIND, EPI, 64>(c, p);
+        if (tok == 128) return launch_rows<KIND, EPI, 128, KN>(c, p);
+    if (tok == 16) return launch_rows<KIND, EPI, 16, KN>(c, p);
+    if (tok == 32) return launch_rows<KIND, EPI, 32, KN>(c, p);
+    return launch_rows<KIND, EPI, 64, KN>(c, p);
 }
 
 int grouped_rows_launch(const GroupedCall &c, const GroupedParams &p, int tok) {
     if (c.kind == O64_KIND_BF16) {
-        if (c.epi == GEPI_BF16) return launch_rows_tok<MMA_F16, GEPI_BF16>(c, p, tok);
+        if (c.epi == GEPI_BF16) return c.b_kn ? launch_rows_tok<MMA_F16, GEPI_BF16, true>(c, p, tok) : launch_rows_tok<MMA_F16, GEPI_BF16>(c, p, tok);
     } else if (c.kind == O64_KIND_FP8) {
-        if (c.epi == GEPI_BF16) return launch_rows_tok<MMA_F8F6F4, GEPI_BF16>(c, p, tok);
+        if (c.epi == GEPI_BF16) return c.b_kn ? launch_rows_tok<MMA_F8F6F4, GEPI_BF16, true>(c, p, tok) : launch_rows_tok<MMA_F8F6F4, GEPI_BF16>(c, p, tok);
         if (c.epi == GEPI_SWIGLU_BF16) return launch_rows_tok<MMA_F8F6F4, GEPI_SWIGLU_BF16>(c, p, tok);
         if (c.epi == GEPI_SWIGLU_E4M3) return launch_rows_tok<MMA_F8F6F4, GEPI_SWIGLU_E4M3>(c, p, tok);
     }
