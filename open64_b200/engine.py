@@ -74,8 +74,8 @@ def _matrix(t, name, dtype):
 
 
 def _new(like, shape, dtype):
-    """A result on the device of `like` (empty_like costs the host half of what empty does)."""
-    if like.shape == shape and like.is_contiguous():
+    """A contiguous result on the device of `like` (empty_like costs the host half of what empty does)."""
+    if like.is_contiguous() and like.shape == shape:
         return torch.empty_like(like, dtype=dtype)
     return like.new_empty(shape, dtype=dtype)
 
@@ -342,10 +342,14 @@ class Engine:
         (scale_block 0, one per row; None for bf16).  `summed` is x + residual in bf16 (x itself without a
         residual); pass summed=x or summed=residual to add in place.  rstd [T] is what rms_norm_backward
         needs."""
-        T, N = shape = _matrix(x, "x", _BF16).shape
+        shape = x.shape
+        if x.dtype is not _BF16 or len(shape) != 2 or not x.is_cuda:
+            _matrix(x, "x", _BF16)  # says what is wrong
+        T, N = shape
         if not x.is_contiguous():
             x = _rows(x)
-        _want(weight, "weight", (_BF16, _F32), (N,))
+        if weight.dtype is not _F32 and weight.dtype is not _BF16 or weight.shape != (N,):
+            _want(weight, "weight", (_BF16, _F32), (N,))
         if not weight.is_contiguous():
             weight = weight.contiguous()
         quantized = out_kind == _lib.OUT_E4M3
@@ -354,15 +358,26 @@ class Engine:
         p_residual = p_summed = None
         ldr = lds = 0
         if residual is not None:
-            _want(residual, "residual", (_BF16,), shape)
-            if not residual.is_contiguous():
+            if residual.dtype is not _BF16 or residual.shape != shape:
+                _want(residual, "residual", (_BF16,), shape)
+            if residual.is_contiguous():
+                ldr = N
+            else:
                 residual = _rows(residual)
-            summed = _new(x, shape, _BF16) if summed is None else _out(_want(summed, "summed", (_BF16,), shape), "summed")
-            p_residual, ldr, p_summed, lds = residual.data_ptr(), _ld(residual), summed.data_ptr(), _ld(summed)
+                ldr = _ld(residual)
+            if summed is None:
+                summed, lds = _new(x, shape, _BF16), N
+            else:
+                lds = _ld(_out(_want(summed, "summed", (_BF16,), shape), "summed"))
+            p_residual, p_summed = residual.data_ptr(), summed.data_ptr()
         elif summed is not None:
             raise O64Error(_lib.ERR_CONFORM, "rms_norm: summed without a residual")
         dtype = _E4M3 if quantized else _BF16
-        y = _new(x, shape, dtype) if out is None else _out(_want(out, "out", (dtype,), shape), "out")
+        if out is None:
+            y, ldy = _new(x, shape, dtype), N
+        else:
+            y = _out(_want(out, "out", (dtype,), shape), "out")
+            ldy = _ld(y)
         p_scales, ldscales = None, 0
         if quantized:
             blocks = (N + 127) // 128
@@ -380,7 +395,7 @@ class Engine:
         elif T > 1 and _want(rstd, "rstd", (_F32,), (T,)).stride(0) != 1:
             raise O64Error(_lib.ERR_CONFORM, "rms_norm: rstd is not contiguous")
         rc = self.lib.o64_rmsnorm_bf16(self._h, T, N, x.data_ptr(), _ld(x), p_residual, ldr, p_summed, lds, weight.data_ptr(),
-                                       weight.dtype is _F32, eps, out_kind, scale_block, y.data_ptr(), _ld(y), p_scales, ldscales,
+                                       weight.dtype is _F32, eps, out_kind, scale_block, y.data_ptr(), ldy, p_scales, ldscales,
                                        rstd.data_ptr(), _stream(x))
         if rc:
             check(rc, "o64_rmsnorm_bf16")
@@ -408,15 +423,16 @@ class Engine:
 
     def _block_operands(self, A8, scaleA, B8, scaleB, transB, swiglu, groups):
         """Checks an e4m3 product with block scales; returns (M, N, K, A8, scaleA, B8, scaleB) as the library reads them."""
-        M, K = _matrix(A8, "A8", _E4M3).shape
-        if groups is None and B8.dim() == 2:
-            rows, cols = B8.shape  # the common case, checked in one go
+        if len(A8.shape) == 2 and len(B8.shape) == (2 if groups is None else 3) and A8.dtype is _E4M3:
+            M, K = A8.shape  # the common case, checked in one go
+            *lead, rows, cols = B8.shape
             n = rows if transB else cols
             if (B8.dtype is _E4M3 and (cols if transB else rows) == K and not (swiglu and n % 256) and (K | cols) % 16 == 0 and
                     scaleA.dtype is _F32 and scaleB.dtype is _F32 and scaleA.shape == (M, (K + 127) // 128) and
-                    scaleB.shape == ((rows + 127) // 128, (cols + 127) // 128) and A8.is_contiguous() and B8.is_contiguous() and
+                    scaleB.shape == (*lead, (rows + 127) // 128, (cols + 127) // 128) and A8.is_contiguous() and B8.is_contiguous() and
                     scaleA.is_contiguous() and scaleB.is_contiguous() and (A8.data_ptr() | B8.data_ptr()) % 16 == 0):
                 return M, n // 2 if swiglu else n, K, A8, scaleA, B8, scaleB
+        M, K = _matrix(A8, "A8", _E4M3).shape
         lead = () if groups is None else (groups,)
         _want(B8, "B8", (_E4M3,), (*lead, None, K) if transB else (*lead, K, None))
         rows, cols = B8.shape[-2:]
@@ -445,17 +461,19 @@ class Engine:
 
     @staticmethod
     def _offsets(offsets, groups):
-        _want(offsets, "offsets", (torch.int32,), (groups + 1,))
-        return offsets.contiguous()
+        if offsets.dtype is not torch.int32 or offsets.shape != (groups + 1,) or not offsets.is_cuda:
+            _want(offsets, "offsets", (torch.int32,), (groups + 1,))
+        return offsets if offsets.is_contiguous() else offsets.contiguous()
 
     def gemm_fp8_block(self, A8, scaleA, B8, scaleB, transB=True, out=None):
         """bf16 sum over blocks of 128 of K of scaleA[m,b] * scaleB[n/128,b] * (A8 @ B8^T in block b).  A8 [M,K],
         scaleA [M, ceil(K/128)]; B8 [N,K] (or [K,N]: transB False), scaleB one value per 128 x 128 of B8."""
         M, N, K, A8, scaleA, B8, scaleB = self._block_operands(A8, scaleA, B8, scaleB, transB, False, None)
         out = self._bf16_out(out, M, N, A8)
-        check(self.lib.o64_gemm_fp8_block(self._h, M, N, K, A8.data_ptr(), _ld(A8), scaleA.data_ptr(), _ld(scaleA), B8.data_ptr(), _ld(B8),
-                                          1 if transB else 0, scaleB.data_ptr(), _ld(scaleB), out.data_ptr(), _ld(out), _stream(A8)),
-              "o64_gemm_fp8_block")
+        rc = self.lib.o64_gemm_fp8_block(self._h, M, N, K, A8.data_ptr(), _ld(A8), scaleA.data_ptr(), _ld(scaleA), B8.data_ptr(), _ld(B8),
+                                         transB, scaleB.data_ptr(), _ld(scaleB), out.data_ptr(), _ld(out), _stream(A8))
+        if rc:
+            check(rc, "o64_gemm_fp8_block")
         return out
 
     def gemm_fp8_block_swiglu(self, A8, scaleA, B8, scaleB, out_kind=_lib.OUT_E4M3, out=None, scales=None):
@@ -473,13 +491,18 @@ class Engine:
         """A[rows of g] @ op(B[g]) for each group g: A [T,K] bf16 sorted by group, offsets int32 [G+1] on the
         device, B [G,N,K] (or [G,K,N]: transB False).  Rows outside offsets[0] .. offsets[G] are left as they are."""
         T, K = _matrix(A, "A", _BF16).shape
-        _want(B, "B", (_BF16,), (None, None, K) if transB else (None, K, None))
-        G, N = B.shape[0], B.shape[1] if transB else B.shape[2]
+        if len(B.shape) != 3 or B.dtype is not _BF16 or B.shape[2 if transB else 1] != K:
+            _want(B, "B", (_BF16,), (None, None, K) if transB else (None, K, None))
+        G, rows, cols = B.shape
+        N = rows if transB else cols
         offsets = self._offsets(offsets, G)
-        A, B = _tma(A), _tma(B)
+        if (K | cols) % 8 or not (A.is_contiguous() and B.is_contiguous()) or (A.data_ptr() | B.data_ptr()) % 16:
+            A, B = _tma(A), _tma(B)
         out = self._bf16_out(out, T, N, A)
-        check(self.lib.o64_gemm_grouped_bf16(self._h, G, T, N, K, A.data_ptr(), _ld(A), offsets.data_ptr(), B.data_ptr(), _ld(B), _stride0(B),
-                                             1 if transB else 0, out.data_ptr(), _ld(out), _stream(A)), "o64_gemm_grouped_bf16")
+        rc = self.lib.o64_gemm_grouped_bf16(self._h, G, T, N, K, A.data_ptr(), _ld(A), offsets.data_ptr(), B.data_ptr(), _ld(B), _stride0(B),
+                                            transB, out.data_ptr(), _ld(out), _stream(A))
+        if rc:
+            check(rc, "o64_gemm_grouped_bf16")
         return out
 
     def gemm_grouped_bf16_wgrad(self, dC, A, offsets, out_kind=_lib.OUT_BF16, out=None):
