@@ -9,7 +9,8 @@
 // norm is taken of the sum in fp32; the stream s that goes on to the next layer is that sum rounded
 // to bf16 once.
 //
-// Bound by HBM.  Many rows run on a few blocks per SM that stay: rows come in by bulk copies, a ring of
+// Bound by HBM: 16384 x 8192 with the residual to e4m3 155 us = 6.1 TB/s (0.93 of a copy), backward 8192 x 8192 with the
+// residual 94 us = 5.7 TB/s.  Many rows run on a few blocks per SM that stay: rows come in by bulk copies, a ring of
 // three ahead, so that loads go on while a row is reduced, converted and stored, and a thread keeps its
 // columns of w.  Few rows, or rows that are not 16-byte aligned, run on a block per row that loads for
 // itself.
@@ -137,8 +138,10 @@ struct FwdParams {
     int w_f32, row_scale;
 };
 
+// amax / 448, by the reciprocal: within an ulp (with this and a fast 1 / scale 6247 rows of 9984 take 61 us, with two
+// divisions per eight values 65)
 __device__ __forceinline__ float scale_of(float amax) {
-    const float s = amax / kE4m3Max;
+    const float s = amax * (1.0f / kE4m3Max);
     return s < kMinNormal ? 1.0f : s;  // (NaN stays NaN)
 }
 
@@ -213,7 +216,7 @@ __global__ void __launch_bounds__(kNormMaxThreads) norm_forward_kernel(const Fwd
             }
             // one reciprocal per block instead of a division per value: within an ulp of h / scale before
             // the rounding to four bits
-            const float inv = 1.0f / scale;
+            const float inv = __fdividef(1.0f, scale);
             const uint2 q2 = quant8(v[i], inv);
             const uint32_t q[2] = {q2.x, q2.y};
             if constexpr (VEC) {
@@ -307,6 +310,8 @@ __global__ void __launch_bounds__(kNormMaxThreads) norm_backward_kernel(const Bw
 // ---- many rows: a ring of bulk copies -------------------------------------------------------------
 constexpr int kNormWait = 0x801;
 constexpr int kNormMaxStages = 3;
+constexpr int kRingMaxThreads = 1024;  // a row's; 64 registers
+constexpr int kRingNv = 2;             // vectors of eight columns a thread, in the ring kernels
 
 __device__ __forceinline__ void bulk_load(uint32_t dst, const void *src, uint32_t bytes, uint32_t bar) {
     asm volatile("cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];" ::"r"(dst), "l"(src),
@@ -325,12 +330,20 @@ __device__ __forceinline__ void smem8(const uint8_t *at, float (&v)[8]) {
     }
 }
 
+// The sum of the warps' values, for every thread.
+__device__ __forceinline__ float block_sum(const float *slot) {
+    float v = (threadIdx.x & 31) < (blockDim.x >> 5) ? slot[threadIdx.x & 31] : 0.0f;
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
+    return v;
+}
+
 // In both kernels a copy that does not arrive within the budget is reported and its rows are undefined; every
 // thread still walks to the end (the flag ends the remaining waits at once).
-template <int NV, bool E4M3>
-__global__ void __launch_bounds__(kNormMaxThreads, NV == 2 ? 2 : 1) norm_forward_ring_kernel(const FwdParams p, int stages, int *status, unsigned long long wait_ns) {
+template <bool E4M3>
+__global__ void __launch_bounds__(kRingMaxThreads) norm_forward_ring_kernel(const FwdParams p, int stages, int *status, unsigned long long wait_ns) {
     extern __shared__ __align__(128) uint8_t smem[];
-    __shared__ float slots[2][16];
+    __shared__ float slots[2][32];
     __shared__ __align__(8) uint64_t bars[kNormMaxStages];
     __shared__ int abort_word;
     const int n = p.N;
@@ -354,18 +367,18 @@ __global__ void __launch_bounds__(kNormMaxThreads, NV == 2 ? 2 : 1) norm_forward
             const long long row = blockIdx.x + (long long)s * gridDim.x;
             if (row < p.T) load(row, s);
         }
-    float w[NV][8];
+    float w[kRingNv][8];
 #pragma unroll
-    for (int i = 0; i < NV; ++i) load_w8<true>(p.W, p.w_f32, (i * blockDim.x + threadIdx.x) * 8, n, w[i]);
+    for (int i = 0; i < kRingNv; ++i) load_w8<true>(p.W, p.w_f32, (i * blockDim.x + threadIdx.x) * 8, n, w[i]);
     int stage = 0, turn = 0;
     uint32_t phase = 0;
     for (long long row = blockIdx.x; row < p.T; row += gridDim.x, turn ^= 1) {
         mbar_wait_bounded(smem_u32(&bars[stage]), phase, &abort_word, status, kNormWait, wait_ns);
         const uint8_t *at = smem + stage * stage_bytes;
-        float v[NV][8];
+        float v[kRingNv][8];
         float sq = 0.0f;
 #pragma unroll
-        for (int i = 0; i < NV; ++i) {
+        for (int i = 0; i < kRingNv; ++i) {
             const int col = (i * blockDim.x + threadIdx.x) * 8;
 #pragma unroll
             for (int e = 0; e < 8; ++e) v[i][e] = 0.0f;
@@ -390,16 +403,15 @@ __global__ void __launch_bounds__(kNormMaxThreads, NV == 2 ? 2 : 1) norm_forward
             fence_proxy_async_smem();
             load(row + (long long)stages * gridDim.x, stage);
         }
-        float sum = slots[turn][0];
-        for (int i = 1; i < (int)(blockDim.x >> 5); ++i) sum += slots[turn][i];
+        const float sum = block_sum(slots[turn]);
         const float rstd = 1.0f / sqrtf(sum / (float)n + p.eps);
         if (p.rstd && threadIdx.x == 0) p.rstd[row] = rstd;
         if (p.S) {
 #pragma unroll
-            for (int i = 0; i < NV; ++i) store8<true>(p.S + row * p.lds, (i * blockDim.x + threadIdx.x) * 8, n, v[i]);
+            for (int i = 0; i < kRingNv; ++i) store8<true>(p.S + row * p.lds, (i * blockDim.x + threadIdx.x) * 8, n, v[i]);
         }
 #pragma unroll
-        for (int i = 0; i < NV; ++i) {
+        for (int i = 0; i < kRingNv; ++i) {
             const int col = (i * blockDim.x + threadIdx.x) * 8;
 #pragma unroll
             for (int e = 0; e < 8; ++e) v[i][e] = v[i][e] * rstd * w[i][e];
@@ -414,7 +426,7 @@ __global__ void __launch_bounds__(kNormMaxThreads, NV == 2 ? 2 : 1) norm_forward
 #pragma unroll
                 for (int o = 8; o > 0; o >>= 1) m = max_nan(m, __shfl_xor_sync(0xffffffffu, m, o));
                 const float scale = scale_of(m);
-                const float inv = 1.0f / scale;
+                const float inv = __fdividef(1.0f, scale);
                 if (col < n) {
                     if ((threadIdx.x & 15) == 0) p.scales[row * p.ldscales + col / 128] = scale;
                     *reinterpret_cast<uint2 *>(static_cast<uint8_t *>(p.Y) + row * p.ldy + col) = quant8(v[i], inv);
@@ -432,10 +444,9 @@ __global__ void __launch_bounds__(kNormMaxThreads, NV == 2 ? 2 : 1) norm_forward
     }
 }
 
-template <int NV>
-__global__ void __launch_bounds__(kNormMaxThreads, NV == 2 ? 2 : 1) norm_backward_ring_kernel(const BwdParams p, int stages, int w_in_smem, int *status, unsigned long long wait_ns) {
+__global__ void __launch_bounds__(kRingMaxThreads) norm_backward_ring_kernel(const BwdParams p, int stages, int w_in_smem, int *status, unsigned long long wait_ns) {
     extern __shared__ __align__(128) uint8_t smem[];
-    __shared__ float slots[2][16];
+    __shared__ float slots[2][32];
     __shared__ __align__(8) uint64_t bars[kNormMaxStages];
     __shared__ int abort_word;
     const int n = p.N;
@@ -460,9 +471,9 @@ __global__ void __launch_bounds__(kNormMaxThreads, NV == 2 ? 2 : 1) norm_backwar
             const long long row = blockIdx.x + (long long)s * gridDim.x;
             if (row < p.T) load(row, s);
         }
-    float dw[NV][8];
+    float dw[kRingNv][8];
 #pragma unroll
-    for (int i = 0; i < NV; ++i) {
+    for (int i = 0; i < kRingNv; ++i) {
         const int col = (i * blockDim.x + threadIdx.x) * 8;
 #pragma unroll
         for (int e = 0; e < 8; ++e) {
@@ -474,7 +485,7 @@ __global__ void __launch_bounds__(kNormMaxThreads, NV == 2 ? 2 : 1) norm_backwar
     const int w_elem = p.w_f32 ? 4 : 2;
     if (w_in_smem) {
 #pragma unroll
-        for (int i = 0; i < NV; ++i) {
+        for (int i = 0; i < kRingNv; ++i) {
             const int col = (i * blockDim.x + threadIdx.x) * 8;
             if (col < n) {
                 const uint4 *src = reinterpret_cast<const uint4 *>(static_cast<const uint8_t *>(p.W) + (size_t)col * w_elem);
@@ -502,7 +513,7 @@ __global__ void __launch_bounds__(kNormMaxThreads, NV == 2 ? 2 : 1) norm_backwar
         const uint8_t *at = smem + stage * stage_bytes;
         float dot = 0.0f;
 #pragma unroll
-        for (int i = 0; i < NV; ++i) {
+        for (int i = 0; i < kRingNv; ++i) {
             const int col = (i * blockDim.x + threadIdx.x) * 8;
             if (col < n) {
                 float g[8], nn[8], w[8];
@@ -526,11 +537,9 @@ __global__ void __launch_bounds__(kNormMaxThreads, NV == 2 ? 2 : 1) norm_backwar
             fence_proxy_async_smem();
             load(row + (long long)(stages - 1) * gridDim.x, before);
         }
-        float sum = slots[turn][0];
-        for (int i = 1; i < (int)(blockDim.x >> 5); ++i) sum += slots[turn][i];
-        const float mean = sum / (float)n;
+        const float mean = block_sum(slots[turn]) / (float)n;
 #pragma unroll
-        for (int i = 0; i < NV; ++i) {
+        for (int i = 0; i < kRingNv; ++i) {
             const int col = (i * blockDim.x + threadIdx.x) * 8;
             if (col < n) {
                 float g[8], nn[8], w[8], out[8], dr[8];
@@ -556,7 +565,7 @@ __global__ void __launch_bounds__(kNormMaxThreads, NV == 2 ? 2 : 1) norm_backwar
     if (p.partial) {
         float *dst = p.partial + (long long)blockIdx.x * n;
 #pragma unroll
-        for (int i = 0; i < NV; ++i) {
+        for (int i = 0; i < kRingNv; ++i) {
             const int col = (i * blockDim.x + threadIdx.x) * 8;
             if (col < n) {
                 *reinterpret_cast<float4 *>(dst + col) = make_float4(dw[i][0], dw[i][1], dw[i][2], dw[i][3]);
@@ -618,21 +627,20 @@ int launch_forward(const FwdParams &p, bool e4m3, dim3 grid, dim3 block, cudaStr
 }
 
 // Blocks that stay on an SM for rows of N columns with `operands` of them on their way, and the depth of their
-// rings: two vectors a thread where 512 threads hold a row so (8191 rows of 5000, backward: 75 us with four vectors
-// and 160 threads a row, 70 us with two and 320), 1024 threads and all shared memory of an SM, at most three rows ahead.
+// rings: 1024 threads and all shared memory of an SM, at most three rows ahead.  Two vectors a thread: with four, 8191
+// rows of 5000 ran backward in 75 us instead of 70 and 6247 rows of 9984 to e4m3 in 92 us instead of 65.
 struct RingShape {
-    int nv, threads, blocks_per_sm, stages;
+    int threads, blocks_per_sm, stages;
     size_t smem;
 };
 bool ring_shape(int64_t N, int operands, int extra_bytes_per_col, RingShape *r) {
-    r->nv = threads_for(N, 2) <= kNormMaxThreads ? 2 : 4;
-    r->threads = threads_for(N, r->nv);
-    if (r->threads > kNormMaxThreads) return false;
+    r->threads = threads_for(N, kRingNv);
+    if (r->threads > kRingMaxThreads) return false;
     const size_t row = (size_t)((N * 2 + 127) / 128 * 128) * operands, extra = (size_t)N * extra_bytes_per_col;
-    const int most = std::min(16, (r->nv == 2 ? 1024 : 512) / r->threads);
+    const int most = std::min(16, 1024 / r->threads);
     for (int b = most; b >= 1; --b)
         for (int s = 3; s >= 2; --s)
-            if ((row * s + extra + 1280) * b <= 227 * 1024 && row * s + extra <= 220 * 1024) {
+            if ((row * s + extra + 1536) * b <= 227 * 1024 && row * s + extra <= 220 * 1024) {
                 r->blocks_per_sm = b, r->stages = s, r->smem = row * s + extra;
                 return true;
             }
@@ -645,20 +653,19 @@ int allow_smem(F kern, KernelSetup &ks) {
                    nullptr);
 }
 
-template <int NV, bool E4M3>
+template <bool E4M3>
 int launch_forward_ring(const FwdParams &p, const RingShape &r, const NormCall &c, int num_sms) {
     static KernelSetup ks;
-    auto kern = norm_forward_ring_kernel<NV, E4M3>;
+    auto kern = norm_forward_ring_kernel<E4M3>;
     const int rc = allow_smem(kern, ks);
     if (rc) return rc;
     kern<<<r.blocks_per_sm * num_sms, r.threads, r.smem, c.stream>>>(p, r.stages, c.status, c.wait_ns);
     return cudaGetLastError() == cudaSuccess ? O64_OK : O64_ERR_CUDA;
 }
 
-template <int NV>
 int launch_backward_ring(const BwdParams &p, const RingShape &r, const NormBackwardCall &c, int grid, int w_in_smem) {
     static KernelSetup ks;
-    auto kern = norm_backward_ring_kernel<NV>;
+    auto kern = norm_backward_ring_kernel;
     const int rc = allow_smem(kern, ks);
     if (rc) return rc;
     kern<<<grid, r.threads, r.smem, c.stream>>>(p, r.stages, w_in_smem, c.status, c.wait_ns);
@@ -680,8 +687,7 @@ int norm_forward(const NormCall &c, int num_sms) {
     p.Y = c.Y, p.ldy = c.ldy, p.scales = c.scales, p.ldscales = c.ldscales, p.rstd = c.rstd, p.row_scale = c.row_scale;
     RingShape r;
     if (vec && !(e4m3 && c.row_scale) && c.N >= kRingCols && ring_shape(c.N, c.R ? 2 : 1, 0, &r) && c.T >= (int64_t)2 * r.blocks_per_sm * num_sms) {
-        if (r.nv == 2) return e4m3 ? launch_forward_ring<2, true>(p, r, c, num_sms) : launch_forward_ring<2, false>(p, r, c, num_sms);
-        return e4m3 ? launch_forward_ring<4, true>(p, r, c, num_sms) : launch_forward_ring<4, false>(p, r, c, num_sms);
+        return e4m3 ? launch_forward_ring<true>(p, r, c, num_sms) : launch_forward_ring<false>(p, r, c, num_sms);
     }
     const int nv = pick_nv(c.N, c.T <= 2 * num_sms ? 1 : 4);
     const int tpr = threads_for(c.N, nv);
@@ -754,7 +760,7 @@ int norm_backward(const NormBackwardCall &c, int num_sms) {
     if (w_in_smem) r = with_w;
     if (fits && c.T >= (int64_t)2 * r.blocks_per_sm * num_sms) {
         const int grid = (int)std::min<int64_t>((int64_t)r.blocks_per_sm * num_sms, blocks * block.y);  // no more partial rows than the workspace has
-        const int rc = r.nv == 2 ? launch_backward_ring<2>(p, r, c, grid, w_in_smem) : launch_backward_ring<4>(p, r, c, grid, w_in_smem);
+        const int rc = launch_backward_ring(p, r, c, grid, w_in_smem);
         if (rc) return rc;
         return c.dW ? add_partials(c, grid) : O64_OK;
     }
