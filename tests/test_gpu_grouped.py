@@ -398,6 +398,77 @@ def test_streams_and_graphs(eng):
     assert all(torch.equal(c, want) for _, c in graphs)
 
 
+@pytest.mark.parametrize("rows", [1, 5, 40, 90, 300])
+def test_calls_that_follow_one_another_without_a_wait(eng, rows):
+    """Each call reads what the one before has just written (few-row kernels set up while it still runs): the same
+    bits as with a wait between, every time."""
+    D, F, G = 384, 256, 3
+    g = gen(rows)
+    T = rows * G
+    off = offsets_of([rows] * G)
+    x, w = bf16((T, D), g), torch.rand((D,), generator=g, device="cuda") + 0.5
+    w13, s13, w2, s2 = e4m3((G, 2 * F, D), g), scales((G, 4, 3), g) * 0.05, e4m3((G, D, F), g), scales((G, 3, 2), g) * 0.05
+    b = bf16((G, D, D), g, 0.05)
+
+    def layer(y, wait):
+        for _ in range(3):
+            y, _ = eng.mlp_swiglu_fp8(y, w, w13, s13, w2, s2, residual=y, offsets=off)
+            wait()
+            y = eng.gemm_grouped_bf16(y, off, b, transB=False)
+            wait()
+            y = eng.rms_norm(y, w)[0]
+            wait()
+        return y
+
+    want = layer(x, torch.cuda.synchronize)
+    got = [layer(x, lambda: None) for _ in range(20)]
+    torch.cuda.synchronize()
+    assert torch.isfinite(want.float()).all() and all(torch.equal(y, want) for y in got)
+
+
+def test_the_first_call_of_a_process_may_be_captured(built):
+    code = """
+import sys, torch
+sys.path.insert(0, {root!r})
+import open64_b200 as o
+e = o.Engine(0)
+a, b = torch.randn(20, 256, device="cuda").to(torch.bfloat16), torch.randn(2, 128, 256, device="cuda").to(torch.bfloat16)
+big = torch.randn(700, 256, device="cuda").to(torch.bfloat16)
+off, off2 = (torch.tensor(v, device="cuda", dtype=torch.int32) for v in ([0, 7, 20], [0, 600, 700]))
+w = torch.ones(256, device="cuda")
+torch.cuda.synchronize()
+graph = torch.cuda.CUDAGraph()
+with torch.cuda.graph(graph):
+    c, d = e.gemm_grouped_bf16(a, off, b), e.gemm_grouped_bf16(big, off2, b)
+    y, _, s, rstd = e.rms_norm(big, w)
+    dx, dw = e.rms_norm_backward(big, s, w, rstd)
+    db = e.gemm_grouped_bf16_wgrad(d, big, off2)
+graph.replay()
+torch.cuda.synchronize()
+assert torch.equal(c, e.gemm_grouped_bf16(a, off, b)) and torch.equal(d, e.gemm_grouped_bf16(big, off2, b))
+assert torch.equal(db, e.gemm_grouped_bf16_wgrad(d, big, off2)) and torch.equal(dx, e.rms_norm_backward(big, s, w, rstd)[0])
+assert e.last_status() == (o.OK, 0)
+print("captured")
+"""
+    import os
+    import subprocess
+    import sys
+    root = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
+    r = subprocess.run([sys.executable, "-c", code.format(root=root)], capture_output=True, text=True, timeout=300)
+    assert r.returncode == 0 and "captured" in r.stdout, r.stderr[-2000:]
+
+
+def test_thousands_of_groups(eng):
+    G, N, K = 3000, 16, 64
+    g = gen(14)
+    sizes = [1 if i % 31 == 0 else 0 for i in range(G)]
+    sizes[-1] = 40
+    T = sum(sizes)
+    a, b = bf16((T, K), g), bf16((G, N, K), g)
+    want, size = grouped(a.double(), sizes, b.double().mT)
+    close_bf16(eng.gemm_grouped_bf16(a, offsets_of(sizes), b), want, size, K)
+
+
 def test_gradients_of_a_grouped_layer_agree_with_differences(eng):
     """loss = sum(W . (A B^T)) by group: its gradients through the input_grad and weight_grad forms against
     central differences in 64 bits of the same loss."""
