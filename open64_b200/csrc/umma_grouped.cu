@@ -55,7 +55,7 @@ constexpr int kGpScaleSlots = 3;
 constexpr int kGpScaleFloats = 132;  // this CTA's 128 rows, then the two column blocks
 constexpr int kGpScales = kGpStaging + 8 * kEpiStagingBytesPerWarp;
 constexpr int kGpBars = kGpScales + kGpScaleSlots * kGpScaleFloats * 4;
-constexpr int kGpNumBars = 2 * kGpStages + 9 + 2 * kGpScaleSlots;
+constexpr int kGpNumBars = 2 * kGpStages + 10 + 2 * kGpScaleSlots;
 static_assert(kGpBars % 8 == 0, "barriers");
 constexpr int kGpTmemPtr = kGpBars + 8 * kGpNumBars;
 constexpr int kGpAbort = kGpTmemPtr + 4;
@@ -137,6 +137,7 @@ grouped_pair_kernel(const __grid_constant__ CUtensorMap tm_a, const __grid_const
     const uint32_t tail_bar = bar_base + 8u * (2 * kGpStages + 4);
     auto scale_full_bar = [&](int s) { return bar_base + 8u * (2 * kGpStages + 9 + s); };
     auto scale_empty_bar = [&](int s) { return bar_base + 8u * (2 * kGpStages + 9 + kGpScaleSlots + s); };
+    const uint32_t cleared_bar = bar_base + 8u * (2 * kGpStages + 9 + 2 * kGpScaleSlots);  // first CTA: the second's tail is cleared
     auto half_bar = [&](int quarter) { return bar_base + 8u * (2 * kGpStages + 5 + quarter); };
     volatile uint32_t *tmem_ptr_smem = reinterpret_cast<volatile uint32_t *>(smem_gen + kGpTmemPtr);
     volatile int *abort_flag = reinterpret_cast<volatile int *>(smem_gen + kGpAbort);
@@ -149,7 +150,7 @@ grouped_pair_kernel(const __grid_constant__ CUtensorMap tm_a, const __grid_const
 
     if (threadIdx.x == 0) {
         for (int s = 0; s < kGpStages; ++s) {
-            mbar_init(full_bar(s), WGRAD ? 2 : 1);  // first CTA: its loader's arrival (WGRAD: both loaders')
+            mbar_init(full_bar(s), 1);  // first CTA: its loader's arrival
             mbar_init(empty_bar(s), 1);
         }
         for (int b = 0; b < 2; ++b) {
@@ -157,6 +158,7 @@ grouped_pair_kernel(const __grid_constant__ CUtensorMap tm_a, const __grid_const
             mbar_init(acc_empty_bar(b), 16);  // eight warps in each CTA
         }
         mbar_init(tail_bar, 1);
+        mbar_init(cleared_bar, 1);
         for (int s = 0; s < kGpScaleSlots; ++s) {
             mbar_init(scale_full_bar(s), 1);
             mbar_init(scale_empty_bar(s), 8);
@@ -203,6 +205,11 @@ grouped_pair_kernel(const __grid_constant__ CUtensorMap tm_a, const __grid_const
         for (int i = pair_id; ok && next_tile<WGRAD>(p, walk, i, kBlockK, t); i += num_pairs) {
             const int m0 = t.mb * kGpTileM + (int)rank * kBlockM;
             const int n0 = t.nb * kOutN;
+            // WGRAD: the maps count the columns in groups of 64 or, where the last group is not whole, one by one (two
+            // boxes a stage instead of four: the issuing thread needs about 100 cycles for each)
+            [[maybe_unused]] const int xa = p.a_groups ? 0 : m0, za = p.a_groups ? m0 / kKnCols : 0;
+            [[maybe_unused]] const int xb = p.b_groups ? 0 : n0 + (int)rank * 128, zb = p.b_groups ? (n0 + (int)rank * 128) / kKnCols : 0;
+            [[maybe_unused]] const int whole = (t.end - t.begin) % kMmaK == 0 ? t.kbs : (t.end - t.begin) / kBlockK;
             for (int kb = 0; kb < t.kbs; ++kb) {
                 ok = mbar_wait_bounded(empty_bar(stage), phase ^ 1u, abort_flag, p.status, kWaitGroupProducer, p.wait_ns);
                 ok = __all_sync(0xffffffffu, ok);
@@ -212,48 +219,45 @@ grouped_pair_kernel(const __grid_constant__ CUtensorMap tm_a, const __grid_const
                 const uint32_t full0 = map_to_cta(full_bar(stage), 0);
                 if constexpr (WGRAD) {
                     const int row = t.begin + kb * kBlockK;
-                    const int left = t.end - row;
-                    // the last block of a group: its loads complete here first, and the rows up to the next
-                    // whole K step are cleared in both operands (whatever lies behind the group may be NaN)
-                    const bool cut = left < kBlockK && left % kMmaK != 0;
-                    const uint32_t bar = cut ? map_to_cta(tail_bar, rank) : full0;
-                    if (leader) {
-                        if (cut)
+                    auto load = [&](uint32_t bar) __attribute__((always_inline)) {
+                        tma_load_3d_pair(a_dst, &tm_a, xa, row, za, bar);
+                        tma_load_3d_pair(b_dst, &tm_b, xb, row, zb, bar);
+                        if (!p.a_groups) tma_load_3d_pair(a_dst + kKnGroupBytes, &tm_a, xa + kKnCols, row, 0, bar);
+                        if (!p.b_groups) tma_load_3d_pair(b_dst + kKnGroupBytes, &tm_b, xb + kKnCols, row, 0, bar);
+                    };
+                    if (kb < whole) {
+                        if (leader) {
+                            if (rank == 0) mbar_arrive_expect_tx(full_bar(stage), 2 * kGpStageBytes);
+                            load(full0);
+                        }
+                    } else {
+                        // the last block of a group: its loads complete here first, and the rows up to the next whole
+                        // K step are cleared in both operands (whatever lies behind the group may be NaN); the
+                        // second CTA says so to the first, whose arrival stands for both
+                        if (leader) {
                             mbar_arrive_expect_tx(tail_bar, kGpStageBytes);
-                        else if (rank == 0)
-                            mbar_arrive_expect_tx(full_bar(stage), 2 * kGpStageBytes);
-                        else
-                            mbar_arrive_cluster(full0);
-                        // (the maps count the columns in groups of 64 or, where the last group is not whole, one by one;
-                        // two boxes a stage instead of four: the issuing thread needs about 120 cycles for each)
-                        if (p.a_groups) {
-                            tma_load_3d_pair(a_dst, &tm_a, 0, row, m0 / kKnCols, bar);
-                        } else {
-#pragma unroll
-                            for (int c = 0; c < kKnGroups; ++c) tma_load_3d_pair(a_dst + c * kKnGroupBytes, &tm_a, m0 + c * kKnCols, row, 0, bar);
+                            load(map_to_cta(tail_bar, rank));
                         }
-                        if (p.b_groups) {
-                            tma_load_3d_pair(b_dst, &tm_b, 0, row, (n0 + (int)rank * 128) / kKnCols, bar);
-                        } else {
-#pragma unroll
-                            for (int c = 0; c < kKnGroups; ++c)
-                                tma_load_3d_pair(b_dst + c * kKnGroupBytes, &tm_b, n0 + (int)rank * 128 + c * kKnCols, row, 0, bar);
-                        }
-                    }
-                    __syncwarp();
-                    if (cut) {
+                        __syncwarp();
                         ok = mbar_wait_bounded(tail_bar, tail_phase, abort_flag, p.status, kWaitGroupTail, p.wait_ns);
                         ok = __all_sync(0xffffffffu, ok);
-                        tail_phase ^= 1u;
                         if (!ok) break;
-                        const int first = left, last = (left + kMmaK - 1) / kMmaK * kMmaK;
+                        const int first = t.end - row, last = (first + kMmaK - 1) / kMmaK * kMmaK;
                         uint8_t *at = smem_gen + stage * kGpStageBytes;
                         for (int c = 0; c < 2 * kKnGroups; ++c)
                             for (int q = first * 8 + lane; q < last * 8; q += 32)
                                 reinterpret_cast<uint4 *>(at + c * kKnGroupBytes)[q] = make_uint4(0, 0, 0, 0);
                         fence_proxy_async_smem();
                         __syncwarp();
-                        if (leader) mbar_arrive_cluster(full0);
+                        if (rank == 1) {
+                            if (leader) mbar_arrive_cluster(map_to_cta(cleared_bar, 0));
+                        } else {
+                            ok = mbar_wait_bounded(cleared_bar, tail_phase, abort_flag, p.status, kWaitGroupTail, p.wait_ns);
+                            ok = __all_sync(0xffffffffu, ok);
+                            if (!ok) break;
+                            if (leader) mbar_arrive(full_bar(stage));
+                        }
+                        tail_phase ^= 1u;
                     }
                 } else if (leader) {
                     if (rank == 0) mbar_arrive_expect_tx(full_bar(stage), 2 * kGpStageBytes);
@@ -326,11 +330,15 @@ grouped_pair_kernel(const __grid_constant__ CUtensorMap tm_a, const __grid_const
                     int steps = kRowBytes / 32;
                     if constexpr (WGRAD) steps = min(steps, (t.end - t.begin - kb * kBlockK + kMmaK - 1) / kMmaK);
                     if (leader) {
+                        if (steps == kRowBytes / 32) {
 #pragma unroll
-                        for (int k = 0; k < kRowBytes / 32; ++k)
-                            if (!WGRAD || k < steps)
+                            for (int k = 0; k < kRowBytes / 32; ++k)
                                 tc_mma_pair<KIND>(d_tmem, a_desc + kAAdvance * k, b_desc + kBAdvance * k, idesc,
                                                   (kScaled ? k : (kb | k)) != 0 ? 1u : 0u);
+                        } else {
+                            for (int k = 0; k < steps; ++k)
+                                tc_mma_pair<KIND>(d_tmem, a_desc + kAAdvance * k, b_desc + kBAdvance * k, idesc, (kb | k) != 0 ? 1u : 0u);
+                        }
                         tc_commit_pair_mask(empty_bar(stage), 3);
                         if (kScaled) tc_commit_pair_mask(acc_full_bar(uses & 1), 3);
                     }
