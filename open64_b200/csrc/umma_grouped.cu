@@ -29,7 +29,7 @@
 // first warpgroup gives its registers up (setmaxnreg: 128 x 56 + 256 x 224 = the 384 x 168 of the launch).
 //
 // Measured: bf16, one group, 4096 x 8192 x 8192: 324 us = 1696 TFLOP/s (bound by the tensor pipe, busy 95 % of the time);
-// its weight gradient 392 us; e4m3 with block scales 248 us = 2215 TFLOP/s, 870 cycles a K block: MMA, commit, the way
+// its weight gradient 340 us; e4m3 with block scales 248 us = 2215 TFLOP/s, 870 cycles a K block: MMA, commit, the way
 // through registers (350 cycles) and the release across the pair are one chain over two buffers (the product without
 // block scales: 194 us).  Two MMAs of 128 columns a block with four buffers: 263 us (their issue and A's second read).
 // Every wait is bounded, as in the other kernels.
