@@ -391,7 +391,7 @@ class Engine:
             raise O64Error(_lib.ERR_DTYPE, "rms_norm: scales of a bf16 result")
         if rstd is None:
             rstd = x.new_empty((T,), dtype=_F32)
-        elif T > 1 and _want(rstd, "rstd", (_F32,), (T,)).stride(0) != 1:
+        elif _want(rstd, "rstd", (_F32,), (T,)).stride(0) != 1 and T > 1:
             raise O64Error(_lib.ERR_CONFORM, "rms_norm: rstd is not contiguous")
         rc = self.lib.o64_rmsnorm_bf16(self._h, T, N, x.data_ptr(), _ld(x), p_residual, ldr, p_summed, lds, weight.data_ptr(),
                                        weight.dtype is _F32, eps, out_kind, scale_block, y.data_ptr(), ldy, p_scales, ldscales,

@@ -281,6 +281,9 @@ def test_refusals(eng):
     wide = torch.zeros((1, 32769), device="cuda", dtype=torch.bfloat16)
     refused(o.ERR_RANK, lambda: eng.rms_norm(wide, wide[0].float()))
     refused(o.ERR_RANK, lambda: eng.rms_norm(x[:, :0], w[:0]))
+    refused(o.ERR_DTYPE, lambda: eng.rms_norm(x[:1], w, rstd=torch.empty(1, device="cuda", dtype=torch.float64)))
+    refused(o.ERR_CONFORM, lambda: eng.rms_norm(x, w, rstd=torch.empty(8, device="cuda")[::2]))
+    refused(o.ERR_CONFORM, lambda: eng.rms_norm_backward(x, x, w, torch.empty(3, device="cuda")))
     L, P = eng.lib, lambda t: t.data_ptr()
     s = torch.cuda.current_stream().cuda_stream
     call = lambda **k: L.o64_rmsnorm_bf16(*{**dict(h=eng._h, T=4, N=256, X=P(x), ldx=256, R=None, ldr=0, S=None, lds=0, W=P(w), f=1, eps=1e-6,
