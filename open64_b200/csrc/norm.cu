@@ -12,8 +12,7 @@
 // Bound by HBM: 16384 x 8192 with the residual to e4m3 155 us = 6.1 TB/s (0.93 of a copy), backward 8192 x 8192 with the
 // residual 94 us = 5.7 TB/s.  Many rows run on a few blocks per SM that stay: rows come in by bulk copies, a ring of
 // three ahead, so that loads go on while a row is reduced, converted and stored, and a thread keeps its
-// columns of w.  Few rows, or rows that are not 16-byte aligned, run on a block per row that loads for
-// itself.
+// columns of w.  Few rows run on a block per row that loads for itself.
 //
 // Gradient, with n = s * rstd, g = dy * w:   dx = rstd * (g - n * mean(g n)) + dr   (x and r receive
 // the same one),   dw[j] = sum over rows of dy n.  The sum over rows runs in two fixed stages (a
@@ -444,6 +443,243 @@ __global__ void __launch_bounds__(kRingMaxThreads) norm_forward_ring_kernel(cons
     }
 }
 
+// Rows that start anywhere (odd N, odd pitches): the same ring of the 16-byte chunks that hold any of a row's bytes
+// (an aligned chunk with one byte of an allocation lies inside it), read from shared memory at the row's own offset;
+// results go back through shared memory too, so that a warp's stores are contiguous.  Two bytes at a time straight from
+// and to global memory, 10000 rows of 5003 with the residual took 248 us to e4m3 and 286 us backward;
+// 112 us and 157 us this way.
+struct OddRow {
+    const __nv_bfloat16 *row;
+    __device__ __forceinline__ uint32_t shift() const { return (uint32_t)(reinterpret_cast<uintptr_t>(row) & 15u); }
+    __device__ __forceinline__ uint32_t bytes(int n) const { return (shift() + (uint32_t)n * 2 + 15u) & ~15u; }
+    __device__ __forceinline__ const void *chunks() const { return reinterpret_cast<const uint8_t *>(row) - shift(); }
+};
+__host__ __device__ constexpr uint32_t odd_pitch(int64_t n) { return (uint32_t)((n * 2 + 16 + 127) / 128 * 128); }
+
+// n two-byte (or one-byte) values from shared memory to a row that starts anywhere, by the whole block.
+template <typename T>
+__device__ __forceinline__ void copy_out(T *dst, const T *src, int n) {
+    constexpr int kWord = 4 / sizeof(T);
+    const int head = min((int)((4u - (reinterpret_cast<uintptr_t>(dst) & 3u)) & 3u) / (int)sizeof(T), n);
+    const int words = (n - head) / kWord;
+    for (int k = threadIdx.x; k < words; k += blockDim.x) {
+        uint32_t w = 0;
+#pragma unroll
+        for (int e = 0; e < kWord; ++e) w |= (uint32_t)src[head + k * kWord + e] << (8 * sizeof(T) * e);
+        *reinterpret_cast<uint32_t *>(dst + head + k * kWord) = w;
+    }
+    const int rest = head + words * kWord;
+    if ((int)threadIdx.x < head) dst[threadIdx.x] = src[threadIdx.x];
+    if ((int)threadIdx.x < n - rest) dst[rest + threadIdx.x] = src[rest + threadIdx.x];
+}
+
+template <bool E4M3>
+__global__ void __launch_bounds__(kRingMaxThreads) norm_forward_odd_kernel(const FwdParams p, int stages, int *status, unsigned long long wait_ns) {
+    extern __shared__ __align__(128) uint8_t smem[];
+    __shared__ float slots[2][32];
+    __shared__ __align__(8) uint64_t bars[kNormMaxStages];
+    __shared__ int abort_word;
+    const int n = p.N;
+    const uint32_t pitch = odd_pitch(n);
+    const uint32_t stage_bytes = pitch * (p.R ? 2 : 1);
+    uint8_t *s_out = smem + stages * stage_bytes, *y_out = s_out + pitch;
+    if (threadIdx.x == 0) {
+        for (int s = 0; s < stages; ++s) mbar_init(smem_u32(&bars[s]), 1);
+        abort_word = 0;
+        fence_mbar_init();
+    }
+    __syncthreads();
+    auto load = [&](long long row, int s) {
+        const uint32_t bar = smem_u32(&bars[s]), dst = smem_u32(smem) + s * stage_bytes;
+        const OddRow x{p.X + row * p.ldx}, r{p.R ? p.R + row * p.ldr : nullptr};
+        mbar_arrive_expect_tx(bar, x.bytes(n) + (p.R ? r.bytes(n) : 0));
+        bulk_load(dst, x.chunks(), x.bytes(n), bar);
+        if (p.R) bulk_load(dst + pitch, r.chunks(), r.bytes(n), bar);
+    };
+    if (threadIdx.x == 0)
+        for (int s = 0; s < stages; ++s) {
+            const long long row = blockIdx.x + (long long)s * gridDim.x;
+            if (row < p.T) load(row, s);
+        }
+    float w[kRingNv][8];
+#pragma unroll
+    for (int i = 0; i < kRingNv; ++i) load_w8<false>(p.W, p.w_f32, (i * blockDim.x + threadIdx.x) * 8, n, w[i]);
+    int stage = 0, turn = 0;
+    uint32_t phase = 0;
+    for (long long row = blockIdx.x; row < p.T; row += gridDim.x, turn ^= 1) {
+        mbar_wait_bounded(smem_u32(&bars[stage]), phase, &abort_word, status, kNormWait, wait_ns);
+        const uint8_t *at = smem + stage * stage_bytes;
+        const __nv_bfloat16 *x = reinterpret_cast<const __nv_bfloat16 *>(at + OddRow{p.X + row * p.ldx}.shift());
+        const __nv_bfloat16 *r = p.R ? reinterpret_cast<const __nv_bfloat16 *>(at + pitch + OddRow{p.R + row * p.ldr}.shift()) : nullptr;
+        float v[kRingNv][8];
+        float sq = 0.0f;
+#pragma unroll
+        for (int i = 0; i < kRingNv; ++i) {
+            const int col = (i * blockDim.x + threadIdx.x) * 8;
+#pragma unroll
+            for (int e = 0; e < 8; ++e) {
+                v[i][e] = 0.0f;
+                if (col + e < n) {
+                    v[i][e] = __bfloat162float(x[col + e]);
+                    if (r) v[i][e] += __bfloat162float(r[col + e]);
+                    sq = fmaf(v[i][e], v[i][e], sq);
+                }
+            }
+        }
+#pragma unroll
+        for (int o = 16; o > 0; o >>= 1) sq += __shfl_xor_sync(0xffffffffu, sq, o);
+        if ((threadIdx.x & 31) == 0) slots[turn][threadIdx.x >> 5] = sq;
+        __syncthreads();  // the stage is in registers, the last row's results have left
+        if (threadIdx.x == 0 && row + (long long)stages * gridDim.x < p.T) {
+            fence_proxy_async_smem();
+            load(row + (long long)stages * gridDim.x, stage);
+        }
+        const float rstd = 1.0f / sqrtf(block_sum(slots[turn]) / (float)n + p.eps);
+        if (p.rstd && threadIdx.x == 0) p.rstd[row] = rstd;
+#pragma unroll
+        for (int i = 0; i < kRingNv; ++i) {
+            const int col = (i * blockDim.x + threadIdx.x) * 8;
+            // (whole vectors: the buffers have room behind the row)
+            if (p.S && col < n) store8<true>(reinterpret_cast<__nv_bfloat16 *>(s_out), col, n, v[i]);
+            float m = 0.0f;
+#pragma unroll
+            for (int e = 0; e < 8; ++e) {
+                v[i][e] = v[i][e] * rstd * w[i][e];
+                if (E4M3 && col + e < n) m = max_nan(m, fabsf(v[i][e]));
+            }
+            if constexpr (!E4M3) {
+                if (col < n) store8<true>(reinterpret_cast<__nv_bfloat16 *>(y_out), col, n, v[i]);
+            } else {
+#pragma unroll
+                for (int o = 8; o > 0; o >>= 1) m = max_nan(m, __shfl_xor_sync(0xffffffffu, m, o));
+                const float scale = scale_of(m);
+                const float inv = __fdividef(1.0f, scale);
+                if (col < n) {
+                    if ((threadIdx.x & 15) == 0) p.scales[row * p.ldscales + col / 128] = scale;
+                    *reinterpret_cast<uint2 *>(y_out + col) = quant8(v[i], inv);
+                }
+            }
+        }
+        __syncthreads();
+        if (p.S) copy_out(reinterpret_cast<uint16_t *>(p.S + row * p.lds), reinterpret_cast<const uint16_t *>(s_out), n);
+        if constexpr (E4M3)
+            copy_out(static_cast<uint8_t *>(p.Y) + row * p.ldy, y_out, n);
+        else
+            copy_out(static_cast<uint16_t *>(p.Y) + row * p.ldy, reinterpret_cast<const uint16_t *>(y_out), n);
+        if (++stage == stages) {
+            stage = 0;
+            phase ^= 1u;
+        }
+    }
+    if (abort_word) {
+        const uint64_t t0 = globaltimer_ns();
+        while (globaltimer_ns() - t0 < 200000ull) __nanosleep(1000);
+    }
+}
+
+__global__ void __launch_bounds__(kRingMaxThreads) norm_backward_odd_kernel(const BwdParams p, int stages, int *status, unsigned long long wait_ns) {
+    extern __shared__ __align__(128) uint8_t smem[];
+    __shared__ float slots[2][32];
+    __shared__ __align__(8) uint64_t bars[kNormMaxStages];
+    __shared__ int abort_word;
+    const int n = p.N;
+    const uint32_t pitch = odd_pitch(n);
+    const uint32_t stage_bytes = pitch * (p.dR ? 3 : 2);
+    uint8_t *dx_out = smem + stages * stage_bytes;
+    if (threadIdx.x == 0) {
+        for (int s = 0; s < stages; ++s) mbar_init(smem_u32(&bars[s]), 1);
+        abort_word = 0;
+        fence_mbar_init();
+    }
+    __syncthreads();
+    auto load = [&](long long row, int s) {
+        const uint32_t bar = smem_u32(&bars[s]), dst = smem_u32(smem) + s * stage_bytes;
+        const OddRow y{p.dY + row * p.lddy}, z{p.S + row * p.lds}, r{p.dR ? p.dR + row * p.lddr : nullptr};
+        mbar_arrive_expect_tx(bar, y.bytes(n) + z.bytes(n) + (p.dR ? r.bytes(n) : 0));
+        bulk_load(dst, y.chunks(), y.bytes(n), bar);
+        bulk_load(dst + pitch, z.chunks(), z.bytes(n), bar);
+        if (p.dR) bulk_load(dst + 2 * pitch, r.chunks(), r.bytes(n), bar);
+    };
+    if (threadIdx.x == 0)
+        for (int s = 0; s < stages; ++s) {
+            const long long row = blockIdx.x + (long long)s * gridDim.x;
+            if (row < p.T) load(row, s);
+        }
+    float dw[kRingNv][8], w[kRingNv][8];
+#pragma unroll
+    for (int i = 0; i < kRingNv; ++i) {
+        load_w8<false>(p.W, p.w_f32, (i * blockDim.x + threadIdx.x) * 8, n, w[i]);
+#pragma unroll
+        for (int e = 0; e < 8; ++e) dw[i][e] = 0.0f;
+    }
+    int stage = 0, turn = 0;
+    uint32_t phase = 0;
+    for (long long row = blockIdx.x; row < p.T; row += gridDim.x, turn ^= 1) {
+        const float rstd = p.rstd[row];
+        mbar_wait_bounded(smem_u32(&bars[stage]), phase, &abort_word, status, kNormWait, wait_ns);
+        const uint8_t *at = smem + stage * stage_bytes;
+        const __nv_bfloat16 *dy = reinterpret_cast<const __nv_bfloat16 *>(at + OddRow{p.dY + row * p.lddy}.shift());
+        const __nv_bfloat16 *z = reinterpret_cast<const __nv_bfloat16 *>(at + pitch + OddRow{p.S + row * p.lds}.shift());
+        const __nv_bfloat16 *dr = p.dR ? reinterpret_cast<const __nv_bfloat16 *>(at + 2 * pitch + OddRow{p.dR + row * p.lddr}.shift()) : nullptr;
+        float dot = 0.0f;
+#pragma unroll
+        for (int i = 0; i < kRingNv; ++i) {
+            const int col = (i * blockDim.x + threadIdx.x) * 8;
+#pragma unroll
+            for (int e = 0; e < 8; ++e)
+                if (col + e < n) {
+                    const float g = __bfloat162float(dy[col + e]), x = __bfloat162float(z[col + e]) * rstd;
+                    dw[i][e] = fmaf(g, x, dw[i][e]);
+                    dot = fmaf(g * w[i][e], x, dot);
+                }
+        }
+#pragma unroll
+        for (int o = 16; o > 0; o >>= 1) dot += __shfl_xor_sync(0xffffffffu, dot, o);
+        if ((threadIdx.x & 31) == 0) slots[turn][threadIdx.x >> 5] = dot;
+        __syncthreads();  // (the last row's results have left, too)
+        const float mean = block_sum(slots[turn]) / (float)n;
+#pragma unroll
+        for (int i = 0; i < kRingNv; ++i) {
+            const int col = (i * blockDim.x + threadIdx.x) * 8;
+            float out[8];
+#pragma unroll
+            for (int e = 0; e < 8; ++e) {
+                out[e] = 0.0f;
+                if (col + e < n) {
+                    out[e] = rstd * (__bfloat162float(dy[col + e]) * w[i][e] - __bfloat162float(z[col + e]) * rstd * mean);
+                    if (dr) out[e] += __bfloat162float(dr[col + e]);
+                }
+            }
+            if (col < n) store8<true>(reinterpret_cast<__nv_bfloat16 *>(dx_out), col, n, out);
+        }
+        __syncthreads();
+        if (threadIdx.x == 0 && row + (long long)stages * gridDim.x < p.T) {
+            fence_proxy_async_smem();
+            load(row + (long long)stages * gridDim.x, stage);
+        }
+        copy_out(reinterpret_cast<uint16_t *>(p.dX + row * p.lddx), reinterpret_cast<const uint16_t *>(dx_out), n);
+        if (++stage == stages) {
+            stage = 0;
+            phase ^= 1u;
+        }
+    }
+    griddep_launch_dependents();
+    if (p.partial) {
+        float *dst = p.partial + (long long)blockIdx.x * n;
+#pragma unroll
+        for (int i = 0; i < kRingNv; ++i)
+#pragma unroll
+            for (int e = 0; e < 8; ++e) {
+                const int col = (i * blockDim.x + threadIdx.x) * 8 + e;
+                if (col < n) dst[col] = dw[i][e];
+            }
+    }
+    if (abort_word) {
+        const uint64_t t0 = globaltimer_ns();
+        while (globaltimer_ns() - t0 < 200000ull) __nanosleep(1000);
+    }
+}
+
 __global__ void __launch_bounds__(kRingMaxThreads) norm_backward_ring_kernel(const BwdParams p, int stages, int w_in_smem, int *status, unsigned long long wait_ns) {
     extern __shared__ __align__(128) uint8_t smem[];
     __shared__ float slots[2][32];
@@ -633,10 +869,11 @@ struct RingShape {
     int threads, blocks_per_sm, stages;
     size_t smem;
 };
-bool ring_shape(int64_t N, int operands, int extra_bytes_per_col, RingShape *r) {
+bool ring_shape(int64_t N, int operands, int extra_bytes_per_col, RingShape *r, bool odd = false) {
     r->threads = threads_for(N, kRingNv);
     if (r->threads > kRingMaxThreads) return false;
-    const size_t row = (size_t)((N * 2 + 127) / 128 * 128) * operands, extra = (size_t)N * extra_bytes_per_col;
+    const size_t row = odd ? (size_t)odd_pitch(N) * operands : (size_t)((N * 2 + 127) / 128 * 128) * operands;
+    const size_t extra = odd ? (size_t)odd_pitch(N) * 2 : (size_t)N * extra_bytes_per_col;  // odd: two rows of results
     const int most = std::min(16, 1024 / r->threads);
     for (int b = most; b >= 1; --b)
         for (int s = 3; s >= 2; --s)
@@ -660,6 +897,25 @@ int launch_forward_ring(const FwdParams &p, const RingShape &r, const NormCall &
     const int rc = allow_smem(kern, ks);
     if (rc) return rc;
     kern<<<r.blocks_per_sm * num_sms, r.threads, r.smem, c.stream>>>(p, r.stages, c.status, c.wait_ns);
+    return cudaGetLastError() == cudaSuccess ? O64_OK : O64_ERR_CUDA;
+}
+
+template <bool E4M3>
+int launch_forward_odd(const FwdParams &p, const RingShape &r, const NormCall &c, int num_sms) {
+    static KernelSetup ks;
+    auto kern = norm_forward_odd_kernel<E4M3>;
+    const int rc = allow_smem(kern, ks);
+    if (rc) return rc;
+    kern<<<r.blocks_per_sm * num_sms, r.threads, r.smem, c.stream>>>(p, r.stages, c.status, c.wait_ns);
+    return cudaGetLastError() == cudaSuccess ? O64_OK : O64_ERR_CUDA;
+}
+
+int launch_backward_odd(const BwdParams &p, const RingShape &r, const NormBackwardCall &c, int grid) {
+    static KernelSetup ks;
+    auto kern = norm_backward_odd_kernel;
+    const int rc = allow_smem(kern, ks);
+    if (rc) return rc;
+    kern<<<grid, r.threads, r.smem, c.stream>>>(p, r.stages, c.status, c.wait_ns);
     return cudaGetLastError() == cudaSuccess ? O64_OK : O64_ERR_CUDA;
 }
 
@@ -689,6 +945,8 @@ int norm_forward(const NormCall &c, int num_sms) {
     if (vec && !(e4m3 && c.row_scale) && c.N >= kRingCols && ring_shape(c.N, c.R ? 2 : 1, 0, &r) && c.T >= (int64_t)2 * r.blocks_per_sm * num_sms) {
         return e4m3 ? launch_forward_ring<true>(p, r, c, num_sms) : launch_forward_ring<false>(p, r, c, num_sms);
     }
+    if (!vec && !(e4m3 && c.row_scale) && c.N >= kRingCols && ring_shape(c.N, c.R ? 2 : 1, 0, &r, true) && c.T >= (int64_t)2 * r.blocks_per_sm * num_sms)
+        return e4m3 ? launch_forward_odd<true>(p, r, c, num_sms) : launch_forward_odd<false>(p, r, c, num_sms);
     const int nv = pick_nv(c.N, c.T <= 2 * num_sms ? 1 : 4);
     const int tpr = threads_for(c.N, nv);
     const int rows = tpr >= 128 ? 1 : 128 / tpr;
@@ -763,6 +1021,12 @@ int norm_backward(const NormBackwardCall &c, int num_sms) {
         const int rc = launch_backward_ring(p, r, c, grid, w_in_smem);
         if (rc) return rc;
         return c.dW ? add_partials(c, grid) : O64_OK;
+    }
+    if (!vec && c.N >= kRingCols && ring_shape(c.N, c.dR ? 3 : 2, 0, &r, true) && c.T >= (int64_t)2 * r.blocks_per_sm * num_sms) {
+        const int odd_grid = (int)std::min<int64_t>((int64_t)r.blocks_per_sm * num_sms, blocks * block.y);
+        const int rc = launch_backward_odd(p, r, c, odd_grid);
+        if (rc) return rc;
+        return c.dW ? add_partials(c, odd_grid) : O64_OK;
     }
     const unsigned grid = (unsigned)blocks;
     switch (nv) {

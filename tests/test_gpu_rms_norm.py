@@ -79,7 +79,7 @@ def test_e4m3(eng, T, N, block):
     check_e4m3(y, scales, h, size, block)
 
 
-MANY = [(1500, 2048), (1000, 4096), (1200, 5000), (601, 8192), (300, 16384), (890, 2056)]  # rows in a ring of bulk copies
+MANY = [(1500, 2048), (1000, 4096), (1200, 5000), (601, 8192), (300, 16384), (890, 2056), (4800, 257), (1300, 5003), (2500, 1001), (601, 8190), (300, 16383)]  # rows in a ring of bulk copies
 
 
 @pytest.mark.parametrize("T,N", MANY)
@@ -160,7 +160,7 @@ def test_offsets_past_32_bits(eng):
 
 
 BACK = [(1, 1), (1, 4096), (3, 64), (5, 127), (130, 128), (64, 1000), (1000, 512), (445, 2141), (900, 4096), (50, 5000), (13, 8192), (3, 16392),
-        (2, 32768), (4, 32761), (2000, 2048), (1300, 5000), (601, 8192), (305, 16384), (888, 4104)]
+        (2, 32768), (4, 32761), (2000, 2048), (1300, 5000), (601, 8192), (305, 16384), (888, 4104), (4800, 257), (1300, 5003), (2500, 1001), (601, 8190), (305, 16383)]
 
 
 @pytest.mark.parametrize("T,N", BACK)
@@ -219,6 +219,28 @@ def test_backward_in_place_and_without_weight_gradient(eng):
     rc = eng.lib.o64_rmsnorm_bf16_backward(eng._h, T, N, P(dy), N, P(s), N, P(w), 1, P(rstd), P(r), N, P(out), N, None, None,
                                            torch.cuda.current_stream().cuda_stream)
     assert rc == o.OK and torch.equal(out, want)
+
+
+@pytest.mark.parametrize("T,N", [(1300, 5003), (1500, 2048), (4800, 257)])
+def test_many_rows_in_place(eng, T, N):
+    """dx over dr, the sum over the residual, in rows that share 16-byte chunks with their neighbours."""
+    x, r, w = data(T, N, 31)
+    want = eng.rms_norm(x, w, r)
+    r2 = r.clone()
+    got = eng.rms_norm(x, w, r2, summed=r2)
+    assert got[2] is r2 and all(torch.equal(a, b) for a, b in zip((got[0], got[2], got[3]), (want[0], want[2], want[3])))
+    dx, dw = eng.rms_norm_backward(x, want[2], w, want[3], r)
+    r3 = r.clone()
+    got = eng.rms_norm_backward(x, want[2], w, want[3], r3, dx=r3)
+    assert got[0] is r3 and torch.equal(r3, dx) and torch.equal(got[1], dw)
+    x2 = x.clone()
+    got = eng.rms_norm_backward(x2, want[2], w, want[3], r, dx=x2)
+    assert torch.equal(x2, dx) and torch.equal(got[1], dw)
+    view = torch.zeros((T * N + 1,), device="cuda", dtype=torch.bfloat16)[1:].view(T, N)  # a base off 16 bytes
+    view.copy_(x)
+    odd = eng.rms_norm(view, w, r, out_kind=o.OUT_E4M3)
+    _, _, h, size = formula(x, r, w, 1e-6)
+    check_e4m3(odd[0], odd[1], h, size, 128)
 
 
 def test_no_rows(eng):
