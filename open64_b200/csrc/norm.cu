@@ -9,7 +9,7 @@
 // norm is taken of the sum in fp32; the stream s that goes on to the next layer is that sum rounded
 // to bf16 once.
 //
-// Bound by HBM: 16384 x 8192 with the residual to e4m3 155 us = 6.1 TB/s (0.93 of a copy), backward 8192 x 8192 with the
+// Bound by HBM: 16384 x 8192 with the residual to e4m3 159 us = 5.9 TB/s (0.91 of a copy), backward 8192 x 8192 with the
 // residual 94 us = 5.7 TB/s.  Many rows run on a few blocks per SM that stay: rows come in by bulk copies, a ring of
 // three ahead, so that loads go on while a row is reduced, converted and stored, and a thread keeps its
 // columns of w.  Few rows run on a block per row that loads for itself.
@@ -137,10 +137,12 @@ struct FwdParams {
     int w_f32, row_scale;
 };
 
-// amax / 448, by the reciprocal: within an ulp (with this and a fast 1 / scale 6247 rows of 9984 take 61 us, with two
-// divisions per eight values 65)
+// amax / 448, and 1 / scale where it is used, are correctly rounded divisions: by a reciprocal and a fast division about
+// as many values again fell on the other side of a rounding to e4m3 (46 rows of 13664, relative error 4.7e-05 instead of
+// 1.1e-05). They cost 16384 x 8192 159 us instead of 155, and 6247 rows of 9984 65 us instead of 61. A division per value
+// took 194 us and left as many (1060 of 134 million values instead of 1176).
 __device__ __forceinline__ float scale_of(float amax) {
-    const float s = amax * (1.0f / kE4m3Max);
+    const float s = amax / kE4m3Max;
     return s < kMinNormal ? 1.0f : s;  // (NaN stays NaN)
 }
 
@@ -213,9 +215,9 @@ __global__ void __launch_bounds__(kNormMaxThreads) norm_forward_kernel(const Fwd
                 scale = scale_of(m);
                 if (col < n && (threadIdx.x & 15) == 0) p.scales[row * p.ldscales + col / 128] = scale;
             }
-            // one reciprocal per block instead of a division per value: within an ulp of h / scale before
+            // one reciprocal per block instead of a division per value: within 1.5 ulp of h / scale before
             // the rounding to four bits
-            const float inv = __fdividef(1.0f, scale);
+            const float inv = 1.0f / scale;
             const uint2 q2 = quant8(v[i], inv);
             const uint32_t q[2] = {q2.x, q2.y};
             if constexpr (VEC) {
@@ -425,7 +427,7 @@ __global__ void __launch_bounds__(kRingMaxThreads) norm_forward_ring_kernel(cons
 #pragma unroll
                 for (int o = 8; o > 0; o >>= 1) m = max_nan(m, __shfl_xor_sync(0xffffffffu, m, o));
                 const float scale = scale_of(m);
-                const float inv = __fdividef(1.0f, scale);
+                const float inv = 1.0f / scale;
                 if (col < n) {
                     if ((threadIdx.x & 15) == 0) p.scales[row * p.ldscales + col / 128] = scale;
                     *reinterpret_cast<uint2 *>(static_cast<uint8_t *>(p.Y) + row * p.ldy + col) = quant8(v[i], inv);
@@ -553,7 +555,7 @@ __global__ void __launch_bounds__(kRingMaxThreads) norm_forward_odd_kernel(const
 #pragma unroll
                 for (int o = 8; o > 0; o >>= 1) m = max_nan(m, __shfl_xor_sync(0xffffffffu, m, o));
                 const float scale = scale_of(m);
-                const float inv = __fdividef(1.0f, scale);
+                const float inv = 1.0f / scale;
                 if (col < n) {
                     if ((threadIdx.x & 15) == 0) p.scales[row * p.ldscales + col / 128] = scale;
                     *reinterpret_cast<uint2 *>(y_out + col) = quant8(v[i], inv);
