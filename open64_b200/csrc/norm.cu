@@ -9,7 +9,7 @@
 // norm is taken of the sum in fp32; the stream s that goes on to the next layer is that sum rounded
 // to bf16 once.
 //
-// Bound by HBM: 16384 x 8192 with the residual to e4m3 159 us = 5.9 TB/s (0.91 of a copy), backward 8192 x 8192 with the
+// Bound by HBM: 16384 x 8192 with the residual to e4m3 157 us = 6.0 TB/s (0.92 of a copy), backward 8192 x 8192 with the
 // residual 94 us = 5.7 TB/s.  Many rows run on a few blocks per SM that stay: rows come in by bulk copies, a ring of
 // three ahead, so that loads go on while a row is reduced, converted and stored, and a thread keeps its
 // columns of w.  Few rows run on a block per row that loads for itself.
@@ -21,6 +21,7 @@
 #include <cuda_fp8.h>
 
 #include <algorithm>
+#include <cfloat>
 
 #include "norm.cuh"
 #include "ptx_sm100.cuh"
@@ -114,11 +115,20 @@ __device__ __forceinline__ float row_reduce(float v, float *slot) {
     return r;
 }
 
-__device__ __forceinline__ uint2 quant8(const float (&v)[8], float inv) {
+// Eight values over the scale of their block, inv = 1 / scale, to e4m3. One division per block: the product with inv is
+// off by up to 1.5 ulp, which puts some values on the other side of a rounding to four bits, so a step with the
+// product's own remainder follows, q - (q scale - v) inv, in two packed multiply-adds. 16384 x 8192: 1060 of 134
+// million values are other than from 64 bits, 1176 without the step, as many as with it from a division per value,
+// which takes 194 us instead of 157. (With q scale - v and not v - q scale a zero keeps its sign.) Under an infinite scale
+// inv is 0 and nothing is to be put right: the remainder would be 0 * inf.
+__device__ __forceinline__ uint2 quant8(const float (&v)[8], float scale, float inv) {
+    const float back = scale <= FLT_MAX ? scale : 0.0f;
     uint32_t q[2] = {0, 0};
 #pragma unroll
     for (int e = 0; e < 4; ++e) {
-        const float2 two = make_float2(v[2 * e] * inv, v[2 * e + 1] * inv);
+        float2 two = make_float2(v[2 * e] * inv, v[2 * e + 1] * inv);
+        const float2 rest = __ffma2_rn(two, make_float2(back, back), make_float2(-v[2 * e], -v[2 * e + 1]));
+        two = __ffma2_rn(rest, make_float2(-inv, -inv), two);
         q[e >> 1] |= (uint32_t)__nv_cvt_float2_to_fp8x2(two, __NV_SATFINITE, __NV_E4M3) << (16 * (e & 1));
     }
     return make_uint2(q[0], q[1]);
@@ -137,10 +147,6 @@ struct FwdParams {
     int w_f32, row_scale;
 };
 
-// amax / 448, and 1 / scale where it is used, are correctly rounded divisions: by a reciprocal and a fast division about
-// as many values again fell on the other side of a rounding to e4m3 (46 rows of 13664, relative error 4.7e-05 instead of
-// 1.1e-05). They cost 16384 x 8192 159 us instead of 155, and 6247 rows of 9984 65 us instead of 61. A division per value
-// took 194 us and left as many (1060 of 134 million values instead of 1176).
 __device__ __forceinline__ float scale_of(float amax) {
     const float s = amax / kE4m3Max;
     return s < kMinNormal ? 1.0f : s;  // (NaN stays NaN)
@@ -215,10 +221,8 @@ __global__ void __launch_bounds__(kNormMaxThreads) norm_forward_kernel(const Fwd
                 scale = scale_of(m);
                 if (col < n && (threadIdx.x & 15) == 0) p.scales[row * p.ldscales + col / 128] = scale;
             }
-            // one reciprocal per block instead of a division per value: within 1.5 ulp of h / scale before
-            // the rounding to four bits
             const float inv = 1.0f / scale;
-            const uint2 q2 = quant8(v[i], inv);
+            const uint2 q2 = quant8(v[i], scale, inv);
             const uint32_t q[2] = {q2.x, q2.y};
             if constexpr (VEC) {
                 if (col < n) *reinterpret_cast<uint2 *>(y + col) = q2;
@@ -430,7 +434,7 @@ __global__ void __launch_bounds__(kRingMaxThreads) norm_forward_ring_kernel(cons
                 const float inv = 1.0f / scale;
                 if (col < n) {
                     if ((threadIdx.x & 15) == 0) p.scales[row * p.ldscales + col / 128] = scale;
-                    *reinterpret_cast<uint2 *>(static_cast<uint8_t *>(p.Y) + row * p.ldy + col) = quant8(v[i], inv);
+                    *reinterpret_cast<uint2 *>(static_cast<uint8_t *>(p.Y) + row * p.ldy + col) = quant8(v[i], scale, inv);
                 }
             }
         }
@@ -558,7 +562,7 @@ __global__ void __launch_bounds__(kRingMaxThreads) norm_forward_odd_kernel(const
                 const float inv = 1.0f / scale;
                 if (col < n) {
                     if ((threadIdx.x & 15) == 0) p.scales[row * p.ldscales + col / 128] = scale;
-                    *reinterpret_cast<uint2 *>(y_out + col) = quant8(v[i], inv);
+                    *reinterpret_cast<uint2 *>(y_out + col) = quant8(v[i], scale, inv);
                 }
             }
         }

@@ -114,6 +114,22 @@ def test_zero_rows_tiny_values_and_block_of_zeros(eng):
     check_e4m3(y, scales, h, size, 128)
 
 
+@pytest.mark.parametrize("T,N", [(3, 256), (4800, 2048), (4800, 2051)])
+def test_e4m3_signs_of_zeros_and_a_block_past_the_largest_float(eng, T, N):
+    """h of column 5 is past fp32's largest: its block's scale is infinite, its finite values are zeros, inf / inf is NaN."""
+    x, _, w = data(T, N, 5, residual=False)
+    x[:, 5], w[5] = 8, 3e38
+    x[:, 130], x[:, 131] = 0.0, -0.0
+    y, scales, _, _ = eng.rms_norm(x, w, out_kind=o.OUT_E4M3)
+    torch.cuda.synchronize()
+    assert torch.isinf(scales[:, 0]).all()
+    assert torch.isnan(y[:, 5].float()).all()
+    assert (y[:, :5].float() == 0).all() and (y[:, 6:128].float() == 0).all()
+    assert (y[:, 130].view(torch.uint8) == 0).all() and (y[:, 131].view(torch.uint8) == 0x80).all()
+    _, _, h, size = formula(x, None, w, 1e-6)
+    check_e4m3(y[:, 128:], scales[:, 1:], h[:, 128:], size[:, 128:], 128)
+
+
 def test_nan_and_infinity_stay_in_their_row_and_block(eng):
     x, r, w = data(6, 1000, 5)
     clean, clean_scales, _, _ = eng.rms_norm(x, w, r, out_kind=o.OUT_E4M3)
