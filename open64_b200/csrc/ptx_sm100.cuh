@@ -252,6 +252,19 @@ __device__ __forceinline__ void mbar_arrive_cluster(uint32_t bar_cluster_addr) {
     asm volatile("mbarrier.arrive.shared::cluster.b64 _, [%0];" ::"r"(bar_cluster_addr) : "memory");
 }
 
+// The arrival that also publishes this thread's ordinary writes (and those ordered before it) to a
+// thread of the partner CTA, which takes them up with mbar_acquire_cluster.
+__device__ __forceinline__ void mbar_arrive_release_cluster(uint32_t bar_cluster_addr) {
+    asm volatile("mbarrier.arrive.release.cluster.shared::cluster.b64 _, [%0];" ::"r"(bar_cluster_addr) : "memory");
+}
+// One probe of a phase known to be complete, with the acquire that belongs to it.
+__device__ __forceinline__ void mbar_acquire_cluster(uint32_t bar, uint32_t parity) {
+    asm volatile(
+        "{\n\t.reg .pred p;\n\t"
+        "mbarrier.test_wait.parity.acquire.cluster.shared::cta.b64 p, [%0], %1;\n\t}" ::"r"(bar), "r"(parity)
+        : "memory");
+}
+
 // The same arrival delivered to the barrier at this shared-memory offset in every CTA of
 // `cta_mask` (one instruction for both CTAs of a pair).
 __device__ __forceinline__ void tc_commit_pair_mask(uint32_t bar, uint16_t cta_mask) {

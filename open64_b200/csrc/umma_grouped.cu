@@ -55,7 +55,7 @@ constexpr int kGpScaleSlots = 3;
 constexpr int kGpScaleFloats = 132;  // this CTA's 128 rows, then the two column blocks
 constexpr int kGpScales = kGpStaging + 8 * kEpiStagingBytesPerWarp;
 constexpr int kGpBars = kGpScales + kGpScaleSlots * kGpScaleFloats * 4;
-constexpr int kGpNumBars = 2 * kGpStages + 10 + 2 * kGpScaleSlots;
+constexpr int kGpNumBars = 3 * kGpStages + 9 + 2 * kGpScaleSlots;
 static_assert(kGpBars % 8 == 0, "barriers");
 constexpr int kGpTmemPtr = kGpBars + 8 * kGpNumBars;
 constexpr int kGpAbort = kGpTmemPtr + 4;
@@ -137,7 +137,8 @@ grouped_pair_kernel(const __grid_constant__ CUtensorMap tm_a, const __grid_const
     const uint32_t tail_bar = bar_base + 8u * (2 * kGpStages + 4);
     auto scale_full_bar = [&](int s) { return bar_base + 8u * (2 * kGpStages + 9 + s); };
     auto scale_empty_bar = [&](int s) { return bar_base + 8u * (2 * kGpStages + 9 + kGpScaleSlots + s); };
-    const uint32_t cleared_bar = bar_base + 8u * (2 * kGpStages + 9 + 2 * kGpScaleSlots);  // first CTA: the second's tail is cleared
+    // first CTA: the second's tail in this stage is cleared
+    auto cleared_bar = [&](int s) { return bar_base + 8u * (2 * kGpStages + 9 + 2 * kGpScaleSlots + s); };
     auto half_bar = [&](int quarter) { return bar_base + 8u * (2 * kGpStages + 5 + quarter); };
     volatile uint32_t *tmem_ptr_smem = reinterpret_cast<volatile uint32_t *>(smem_gen + kGpTmemPtr);
     volatile int *abort_flag = reinterpret_cast<volatile int *>(smem_gen + kGpAbort);
@@ -152,13 +153,13 @@ grouped_pair_kernel(const __grid_constant__ CUtensorMap tm_a, const __grid_const
         for (int s = 0; s < kGpStages; ++s) {
             mbar_init(full_bar(s), 1);  // first CTA: its loader's arrival
             mbar_init(empty_bar(s), 1);
+            mbar_init(cleared_bar(s), 1);
         }
         for (int b = 0; b < 2; ++b) {
             mbar_init(acc_full_bar(b), 1);
             mbar_init(acc_empty_bar(b), 16);  // eight warps in each CTA
         }
         mbar_init(tail_bar, 1);
-        mbar_init(cleared_bar, 1);
         for (int s = 0; s < kGpScaleSlots; ++s) {
             mbar_init(scale_full_bar(s), 1);
             mbar_init(scale_empty_bar(s), 8);
@@ -199,6 +200,7 @@ grouped_pair_kernel(const __grid_constant__ CUtensorMap tm_a, const __grid_const
         const bool leader = elect_one();
         int stage = 0;
         uint32_t phase = 0, tail_phase = 0;
+        [[maybe_unused]] uint32_t cleared_phases = 0;  // first CTA: a bit for each stage's barrier
         bool ok = true;
         TileWalk walk;
         GroupTile t;
@@ -233,7 +235,10 @@ grouped_pair_kernel(const __grid_constant__ CUtensorMap tm_a, const __grid_const
                     } else {
                         // the last block of a group: its loads complete here first, and the rows up to the next whole
                         // K step are cleared in both operands (whatever lies behind the group may be NaN); the
-                        // second CTA says so to the first, whose arrival stands for both
+                        // second CTA says so to the first, whose arrival stands for both.  On a barrier of the
+                        // stage's own: the stage is free again, and the second CTA can speak on it again, only
+                        // after the first has heard it.  (On one barrier for all, the second could be two tails
+                        // ahead, whose parity is that of none.)
                         if (leader) {
                             mbar_arrive_expect_tx(tail_bar, kGpStageBytes);
                             load(map_to_cta(tail_bar, rank));
@@ -250,11 +255,14 @@ grouped_pair_kernel(const __grid_constant__ CUtensorMap tm_a, const __grid_const
                         fence_proxy_async_smem();
                         __syncwarp();
                         if (rank == 1) {
-                            if (leader) mbar_arrive_cluster(map_to_cta(cleared_bar, 0));
+                            if (leader) mbar_arrive_release_cluster(map_to_cta(cleared_bar(stage), 0));
                         } else {
-                            ok = mbar_wait_bounded(cleared_bar, tail_phase, abort_flag, p.status, kWaitGroupTail, p.wait_ns);
+                            const uint32_t cleared_phase = (cleared_phases >> stage) & 1u;
+                            ok = mbar_wait_bounded(cleared_bar(stage), cleared_phase, abort_flag, p.status, kWaitGroupTail, p.wait_ns);
                             ok = __all_sync(0xffffffffu, ok);
                             if (!ok) break;
+                            cleared_phases ^= 1u << stage;
+                            mbar_acquire_cluster(cleared_bar(stage), cleared_phase);
                             if (leader) mbar_arrive(full_bar(stage));
                         }
                         tail_phase ^= 1u;
