@@ -23,8 +23,8 @@
 // K blocks ahead: fetched by each thread for itself two blocks ahead, they cost 600 to 800 cycles a block
 // (32 rows are 32 sectors, and the move from one pipeline register to the next waits for the load).
 //
-// Warp roles (three warpgroups a CTA): 0 loads, 1 issues the MMAs (first CTA of the pair), 2 fetches scales,
-// 4..11 add and store.
+// Warp roles (three warpgroups a CTA): 0 loads, 1 issues the MMAs (first CTA of the pair), 2 fetches scales or, in the
+// weight gradient, clears the cut last blocks, 4..11 add and store.
 // The sums take 128 registers of a thread and two chunks on their way from tensor memory 64 more, so the
 // first warpgroup gives its registers up (setmaxnreg: 128 x 56 + 256 x 224 = the 384 x 168 of the launch).
 //
@@ -36,6 +36,7 @@
 #include <cstdio>
 #include <cstdlib>
 #include <cstring>
+#include <type_traits>
 
 #include "grouped.cuh"
 
@@ -55,11 +56,12 @@ constexpr int kGpScaleSlots = 3;
 constexpr int kGpScaleFloats = 132;  // this CTA's 128 rows, then the two column blocks
 constexpr int kGpScales = kGpStaging + 8 * kEpiStagingBytesPerWarp;
 constexpr int kGpBars = kGpScales + kGpScaleSlots * kGpScaleFloats * 4;
-constexpr int kGpNumBars = 3 * kGpStages + 9 + 2 * kGpScaleSlots;
+constexpr int kGpNumBars = 4 * kGpStages + 8 + 2 * kGpScaleSlots;
 static_assert(kGpBars % 8 == 0, "barriers");
 constexpr int kGpTmemPtr = kGpBars + 8 * kGpNumBars;
 constexpr int kGpAbort = kGpTmemPtr + 4;
-constexpr int kGpTotal = kGpAbort + 4;
+constexpr int kGpLoaded = kGpAbort + 4;  // the tile that this CTA's loader is at
+constexpr int kGpTotal = kGpLoaded + 4;
 constexpr int kGpDynamic = kGpTotal + 1024;
 static_assert(kGpDynamic <= 227 * 1024, "shared memory");
 
@@ -105,6 +107,29 @@ __host__ __device__ constexpr uint32_t grouped_idesc(uint32_t fmt, bool a_mn, bo
     return make_idesc(1u, fmt, fmt, b_mn ? 1u : 0u, kGpTileM, kGpTileN) | ((a_mn ? 1u : 0u) << 15);
 }
 
+// Waits as mbar_wait_bounded does for a phase that may be many tiles away: the budget starts anew whenever *progress
+// has moved.
+__device__ __forceinline__ bool mbar_wait_following(uint32_t bar, uint32_t parity, const volatile uint32_t *progress,
+                                                    volatile int *abort_flag, int *status_word, int code, uint64_t budget_ns) {
+    uint32_t probes = 0, seen = *progress;
+    uint64_t t0 = globaltimer_ns();
+    while (!mbar_try_wait(bar, parity)) {
+        if ((++probes & 255u) != 0) continue;
+        if (*abort_flag) return false;
+        const uint32_t at = *progress;
+        const uint64_t now = globaltimer_ns();
+        if (at != seen) {
+            seen = at;
+            t0 = now;
+        } else if (now - t0 > budget_ns) {
+            atomicCAS(status_word, 0, code);
+            *abort_flag = 1;
+            return false;
+        }
+    }
+    return true;
+}
+
 }  // namespace
 
 // KIND: MMA_F16 (bf16) or MMA_F8F6F4 (e4m3 with block scales).  WGRAD: both operands lie with the sum's
@@ -134,14 +159,20 @@ grouped_pair_kernel(const __grid_constant__ CUtensorMap tm_a, const __grid_const
     auto empty_bar = [&](int s) { return bar_base + 8u * (kGpStages + s); };
     auto acc_full_bar = [&](int b) { return bar_base + 8u * (2 * kGpStages + b); };
     auto acc_empty_bar = [&](int b) { return bar_base + 8u * (2 * kGpStages + 2 + b); };
-    const uint32_t tail_bar = bar_base + 8u * (2 * kGpStages + 4);
-    auto scale_full_bar = [&](int s) { return bar_base + 8u * (2 * kGpStages + 9 + s); };
-    auto scale_empty_bar = [&](int s) { return bar_base + 8u * (2 * kGpStages + 9 + kGpScaleSlots + s); };
-    // first CTA: the second's tail in this stage is cleared
-    auto cleared_bar = [&](int s) { return bar_base + 8u * (2 * kGpStages + 9 + 2 * kGpScaleSlots + s); };
-    auto half_bar = [&](int quarter) { return bar_base + 8u * (2 * kGpStages + 5 + quarter); };
+    auto half_bar = [&](int quarter) { return bar_base + 8u * (2 * kGpStages + 4 + quarter); };
+    auto scale_full_bar = [&](int s) { return bar_base + 8u * (2 * kGpStages + 8 + s); };
+    auto scale_empty_bar = [&](int s) { return bar_base + 8u * (2 * kGpStages + 8 + kGpScaleSlots + s); };
+    // a group's cut last block: this CTA's half has come; first CTA: the second's half is cleared
+    auto tail_bar = [&](int s) { return bar_base + 8u * (2 * kGpStages + 8 + 2 * kGpScaleSlots + s); };
+    auto cleared_bar = [&](int s) { return bar_base + 8u * (3 * kGpStages + 8 + 2 * kGpScaleSlots + s); };
+    // WGRAD: a tile's K blocks that need no clearing (rows up to a whole K step; what lies behind is not multiplied)
+    [[maybe_unused]] auto whole_blocks = [](const GroupTile &t) {
+        return (t.end - t.begin) % kMmaK == 0 ? t.kbs : (t.end - t.begin) / kBlockK;
+    };
     volatile uint32_t *tmem_ptr_smem = reinterpret_cast<volatile uint32_t *>(smem_gen + kGpTmemPtr);
     volatile int *abort_flag = reinterpret_cast<volatile int *>(smem_gen + kGpAbort);
+
+    [[maybe_unused]] volatile uint32_t *loaded = reinterpret_cast<volatile uint32_t *>(smem_gen + kGpLoaded);
 
     const int warp = threadIdx.x >> 5;
     const int lane = threadIdx.x & 31;
@@ -153,19 +184,20 @@ grouped_pair_kernel(const __grid_constant__ CUtensorMap tm_a, const __grid_const
         for (int s = 0; s < kGpStages; ++s) {
             mbar_init(full_bar(s), 1);  // first CTA: its loader's arrival
             mbar_init(empty_bar(s), 1);
+            mbar_init(tail_bar(s), 1);
             mbar_init(cleared_bar(s), 1);
         }
         for (int b = 0; b < 2; ++b) {
             mbar_init(acc_full_bar(b), 1);
             mbar_init(acc_empty_bar(b), 16);  // eight warps in each CTA
         }
-        mbar_init(tail_bar, 1);
         for (int s = 0; s < kGpScaleSlots; ++s) {
             mbar_init(scale_full_bar(s), 1);
             mbar_init(scale_empty_bar(s), 8);
         }
         for (int q = 0; q < 4; ++q) mbar_init(half_bar(q), 2);  // the two warps that share 32 rows
         *abort_flag = 0;
+        *loaded = 0;
         fence_mbar_init();
         tma_prefetch_desc(&tm_a);
         tma_prefetch_desc(&tm_b);
@@ -199,8 +231,7 @@ grouped_pair_kernel(const __grid_constant__ CUtensorMap tm_a, const __grid_const
         // ------------------------------ loads (both CTAs) -----------------------------------
         const bool leader = elect_one();
         int stage = 0;
-        uint32_t phase = 0, tail_phase = 0;
-        [[maybe_unused]] uint32_t cleared_phases = 0;  // first CTA: a bit for each stage's barrier
+        uint32_t phase = 0;
         bool ok = true;
         TileWalk walk;
         GroupTile t;
@@ -211,74 +242,38 @@ grouped_pair_kernel(const __grid_constant__ CUtensorMap tm_a, const __grid_const
             // boxes a stage instead of four: the issuing thread needs about 100 cycles for each)
             [[maybe_unused]] const int xa = p.a_groups ? 0 : m0, za = p.a_groups ? m0 / kKnCols : 0;
             [[maybe_unused]] const int xb = p.b_groups ? 0 : n0 + (int)rank * 128, zb = p.b_groups ? (n0 + (int)rank * 128) / kKnCols : 0;
-            [[maybe_unused]] const int whole = (t.end - t.begin) % kMmaK == 0 ? t.kbs : (t.end - t.begin) / kBlockK;
-            for (int kb = 0; kb < t.kbs; ++kb) {
+            auto load_block = [&](int kb, auto cut) __attribute__((always_inline)) {
                 ok = mbar_wait_bounded(empty_bar(stage), phase ^ 1u, abort_flag, p.status, kWaitGroupProducer, p.wait_ns);
                 ok = __all_sync(0xffffffffu, ok);
-                if (!ok) break;
+                if (!ok) return;
                 const uint32_t a_dst = smem_base + stage * kGpStageBytes;
                 const uint32_t b_dst = a_dst + kABytes;
-                const uint32_t full0 = map_to_cta(full_bar(stage), 0);
-                if constexpr (WGRAD) {
-                    const int row = t.begin + kb * kBlockK;
-                    auto load = [&](uint32_t bar) __attribute__((always_inline)) {
+                if (leader) {
+                    uint32_t bar;
+                    if constexpr (decltype(cut)::value) {  // the clearing warps pass it on
+                        mbar_arrive_expect_tx(tail_bar(stage), kGpStageBytes);
+                        bar = map_to_cta(tail_bar(stage), rank);
+                    } else {
+                        if (rank == 0) mbar_arrive_expect_tx(full_bar(stage), 2 * kGpStageBytes);
+                        bar = map_to_cta(full_bar(stage), 0);
+                    }
+                    if constexpr (WGRAD) {
+                        const int row = t.begin + kb * kBlockK;
                         tma_load_3d_pair(a_dst, &tm_a, xa, row, za, bar);
                         tma_load_3d_pair(b_dst, &tm_b, xb, row, zb, bar);
                         if (!p.a_groups) tma_load_3d_pair(a_dst + kKnGroupBytes, &tm_a, xa + kKnCols, row, 0, bar);
                         if (!p.b_groups) tma_load_3d_pair(b_dst + kKnGroupBytes, &tm_b, xb + kKnCols, row, 0, bar);
-                    };
-                    if (kb < whole) {
-                        if (leader) {
-                            if (rank == 0) mbar_arrive_expect_tx(full_bar(stage), 2 * kGpStageBytes);
-                            load(full0);
-                        }
                     } else {
-                        // the last block of a group: its loads complete here first, and the rows up to the next whole
-                        // K step are cleared in both operands (whatever lies behind the group may be NaN); the
-                        // second CTA says so to the first, whose arrival stands for both.  On a barrier of the
-                        // stage's own: the stage is free again, and the second CTA can speak on it again, only
-                        // after the first has heard it.  (On one barrier for all, the second could be two tails
-                        // ahead, whose parity is that of none.)
-                        if (leader) {
-                            mbar_arrive_expect_tx(tail_bar, kGpStageBytes);
-                            load(map_to_cta(tail_bar, rank));
-                        }
-                        __syncwarp();
-                        ok = mbar_wait_bounded(tail_bar, tail_phase, abort_flag, p.status, kWaitGroupTail, p.wait_ns);
-                        ok = __all_sync(0xffffffffu, ok);
-                        if (!ok) break;
-                        const int first = t.end - row, last = (first + kMmaK - 1) / kMmaK * kMmaK;
-                        uint8_t *at = smem_gen + stage * kGpStageBytes;
-                        for (int c = 0; c < 2 * kKnGroups; ++c)
-                            for (int q = first * 8 + lane; q < last * 8; q += 32)
-                                reinterpret_cast<uint4 *>(at + c * kKnGroupBytes)[q] = make_uint4(0, 0, 0, 0);
-                        fence_proxy_async_smem();
-                        __syncwarp();
-                        if (rank == 1) {
-                            if (leader) mbar_arrive_release_cluster(map_to_cta(cleared_bar(stage), 0));
-                        } else {
-                            const uint32_t cleared_phase = (cleared_phases >> stage) & 1u;
-                            ok = mbar_wait_bounded(cleared_bar(stage), cleared_phase, abort_flag, p.status, kWaitGroupTail, p.wait_ns);
-                            ok = __all_sync(0xffffffffu, ok);
-                            if (!ok) break;
-                            cleared_phases ^= 1u << stage;
-                            mbar_acquire_cluster(cleared_bar(stage), cleared_phase);
-                            if (leader) mbar_arrive(full_bar(stage));
-                        }
-                        tail_phase ^= 1u;
-                    }
-                } else if (leader) {
-                    if (rank == 0) mbar_arrive_expect_tx(full_bar(stage), 2 * kGpStageBytes);
-                    tma_load_2d_pair(a_dst, &tm_a, kb * kBlockK, t.begin + m0, full0);
-                    if constexpr (B_KN) {
+                        tma_load_2d_pair(a_dst, &tm_a, kb * kBlockK, t.begin + m0, bar);
+                        if constexpr (B_KN) {
 #pragma unroll
-                        for (int c = 0; c < kKnGroups; ++c)
-                            tma_load_3d_pair(b_dst + c * kKnGroupBytes, &tm_b, n0 + (int)rank * 128 + c * kKnCols, kb * kBlockK,
-                                             t.g, full0);
-                    } else {
-                        // SwiGLU: the first CTA holds gate rows, the second the matching up rows
-                        const int y = kSwiglu ? n0 + (rank ? p.N : 0) : n0 + (int)rank * 128;
-                        tma_load_3d_pair(b_dst, &tm_b, kb * kBlockK, y, t.g, full0);
+                            for (int c = 0; c < kKnGroups; ++c)
+                                tma_load_3d_pair(b_dst + c * kKnGroupBytes, &tm_b, n0 + (int)rank * 128 + c * kKnCols, kb * kBlockK, t.g, bar);
+                        } else {
+                            // SwiGLU: the first CTA holds gate rows, the second the matching up rows
+                            const int y = kSwiglu ? n0 + (rank ? p.N : 0) : n0 + (int)rank * 128;
+                            tma_load_3d_pair(b_dst, &tm_b, kb * kBlockK, y, t.g, bar);
+                        }
                     }
                 }
                 __syncwarp();
@@ -286,6 +281,14 @@ grouped_pair_kernel(const __grid_constant__ CUtensorMap tm_a, const __grid_const
                     stage = 0;
                     phase ^= 1u;
                 }
+            };
+            if constexpr (WGRAD) {
+                if (leader) *loaded = (uint32_t)i + 1;
+                const int whole = whole_blocks(t);
+                for (int kb = 0; ok && kb < whole; ++kb) load_block(kb, std::false_type());
+                if (ok && whole < t.kbs) load_block(whole, std::true_type());
+            } else {
+                for (int kb = 0; ok && kb < t.kbs; ++kb) load_block(kb, std::false_type());
             }
         }
         __syncwarp();
@@ -362,6 +365,48 @@ grouped_pair_kernel(const __grid_constant__ CUtensorMap tm_a, const __grid_const
                     ++uses;
                 }
             }
+        }
+        __syncwarp();
+    } else if (WGRAD && warp == 2) {
+        // ------------------------------ cut last blocks (both CTAs) --------------------------
+        // The rows from a group's end to the next whole K step are cleared in both operands (whatever lies behind the
+        // group may be NaN).  The second CTA says so to the first, whose arrival on the stage's full barrier stands for
+        // both.  Every barrier of this way is the stage's own: nobody speaks on one again before the stage is free
+        // again, so before it has been heard.  (On one barrier for all stages the second CTA could be two tails ahead,
+        // whose parity is that of none.)  A warp of its own, since the loading warp stands still meanwhile and longer for
+        // the arrival that publishes plain writes to the other CTA: 8192 rows, 8 experts of 4096 x 14336, 900-1000 us with
+        // the clearing there, 850-875 us here.
+        uint32_t phases = 0;  // a bit for each stage
+        int done = 0;         // blocks before this tile, modulo the ring
+        bool ok = true;
+        TileWalk walk;
+        GroupTile t;
+        for (int i = pair_id; ok && next_tile<WGRAD>(p, walk, i, kBlockK, t); i += num_pairs) {
+            const int stage = (done + t.kbs - 1 + kGpStages) % kGpStages;
+            done = (done + t.kbs) % kGpStages;
+            if (whole_blocks(t) == t.kbs) continue;
+            const uint32_t phase = (phases >> stage) & 1u;
+            phases ^= 1u << stage;
+            ok = mbar_wait_following(tail_bar(stage), phase, loaded, abort_flag, p.status, kWaitGroupTail, p.wait_ns);
+            ok = __all_sync(0xffffffffu, ok);
+            if (!ok) break;
+            const int first = (t.end - t.begin) % kBlockK, last = (first + kMmaK - 1) / kMmaK * kMmaK;
+            uint8_t *at = smem_gen + stage * kGpStageBytes;
+            for (int c = 0; c < 2 * kKnGroups; ++c)
+                for (int q = first * 8 + lane; q < last * 8; q += 32)
+                    reinterpret_cast<uint4 *>(at + c * kKnGroupBytes)[q] = make_uint4(0, 0, 0, 0);
+            fence_proxy_async_smem();
+            __syncwarp();
+            if (rank == 1) {
+                if (lane == 0) mbar_arrive_release_cluster(map_to_cta(cleared_bar(stage), 0));
+            } else {
+                ok = mbar_wait_bounded(cleared_bar(stage), phase, abort_flag, p.status, kWaitGroupTail, p.wait_ns);
+                ok = __all_sync(0xffffffffu, ok);
+                if (!ok) break;
+                mbar_acquire_cluster(cleared_bar(stage), phase);
+                if (lane == 0) mbar_arrive(full_bar(stage));
+            }
+            __syncwarp();
         }
         __syncwarp();
     } else if (kScaled && warp == 2) {
