@@ -122,11 +122,12 @@ def _tma(t):
         return t
     if 0 in t.shape:
         return t
+    t = t.detach()
     *lead, cols = t.shape
     ld = cols + -cols % (16 // e)
     strides = (ld, 1) if t.dim() == 2 else (lead[1] * ld, ld, 1)
     # in the widest words that the rows are made of (byte by byte a 17 MB weight took 25 us)
-    bits = 8 | cols * e | t.data_ptr()
+    bits = 8 | cols * e | t.data_ptr() | t.storage_offset() * e
     for n, stride in zip(lead, t.stride()):
         if n > 1:
             bits |= stride * e
@@ -134,6 +135,8 @@ def _tma(t):
     if width <= e:
         return torch.empty_strided(t.shape, strides, dtype=t.dtype, device=t.device).copy_(t)
     n = width // e
+    # (an extent of one has no stride, but the view as words wants one that words divide)
+    t = t.as_strided(t.shape, [s if m > 1 else ld for m, s in zip(lead, t.stride())] + [1])
     words = torch.empty_strided((*lead, cols // n), (*(s // n for s in strides[:-1]), 1), dtype=_WORDS[width], device=t.device)
     return words.copy_(t.view(_WORDS[width])).view(t.dtype)
 
