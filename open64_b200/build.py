@@ -22,7 +22,7 @@ WHIRL_SRC = os.path.join(HERE, "whirl", "o64whirl.cpp")
 WHIRL_OUT = os.path.join(HERE, "whirl", "o64whirl")
 
 SOURCES = ["api.cu", "umma_gemm.cu", "umma_gemm_2cta.cu", "umma_gemm_wide.cu", "umma_gemm_skinny.cu", "umma_grouped.cu", "umma_grouped_rows.cu", "norm.cu", "simt_kernels.cu", "simt_generic.cu", "plan.cpp", "no_alloc.cu", "dotprod.cu"]
-HEADERS = ["ptx_sm100.cuh", "umma_gemm.cuh", "umma_common.cuh", "grouped.cuh", "norm.cuh", "simt_kernels.cuh", "../../include/o64gemm.h"]
+HEADERS = ["ptx_sm100.cuh", "umma_gemm.cuh", "umma_common.cuh", "grouped.cuh", "e4m3.cuh", "norm.cuh", "simt_kernels.cuh", "../../include/o64gemm.h"]
 
 NVCC_FLAGS = [
     "-gencode", "arch=compute_100a,code=sm_100a", "-lineinfo", "-O3", "-std=c++17",

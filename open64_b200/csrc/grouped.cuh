@@ -4,6 +4,7 @@
 #pragma once
 #include <cuda.h>
 
+#include "e4m3.cuh"
 #include "umma_common.cuh"
 
 namespace o64 {
@@ -111,16 +112,5 @@ __device__ __forceinline__ void tma_store_3d(const void *tmap, uint32_t smem_src
 // silu(g) * u.  exp and the division are the fast ones: together within 2^-20 of the value for |g| < 20, and
 // where exp(-g) passes 2^126 the result, below 1e-35 of u, is zero.
 __device__ __forceinline__ float silu_mul(float g, float u) { return __fdividef(g, 1.0f + __expf(-g)) * u; }
-
-// amax / 448, or 1 where that is no normal number (NaN stays NaN).
-__device__ __forceinline__ float block_scale_of(float amax) {
-    const float s = amax / 448.0f;
-    return s < 1.17549435e-38f ? 1.0f : s;
-}
-__device__ __forceinline__ float fmax_nan(float a, float b) {
-    float r;
-    asm("max.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(a), "f"(b));
-    return r;
-}
 
 }  // namespace o64

@@ -18,11 +18,10 @@
 // the same one),   dw[j] = sum over rows of dy n.  The sum over rows runs in two fixed stages (a
 // partial row per thread group, then one addition per column), so that it does not depend on timing.
 #include <cuda_bf16.h>
-#include <cuda_fp8.h>
 
 #include <algorithm>
-#include <cfloat>
 
+#include "e4m3.cuh"
 #include "norm.cuh"
 #include "ptx_sm100.cuh"
 #include "umma_common.cuh"
@@ -33,14 +32,6 @@ namespace {
 
 constexpr int kNormMaxThreads = 512;
 constexpr int kRingCols = 256;  // narrower rows run on the block-per-row kernel
-constexpr float kE4m3Max = 448.0f;
-constexpr float kMinNormal = 1.17549435e-38f;
-
-__device__ __forceinline__ float max_nan(float a, float b) {  // NaN wins, as in a maximum of the definition
-    float r;
-    asm("max.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(a), "f"(b));
-    return r;
-}
 
 // Eight consecutive bf16 values of a row; columns >= n read as zero.
 template <bool VEC>
@@ -115,22 +106,12 @@ __device__ __forceinline__ float row_reduce(float v, float *slot) {
     return r;
 }
 
-// Eight values over the scale of their block, inv = 1 / scale, to e4m3. One division per block: the product with inv is
-// off by up to 1.5 ulp, which puts some values on the other side of a rounding to four bits, so a step with the
-// product's own remainder follows, q - (q scale - v) inv, in two packed multiply-adds. 16384 x 8192: 1060 of 134
-// million values are other than from 64 bits, 1176 without the step, as many as with it from a division per value,
-// which takes 194 us instead of 157. (With q scale - v and not v - q scale a zero keeps its sign.) Under an infinite scale
-// inv is 0 and nothing is to be put right: the remainder would be 0 * inf.
+// Eight values over the scale of their block, inv = 1 / scale, to e4m3.
 __device__ __forceinline__ uint2 quant8(const float (&v)[8], float scale, float inv) {
-    const float back = scale <= FLT_MAX ? scale : 0.0f;
+    const float back = remainder_scale(scale);
     uint32_t q[2] = {0, 0};
 #pragma unroll
-    for (int e = 0; e < 4; ++e) {
-        float2 two = make_float2(v[2 * e] * inv, v[2 * e + 1] * inv);
-        const float2 rest = __ffma2_rn(two, make_float2(back, back), make_float2(-v[2 * e], -v[2 * e + 1]));
-        two = __ffma2_rn(rest, make_float2(-inv, -inv), two);
-        q[e >> 1] |= (uint32_t)__nv_cvt_float2_to_fp8x2(two, __NV_SATFINITE, __NV_E4M3) << (16 * (e & 1));
-    }
+    for (int e = 0; e < 4; ++e) q[e >> 1] |= quant2(make_float2(v[2 * e], v[2 * e + 1]), back, inv) << (16 * (e & 1));
     return make_uint2(q[0], q[1]);
 }
 
@@ -146,11 +127,6 @@ struct FwdParams {
     float eps;
     int w_f32, row_scale;
 };
-
-__device__ __forceinline__ float scale_of(float amax) {
-    const float s = amax / kE4m3Max;
-    return s < kMinNormal ? 1.0f : s;  // (NaN stays NaN)
-}
 
 // Columns of thread t: (i * blockDim.x + t) * 8 .. + 7 for i < NV, so that 16 neighbouring threads hold
 // one scale block of 128.
@@ -204,7 +180,7 @@ __global__ void __launch_bounds__(kNormMaxThreads) norm_forward_kernel(const Fwd
     } else {
         float scale = 1.0f;
         if (p.row_scale) {
-            scale = scale_of(row_reduce<true>(top, slots[1]));
+            scale = block_scale_of(row_reduce<true>(top, slots[1]));
             if (live && threadIdx.x == 0) p.scales[row * p.ldscales] = scale;
         }
         uint8_t *y = static_cast<uint8_t *>(p.Y) + (live ? row * p.ldy : 0);
@@ -218,7 +194,7 @@ __global__ void __launch_bounds__(kNormMaxThreads) norm_forward_kernel(const Fwd
                     if (col + e < n) m = max_nan(m, fabsf(v[i][e]));
 #pragma unroll
                 for (int o = 8; o > 0; o >>= 1) m = max_nan(m, __shfl_xor_sync(0xffffffffu, m, o));
-                scale = scale_of(m);
+                scale = block_scale_of(m);
                 if (col < n && (threadIdx.x & 15) == 0) p.scales[row * p.ldscales + col / 128] = scale;
             }
             const float inv = 1.0f / scale;
@@ -430,7 +406,7 @@ __global__ void __launch_bounds__(kRingMaxThreads) norm_forward_ring_kernel(cons
                 }
 #pragma unroll
                 for (int o = 8; o > 0; o >>= 1) m = max_nan(m, __shfl_xor_sync(0xffffffffu, m, o));
-                const float scale = scale_of(m);
+                const float scale = block_scale_of(m);
                 const float inv = 1.0f / scale;
                 if (col < n) {
                     if ((threadIdx.x & 15) == 0) p.scales[row * p.ldscales + col / 128] = scale;
@@ -558,7 +534,7 @@ __global__ void __launch_bounds__(kRingMaxThreads) norm_forward_odd_kernel(const
             } else {
 #pragma unroll
                 for (int o = 8; o > 0; o >>= 1) m = max_nan(m, __shfl_xor_sync(0xffffffffu, m, o));
-                const float scale = scale_of(m);
+                const float scale = block_scale_of(m);
                 const float inv = 1.0f / scale;
                 if (col < n) {
                     if ((threadIdx.x & 15) == 0) p.scales[row * p.ldscales + col / 128] = scale;

@@ -647,28 +647,25 @@ grouped_pair_kernel(const __grid_constant__ CUtensorMap tm_a, const __grid_const
                     float2 &h = acc[0][j];
                     h.x = silu_mul(h.x, acc[1][j].x);
                     h.y = silu_mul(h.y, acc[1][j].y);
-                    amax = fmax_nan(amax, fmax_nan(fabsf(h.x), fabsf(h.y)));
+                    amax = max_nan(amax, max_nan(fabsf(h.x), fabsf(h.y)));
                 }
                 // the row's other 64 columns are with the warp of the other half
                 patch_free();
                 reinterpret_cast<float *>(patch)[lane] = amax;
                 meet();
                 if (!ok) break;
-                amax = fmax_nan(amax, reinterpret_cast<const float *>(smem_gen + kGpStaging + ((half ^ 1) * 4 + (warp & 3)) * kEpiStagingBytesPerWarp)[lane]);
+                amax = max_nan(amax, reinterpret_cast<const float *>(smem_gen + kGpStaging + ((half ^ 1) * 4 + (warp & 3)) * kEpiStagingBytesPerWarp)[lane]);
                 meet();  // read before the values overwrite it
                 if (!ok) break;
                 const float scale = block_scale_of(amax);
                 if (half == 0 && lane < rows_here) p.scale_c[(grow0 + lane) * p.ldsc + t.nb] = scale;
-                const float inv = 1.0f / scale;
+                const float inv = 1.0f / scale, back = remainder_scale(scale);
 #pragma unroll
                 for (int q = 0; q < 4; ++q) {
                     uint32_t w[4];
 #pragma unroll
-                    for (int e = 0; e < 4; ++e) {
-                        const float2 a = acc[0][q * 8 + e * 2], b = acc[0][q * 8 + e * 2 + 1];
-                        w[e] = (uint32_t)__nv_cvt_float2_to_fp8x2(make_float2(a.x * inv, a.y * inv), __NV_SATFINITE, __NV_E4M3) |
-                               ((uint32_t)__nv_cvt_float2_to_fp8x2(make_float2(b.x * inv, b.y * inv), __NV_SATFINITE, __NV_E4M3) << 16);
-                    }
+                    for (int e = 0; e < 4; ++e)
+                        w[e] = quant2(acc[0][q * 8 + e * 2], back, inv) | quant2(acc[0][q * 8 + e * 2 + 1], back, inv) << 16;
                     patch[lane * 8 + (q ^ sw)] = make_uint4(w[0], w[1], w[2], w[3]);
                 }
                 if (rows_here > 0) send(n0 + half * 64, 64);

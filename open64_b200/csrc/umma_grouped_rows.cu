@@ -93,23 +93,24 @@ __device__ __forceinline__ void store_e4m3_rows(const uint32_t *amax, const floa
                                                 long long ld_scales, bool write_scales) {
     const int lane = threadIdx.x & 31;
     constexpr int kPer = (ROWS + 31) / 32;
-    float inv[kPer];
+    float inv[kPer], back[kPer];
 #pragma unroll
     for (int i = 0; i < kPer; ++i) {
         const int j = i * 32 + lane;
-        inv[i] = 1.0f;
+        inv[i] = back[i] = 1.0f;
         if (j < rows) {
             const uint32_t m = max(max(amax[j], amax[TOK + j]), max(amax[2 * TOK + j], amax[3 * TOK + j]));
             const float scale = block_scale_of(__uint_as_float(m));
             if (write_scales) scales[j * ld_scales] = scale;
             inv[i] = 1.0f / scale;
+            back[i] = remainder_scale(scale);
         }
     }
 #pragma unroll
     for (int j = 0; j < ROWS; ++j) {
         if (j >= rows) break;
-        const float f = __shfl_sync(0xffffffffu, inv[j / 32], j % 32);
-        dst[j * ld] = (uint8_t)__nv_cvt_float_to_fp8(h[j] * f, __NV_SATFINITE, __NV_E4M3);
+        const float f = __shfl_sync(0xffffffffu, inv[j / 32], j % 32), b = __shfl_sync(0xffffffffu, back[j / 32], j % 32);
+        dst[j * ld] = (uint8_t)__nv_cvt_float_to_fp8(quotient(h[j], b, f), __NV_SATFINITE, __NV_E4M3);
     }
 }
 
