@@ -109,8 +109,28 @@ __device__ __forceinline__ void tma_store_3d(const void *tmap, uint32_t smem_src
                  : "memory");
 }
 
-// silu(g) * u.  exp and the division are the fast ones: together within 2^-20 of the value for |g| < 20, and
-// where exp(-g) passes 2^126 the result, below 1e-35 of u, is zero.
-__device__ __forceinline__ float silu_mul(float g, float u) { return __fdividef(g, 1.0f + __expf(-g)) * u; }
+__device__ __forceinline__ float ex2_approx(float x) {  // 2 ulp; below 2^-126 zero
+    float r;
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(x));
+    return r;
+}
+__device__ __forceinline__ float rcp_approx(float x) {  // 1 ulp; below 2^-126 zero
+    float r;
+    asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(x));
+    return r;
+}
+
+// silu(g) * u = g / (1 + exp(-g)) * u, within 2^-20 of the value.  exp(x) = 2^hi * (1 + lo ln 2) with x log2(e) = hi + lo in two
+// floats: in one, its rounding alone is 2^-20 of the result at g = -20 and four times that at -80.  The power is within
+// 2^-22, the reciprocal 2^-23, five roundings 2^-24 each.  x stays between -87, where exp(x) is nothing beside 1, and 88, where
+// the reciprocal is zero (g -> -inf: the result is below 1e-35 of u), so that neither hi nor 2^hi is infinite.
+__device__ __forceinline__ float silu_mul(float g, float u) {
+    constexpr float kLog2e = 1.44269502f, kLog2eRest = 1.92596299e-8f, kLn2 = 0.693147181f;
+    const float x = fminf(fmaxf(-g, -87.0f), 88.0f);
+    const float hi = x * kLog2e;
+    const float lo = fmaf(x, kLog2eRest, fmaf(x, kLog2e, -hi));
+    const float p = ex2_approx(hi);
+    return g * rcp_approx(1.0f + fmaf(p, lo * kLn2, p)) * u;
+}
 
 }  // namespace o64

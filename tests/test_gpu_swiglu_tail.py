@@ -46,3 +46,45 @@ def test_values_on_the_border_of_two_e4m3_numbers(eng, M, N, K, groups):
     want = torch.cat([up, torch.tensor([448.0], device="cuda")]).double().to(FP8)
     assert torch.equal(scales[known], (64 * t * t)[known, None].expand(-1, N // 128))
     assert torch.equal(h[known].float(), want.float().repeat(N // 128).expand(int(known.sum()), N))
+
+
+@pytest.mark.parametrize("M", ROWS + [20000])
+@pytest.mark.parametrize("low,high", [(-20, 20), (-1, 1), (-60, -20)])
+def test_silu(eng, M, low, high):
+    """The scale of a block of equal values shows silu(gate) to all its bits: within 2^-20 of the value, and the
+    roundings of the product with up and of the division by 448."""
+    g = torch.Generator(device="cuda").manual_seed(M)
+    x = low + (high - low) * torch.rand(M, generator=g, device="cuda")
+    a = torch.zeros((M, 128), device="cuda")
+    a[:, 0] = torch.sign(x)
+    w = torch.zeros((256, 128), device="cuda")
+    w[:, 0] = 1.0
+    sa = x.abs()[:, None].contiguous()
+    _, scales = call(eng, a.to(FP8), sa, w.to(FP8), torch.ones((2, 1), device="cuda"), 0)
+    v = x.double()
+    want = v * torch.sigmoid(v) * v / 448  # the second factor: up is the same number
+    off = (scales[:, 0].double() / want.abs() - 1).abs()
+    assert (off <= 2.0 ** -20 + 2 * 2.0 ** -24)[want.abs() >= 2.0 ** -126].all(), off.max().log2().item()
+
+
+@pytest.mark.parametrize("M", [4, 300, 1200])
+def test_silu_far_out(eng, M):
+    """Gates of any size: as they are above, zero below, infinite and NaN where the formula is."""
+    inf, nan = float("inf"), float("nan")
+    gates = torch.tensor([1e30, -1e30, 3e38, -3e38, 200.0, -200.0, -89.0, 1e-30, -1e-30, inf, -inf, nan], device="cuda")
+    gates = gates.repeat(-(-M // 12))[:M]
+    a = torch.zeros((M, 128), device="cuda")
+    a[:, 0] = torch.where(gates < 0, -1.0, 1.0)
+    w = torch.zeros((256, 128), device="cuda")
+    w[:, 0] = 1.0
+    _, scales = call(eng, a.to(FP8), gates.abs()[:, None].contiguous(), w.to(FP8), torch.tensor([[1.0], [2.0 ** -40]], device="cuda"), 0)
+    v = gates.double()
+    h = v * torch.sigmoid(v) * (v * 2.0 ** -40)
+    got = scales[:, 0].double()
+    assert torch.equal(torch.isnan(got), torch.isnan(h))
+    big = h.abs() > 3.5e38
+    assert torch.isinf(got[big]).all()
+    small = h.abs() / 448 < 2.0 ** -126  # a block of nothing: its scale is 1
+    assert (got[small] == 1).all()
+    rest = ~(big | small | torch.isnan(h))
+    assert ((got / (h.abs() / 448) - 1).abs()[rest] <= 2.0 ** -20 + 2 * 2.0 ** -24).all()
