@@ -67,15 +67,17 @@ struct GroupedParams {
     unsigned long long wait_ns;
 };
 
-// A group's rows, kept inside [0, T) whatever the offsets say; *bad: they are not ascending within 0 .. T.
-__device__ __forceinline__ void group_rows(const GroupedParams &p, int g, int &begin, int &end, bool *bad = nullptr) {
+// A group's rows, kept inside [top, T) whatever the offsets say; *bad: they are not ascending within 0 .. T.  A walk
+// over the groups passes the end of those before: offsets that overlap then make no more tiles than others, which is
+// what the grids and the one tile of a cluster that divides K are sized for.
+__device__ __forceinline__ void group_rows(const GroupedParams &p, int g, int top, int &begin, int &end, bool *bad = nullptr) {
     if (!p.offsets) {
         begin = 0;
         end = p.T;
         return;
     }
     const int a = __ldg(p.offsets + g), b = __ldg(p.offsets + g + 1);
-    begin = min(max(a, 0), p.T);
+    begin = min(max(a, top), p.T);
     end = min(max(b, begin), p.T);
     if (bad) *bad = a < 0 || b < a || b > p.T;
 }

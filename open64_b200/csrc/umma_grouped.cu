@@ -75,16 +75,16 @@ struct GroupTile {
 struct TileWalk {
     int g = 0;
     int base = 0;  // tiles before group g
+    int top = 0;   // the end of the groups before it
 };
 
 template <bool WGRAD>
 __device__ __forceinline__ bool next_tile(const GroupedParams &p, TileWalk &w, int t, int block_k, GroupTile &tile) {
     for (; w.g < p.G; ++w.g) {
-        group_rows(p, w.g, tile.begin, tile.end);
+        group_rows(p, w.g, w.top, tile.begin, tile.end);
         const int rows = tile.end - tile.begin;
         const int mt = WGRAD ? p.num_m_tiles : (rows + kGpTileM - 1) / kGpTileM;
-        // (the host has checked that all of them fit an int; groups that overlap, from bad offsets, may not)
-        const int tiles = (int)min((long long)mt * p.num_n_tiles, (long long)(INT32_MAX - w.base));
+        const int tiles = mt * p.num_n_tiles;  // (the host has checked that all of them together fit an int)
         if (t < w.base + tiles) {
             // bands of eight row tiles, rows fastest: a band's rows of A and one column block of B stay in L2
             const int r = t - w.base;
@@ -98,6 +98,7 @@ __device__ __forceinline__ bool next_tile(const GroupedParams &p, TileWalk &w, i
             return true;
         }
         w.base += tiles;
+        w.top = tile.end;
     }
     return false;
 }
@@ -211,7 +212,7 @@ grouped_pair_kernel(const __grid_constant__ CUtensorMap tm_a, const __grid_const
         for (int g = lane; g < p.G; g += 32) {
             int b, e;
             bool bad;
-            group_rows(p, g, b, e, &bad);
+            group_rows(p, g, 0, b, e, &bad);
             if (bad) atomicCAS(p.status, 0, kBadOffsets);
         }
     }
@@ -720,7 +721,7 @@ grouped_pair_kernel(const __grid_constant__ CUtensorMap tm_a, const __grid_const
 __global__ void grouped_zero_kernel(const GroupedParams p, int elem, int wgrad) {
     for (int g = blockIdx.y; g < p.G; g += gridDim.y) {
         int b = 0, e = p.rows_m;
-        if (!wgrad) group_rows(p, g, b, e);
+        if (!wgrad) group_rows(p, g, 0, b, e);
         uint8_t *c = static_cast<uint8_t *>(p.C) + (wgrad ? (long long)g * p.stride_c * elem : 0);
         for (long long r = b + blockIdx.x; r < e; r += gridDim.x) {
             for (long long i = threadIdx.x; i < (long long)p.N * elem; i += blockDim.x) c[r * p.ldc * elem + i] = 0;

@@ -64,15 +64,16 @@ struct RowsTile {
 struct RowsWalk {
     int g = 0;
     int base = 0;
+    int top = 0;  // the end of the groups before g
 };
 
 template <int TOK>
 __device__ __forceinline__ bool next_rows_tile(const GroupedParams &p, RowsWalk &w, int t, RowsTile &tile) {
     for (; w.g < p.G; ++w.g) {
         int begin, end;
-        group_rows(p, w.g, begin, end);
+        group_rows(p, w.g, w.top, begin, end);
         const int tt = (end - begin + TOK - 1) / TOK;
-        const int tiles = (int)min((long long)tt * p.num_n_tiles, (long long)(INT32_MAX - w.base));
+        const int tiles = tt * p.num_n_tiles;
         if (t < w.base + tiles) {
             const int r = t - w.base;
             tile.g = w.g;
@@ -82,6 +83,7 @@ __device__ __forceinline__ bool next_rows_tile(const GroupedParams &p, RowsWalk 
             return true;
         }
         w.base += tiles;
+        w.top = end;
     }
     return false;
 }
@@ -202,7 +204,7 @@ grouped_rows_kernel(const __grid_constant__ CUtensorMap tm_x, const __grid_const
         for (int g = lane; g < p.G; g += 32) {
             int b, e;
             bool bad;
-            group_rows(p, g, b, e, &bad);
+            group_rows(p, g, 0, b, e, &bad);
             if (bad) atomicCAS(p.status, 0, kBadOffsets);
         }
     }
