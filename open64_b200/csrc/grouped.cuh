@@ -76,7 +76,7 @@ __device__ __forceinline__ void group_rows(const GroupedParams &p, int g, int to
         end = p.T;
         return;
     }
-    const int a = __ldg(p.offsets + g), b = __ldg(p.offsets + g + 1);
+    const int a = p.offsets[g], b = p.offsets[g + 1];
     begin = min(max(a, top), p.T);
     end = min(max(b, begin), p.T);
     if (bad) *bad = a < 0 || b < a || b > p.T;

@@ -16,7 +16,9 @@
 // are launch, first data and the exchange.
 //
 // Warps: 0 loads, 1 issues the MMAs, 2 fetches scales, 4.. add (four for each weight block).  Launched so that
-// its set-up overlaps the previous kernel of the stream (it waits before it touches memory).
+// its set-up overlaps the previous kernel of the stream (it waits before it touches memory).  That kernel may write what
+// is read here while this one already exists, so scales and offsets come by ordinary loads: the read-only path is for
+// memory that nobody writes during a kernel's life.
 #include <cstdio>
 #include <cstdlib>
 #include <cstring>
@@ -330,9 +332,9 @@ grouped_rows_kernel(const __grid_constant__ CUtensorMap tm_x, const __grid_const
             for (int u = 0; u < 4; ++u) {
                 const bool in = kb0 + u < kb_end;
 #pragma unroll
-                for (int r = 0; r < kPer; ++r) next[r][u] = in ? __ldg(sa[r] + kb0 + u) : 0.0f;
-                b0[u] = in ? __ldg(sb0 + (kb0 + u) * sb_step) : 0.0f;
-                b1[u] = kSwiglu && in ? __ldg(sb1 + kb0 + u) : 0.0f;
+                for (int r = 0; r < kPer; ++r) next[r][u] = in ? sa[r][kb0 + u] : 0.0f;
+                b0[u] = in ? sb0[(kb0 + u) * sb_step] : 0.0f;
+                b1[u] = kSwiglu && in ? sb1[kb0 + u] : 0.0f;
             }
         };
         auto begin_tile = [&]() __attribute__((always_inline)) {
