@@ -106,12 +106,48 @@ __device__ __forceinline__ float row_reduce(float v, float *slot) {
     return r;
 }
 
-// Eight values over the scale of their block, inv = 1 / scale, to e4m3.
-__device__ __forceinline__ uint2 quant8(const float (&v)[8], float scale, float inv) {
-    const float back = remainder_scale(scale);
+// h = s * rstd * w as s * pre * w * post: where h becomes e4m3, pre is 7/8 of the power of two below rstd and post (in two
+// floats) the rest.  A block's quotients h / (max |h| / 448) are those of u = s * pre * w, which has a rounding less than h,
+// and with its factor of 7 max |u| / 448 is a division by 64: with a bf16 w both are exact as long as s has 13 bits.
+// 16384 x 8192 with the residual: 6 of 134 million values are other than from 64 bits, 866 from h.
+// (|u| < |h|, so u is finite where h is.  rstd zero, infinite or NaN: u is as the product with rstd.)
+template <bool E4M3>
+struct RowFactors {
+    float pre, post, post_rest;
+    __device__ __forceinline__ explicit RowFactors(float rstd) : pre(rstd), post(1.0f), post_rest(0.0f) {
+        if constexpr (E4M3) {
+            constexpr float kHi = (float)(8.0 / 7.0), kLo = (float)(8.0 / 7.0 - (double)kHi);
+            const uint32_t bits = __float_as_uint(rstd);
+            if (rstd == rstd) pre = 0.875f * __uint_as_float(bits & 0x7f800000u);
+            const float f = __uint_as_float((bits & 0x007fffffu) | 0x3f800000u);
+            post = f * kHi;
+            post_rest = fmaf(f, kLo, fmaf(f, kHi, -post));
+        }
+    }
+};
+
+// The scale of a block of h whose largest |u| is `top`, and what turns its u into quotients.
+struct NormScale {
+    float scale, back, inv;
+};
+__device__ __forceinline__ NormScale norm_scale(float top, const RowFactors<true> &row) {
+    const float d = top / 448.0f;
+    NormScale r;
+    r.back = remainder_scale(d);
+    r.scale = fmaf(d, row.post, r.back * row.post_rest);
+    r.inv = 1.0f / d;
+    if (r.scale < FLT_MIN) {  // no normal number: 1, and values that are all below half of e4m3's smallest
+        r.scale = 1.0f;
+        r.back = r.inv = 0.0f;
+    }
+    return r;
+}
+
+// Eight values of a block to e4m3.
+__device__ __forceinline__ uint2 quant8(const float (&v)[8], const NormScale &s) {
     uint32_t q[2] = {0, 0};
 #pragma unroll
-    for (int e = 0; e < 4; ++e) q[e >> 1] |= quant2(make_float2(v[2 * e], v[2 * e + 1]), back, inv) << (16 * (e & 1));
+    for (int e = 0; e < 4; ++e) q[e >> 1] |= quant2(make_float2(v[2 * e], v[2 * e + 1]), s.back, s.inv) << (16 * (e & 1));
     return make_uint2(q[0], q[1]);
 }
 
@@ -161,6 +197,7 @@ __global__ void __launch_bounds__(kNormMaxThreads) norm_forward_kernel(const Fwd
     }
     const float rstd = 1.0f / sqrtf(row_reduce<false>(sq, slots[0]) / (float)p.N + p.eps);
     if (p.rstd && live && threadIdx.x == 0) p.rstd[row] = rstd;
+    const RowFactors<E4M3> factors(rstd);
     float top = 0.0f;
 #pragma unroll
     for (int i = 0; i < NV; ++i) {
@@ -168,8 +205,8 @@ __global__ void __launch_bounds__(kNormMaxThreads) norm_forward_kernel(const Fwd
         load_w8<VEC>(p.W, p.w_f32, (i * blockDim.x + threadIdx.x) * 8, p.N, w);
 #pragma unroll
         for (int e = 0; e < 8; ++e) {
-            v[i][e] = v[i][e] * rstd * w[e];
-            // past the row's end there is 0 * rstd, which may be NaN: not part of any maximum
+            v[i][e] = v[i][e] * factors.pre * w[e];
+            // past the row's end there is 0 * pre, which may be NaN: not part of any maximum
             if (E4M3 && p.row_scale && (i * blockDim.x + threadIdx.x) * 8 + e < n) top = max_nan(top, fabsf(v[i][e]));
         }
     }
@@ -178,10 +215,10 @@ __global__ void __launch_bounds__(kNormMaxThreads) norm_forward_kernel(const Fwd
         for (int i = 0; i < NV; ++i)
             store8<VEC>(static_cast<__nv_bfloat16 *>(p.Y) + (live ? row * p.ldy : 0), (i * blockDim.x + threadIdx.x) * 8, n, v[i]);
     } else {
-        float scale = 1.0f;
+        NormScale scale;
         if (p.row_scale) {
-            scale = block_scale_of(row_reduce<true>(top, slots[1]));
-            if (live && threadIdx.x == 0) p.scales[row * p.ldscales] = scale;
+            scale = norm_scale(row_reduce<true>(top, slots[1]), factors);
+            if (live && threadIdx.x == 0) p.scales[row * p.ldscales] = scale.scale;
         }
         uint8_t *y = static_cast<uint8_t *>(p.Y) + (live ? row * p.ldy : 0);
 #pragma unroll
@@ -194,11 +231,10 @@ __global__ void __launch_bounds__(kNormMaxThreads) norm_forward_kernel(const Fwd
                     if (col + e < n) m = max_nan(m, fabsf(v[i][e]));
 #pragma unroll
                 for (int o = 8; o > 0; o >>= 1) m = max_nan(m, __shfl_xor_sync(0xffffffffu, m, o));
-                scale = block_scale_of(m);
-                if (col < n && (threadIdx.x & 15) == 0) p.scales[row * p.ldscales + col / 128] = scale;
+                scale = norm_scale(m, factors);
+                if (col < n && (threadIdx.x & 15) == 0) p.scales[row * p.ldscales + col / 128] = scale.scale;
             }
-            const float inv = 1.0f / scale;
-            const uint2 q2 = quant8(v[i], scale, inv);
+            const uint2 q2 = quant8(v[i], scale);
             const uint32_t q[2] = {q2.x, q2.y};
             if constexpr (VEC) {
                 if (col < n) *reinterpret_cast<uint2 *>(y + col) = q2;
@@ -387,6 +423,7 @@ __global__ void __launch_bounds__(kRingMaxThreads) norm_forward_ring_kernel(cons
         const float sum = block_sum(slots[turn]);
         const float rstd = 1.0f / sqrtf(sum / (float)n + p.eps);
         if (p.rstd && threadIdx.x == 0) p.rstd[row] = rstd;
+        const RowFactors<E4M3> factors(rstd);
         if (p.S) {
 #pragma unroll
             for (int i = 0; i < kRingNv; ++i) store8<true>(p.S + row * p.lds, (i * blockDim.x + threadIdx.x) * 8, n, v[i]);
@@ -395,7 +432,7 @@ __global__ void __launch_bounds__(kRingMaxThreads) norm_forward_ring_kernel(cons
         for (int i = 0; i < kRingNv; ++i) {
             const int col = (i * blockDim.x + threadIdx.x) * 8;
 #pragma unroll
-            for (int e = 0; e < 8; ++e) v[i][e] = v[i][e] * rstd * w[i][e];
+            for (int e = 0; e < 8; ++e) v[i][e] = v[i][e] * factors.pre * w[i][e];
             if constexpr (!E4M3) {
                 store8<true>(static_cast<__nv_bfloat16 *>(p.Y) + row * p.ldy, col, n, v[i]);
             } else {
@@ -406,11 +443,10 @@ __global__ void __launch_bounds__(kRingMaxThreads) norm_forward_ring_kernel(cons
                 }
 #pragma unroll
                 for (int o = 8; o > 0; o >>= 1) m = max_nan(m, __shfl_xor_sync(0xffffffffu, m, o));
-                const float scale = block_scale_of(m);
-                const float inv = 1.0f / scale;
+                const NormScale scale = norm_scale(m, factors);
                 if (col < n) {
-                    if ((threadIdx.x & 15) == 0) p.scales[row * p.ldscales + col / 128] = scale;
-                    *reinterpret_cast<uint2 *>(static_cast<uint8_t *>(p.Y) + row * p.ldy + col) = quant8(v[i], scale, inv);
+                    if ((threadIdx.x & 15) == 0) p.scales[row * p.ldscales + col / 128] = scale.scale;
+                    *reinterpret_cast<uint2 *>(static_cast<uint8_t *>(p.Y) + row * p.ldy + col) = quant8(v[i], scale);
                 }
             }
         }
@@ -518,6 +554,7 @@ __global__ void __launch_bounds__(kRingMaxThreads) norm_forward_odd_kernel(const
         }
         const float rstd = 1.0f / sqrtf(block_sum(slots[turn]) / (float)n + p.eps);
         if (p.rstd && threadIdx.x == 0) p.rstd[row] = rstd;
+        const RowFactors<E4M3> factors(rstd);
 #pragma unroll
         for (int i = 0; i < kRingNv; ++i) {
             const int col = (i * blockDim.x + threadIdx.x) * 8;
@@ -526,7 +563,7 @@ __global__ void __launch_bounds__(kRingMaxThreads) norm_forward_odd_kernel(const
             float m = 0.0f;
 #pragma unroll
             for (int e = 0; e < 8; ++e) {
-                v[i][e] = v[i][e] * rstd * w[i][e];
+                v[i][e] = v[i][e] * factors.pre * w[i][e];
                 if (E4M3 && col + e < n) m = max_nan(m, fabsf(v[i][e]));
             }
             if constexpr (!E4M3) {
@@ -534,11 +571,10 @@ __global__ void __launch_bounds__(kRingMaxThreads) norm_forward_odd_kernel(const
             } else {
 #pragma unroll
                 for (int o = 8; o > 0; o >>= 1) m = max_nan(m, __shfl_xor_sync(0xffffffffu, m, o));
-                const float scale = block_scale_of(m);
-                const float inv = 1.0f / scale;
+                const NormScale scale = norm_scale(m, factors);
                 if (col < n) {
-                    if ((threadIdx.x & 15) == 0) p.scales[row * p.ldscales + col / 128] = scale;
-                    *reinterpret_cast<uint2 *>(y_out + col) = quant8(v[i], scale, inv);
+                    if ((threadIdx.x & 15) == 0) p.scales[row * p.ldscales + col / 128] = scale.scale;
+                    *reinterpret_cast<uint2 *>(y_out + col) = quant8(v[i], scale);
                 }
             }
         }
