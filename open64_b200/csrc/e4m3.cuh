@@ -20,12 +20,11 @@ __device__ __forceinline__ float block_scale_of(float amax) {
     return s < FLT_MIN ? 1.0f : s;
 }
 
-// h / scale with inv = 1 / scale. One division per block: the product with inv is off by up to 1.5 ulp, which puts some
-// values on the other side of a rounding to four bits, so a step with the product's own remainder follows,
-// q - (q scale - h) inv, in two multiply-adds. RMS norm of 16384 x 8192: 1060 of 134 million values are other than from 64
-// bits, 1176 without the step, as many as with it from a division per value, which takes 194 us instead of 157. (With
-// q scale - h and not h - q scale a zero keeps its sign.) `back` is remainder_scale(scale): under an infinite scale inv is 0
-// and nothing is to be put right, the remainder would be 0 * inf.
+// h / scale with inv = 1 / scale. One division per block (one per value took RMS norm of 16384 x 8192 from 157 to 194 us): the
+// product with inv is off by up to 1.5 ulp, which puts some values on the other side of a rounding to four bits, so a
+// step with the product's own remainder follows, q - (q scale - h) inv, in two multiply-adds; q is then the quotient rounded
+// once. (With q scale - h and not h - q scale a zero keeps its sign.) `back` is remainder_scale(scale): under an infinite
+// scale inv is 0 and nothing is to be put right, the remainder would be 0 * inf.
 __device__ __forceinline__ float remainder_scale(float scale) { return scale <= FLT_MAX ? scale : 0.0f; }
 __device__ __forceinline__ float quotient(float h, float back, float inv) {
     const float q = h * inv;

@@ -161,8 +161,12 @@ struct FwdParams {
     void *Y;
     float *scales, *rstd;
     float eps;
+    double inv_n;  // 1 / N
     int w_f32, row_scale;
 };
+
+// 1 / sqrt(mean of squares + eps) of a row's sum of squares, rounded once.
+__device__ __forceinline__ float rstd_of(float sum, const FwdParams &p) { return (float)rsqrt(fma((double)sum, p.inv_n, (double)p.eps)); }
 
 // Columns of thread t: (i * blockDim.x + t) * 8 .. + 7 for i < NV, so that 16 neighbouring threads hold
 // one scale block of 128.
@@ -195,7 +199,7 @@ __global__ void __launch_bounds__(kNormMaxThreads) norm_forward_kernel(const Fwd
 #pragma unroll
         for (int i = 0; i < NV; ++i) store8<VEC>(p.S + (live ? row * p.lds : 0), (i * blockDim.x + threadIdx.x) * 8, n, v[i]);
     }
-    const float rstd = 1.0f / sqrtf(row_reduce<false>(sq, slots[0]) / (float)p.N + p.eps);
+    const float rstd = rstd_of(row_reduce<false>(sq, slots[0]), p);
     if (p.rstd && live && threadIdx.x == 0) p.rstd[row] = rstd;
     const RowFactors<E4M3> factors(rstd);
     float top = 0.0f;
@@ -421,7 +425,7 @@ __global__ void __launch_bounds__(kRingMaxThreads) norm_forward_ring_kernel(cons
             load(row + (long long)stages * gridDim.x, stage);
         }
         const float sum = block_sum(slots[turn]);
-        const float rstd = 1.0f / sqrtf(sum / (float)n + p.eps);
+        const float rstd = rstd_of(sum, p);
         if (p.rstd && threadIdx.x == 0) p.rstd[row] = rstd;
         const RowFactors<E4M3> factors(rstd);
         if (p.S) {
@@ -552,7 +556,7 @@ __global__ void __launch_bounds__(kRingMaxThreads) norm_forward_odd_kernel(const
             fence_proxy_async_smem();
             load(row + (long long)stages * gridDim.x, stage);
         }
-        const float rstd = 1.0f / sqrtf(block_sum(slots[turn]) / (float)n + p.eps);
+        const float rstd = rstd_of(block_sum(slots[turn]), p);
         if (p.rstd && threadIdx.x == 0) p.rstd[row] = rstd;
         const RowFactors<E4M3> factors(rstd);
 #pragma unroll
@@ -957,7 +961,7 @@ int norm_forward(const NormCall &c, int num_sms) {
     p.X = static_cast<const __nv_bfloat16 *>(c.X), p.ldx = c.ldx;
     p.R = static_cast<const __nv_bfloat16 *>(c.R), p.ldr = c.ldr;
     p.S = static_cast<__nv_bfloat16 *>(c.S), p.lds = c.lds;
-    p.W = c.W, p.w_f32 = c.w_f32, p.eps = c.eps;
+    p.W = c.W, p.w_f32 = c.w_f32, p.eps = c.eps, p.inv_n = 1.0 / (double)c.N;
     p.Y = c.Y, p.ldy = c.ldy, p.scales = c.scales, p.ldscales = c.ldscales, p.rstd = c.rstd, p.row_scale = c.row_scale;
     RingShape r;
     if (vec && !(e4m3 && c.row_scale) && c.N >= kRingCols && ring_shape(c.N, c.R ? 2 : 1, 0, &r) && c.T >= (int64_t)2 * r.blocks_per_sm * num_sms) {
