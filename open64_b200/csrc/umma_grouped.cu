@@ -561,6 +561,7 @@ grouped_pair_kernel(const __grid_constant__ CUtensorMap tm_a, const __grid_const
                     ok = mbar_wait_bounded(acc_full_bar(uses & 1), (uint32_t)((uses >> 1) & 1), abort_flag, p.status,
                                            kWaitGroupAccFull, p.wait_ns);
                 ok = __shfl_sync(0xffffffffu, ok, 0);
+                __syncwarp();  // (orders memory, which the shuffle does not: the other lanes read what lane 0 has waited for)
                 if (!ok) break;
                 tc_fence_after();
                 const uint32_t t_row = t_lane + (uint32_t)(uses & 1) * kGpTileN;
@@ -640,6 +641,7 @@ grouped_pair_kernel(const __grid_constant__ CUtensorMap tm_a, const __grid_const
                         ok = mbar_wait_bounded(half_bar(quarter), half_phase, abort_flag, p.status, kWaitGroupHalf, p.wait_ns);
                     }
                     ok = __shfl_sync(0xffffffffu, ok, 0);
+                    __syncwarp();  // (orders memory, which the shuffle does not: the other lanes read what lane 0 has waited for)
                     half_phase ^= 1u;
                 };
                 float amax = 0.0f;

@@ -534,6 +534,7 @@ grouped_rows_kernel(const __grid_constant__ CUtensorMap tm_x, const __grid_const
                     if (lane == 0)
                         ok = mbar_wait_bounded(up_empty_bar(quarter), (tiles & 1) ^ 1u, abort_flag, p.status, kWaitGroupHalf, p.wait_ns);
                     ok = __shfl_sync(0xffffffffu, ok, 0);
+                    __syncwarp();  // (orders memory, which the shuffle does not: the other lanes read what lane 0 has waited for)
                     if (!ok) break;
 #pragma unroll
                     for (int j = 0; j < TOK; ++j) xch[j * 128 + n_in] = (j & 1) ? acc[j / 2].y : acc[j / 2].x;
@@ -543,6 +544,7 @@ grouped_rows_kernel(const __grid_constant__ CUtensorMap tm_x, const __grid_const
                     if (lane == 0)
                         ok = mbar_wait_bounded(up_full_bar(quarter), tiles & 1, abort_flag, p.status, kWaitGroupHalf, p.wait_ns);
                     ok = __shfl_sync(0xffffffffu, ok, 0);
+                    __syncwarp();  // (orders memory, which the shuffle does not: the other lanes read what lane 0 has waited for)
                     if (!ok) break;
 #pragma unroll
                     for (int j = 0; j < TOK / 2; ++j) {
@@ -571,6 +573,7 @@ grouped_rows_kernel(const __grid_constant__ CUtensorMap tm_x, const __grid_const
                             ok = mbar_wait_bounded(amax_bar, tiles & 1, abort_flag, p.status, kWaitGroupHalf, p.wait_ns);
                         }
                         ok = __shfl_sync(0xffffffffu, ok, 0);
+                        __syncwarp();  // (orders memory, which the shuffle does not: the other lanes read what lane 0 has waited for)
                         if (!ok) break;
                         float h[TOK];
 #pragma unroll
