@@ -227,7 +227,7 @@ int o64_gemm_s8_scaled(o64_handle_t h, int64_t M, int64_t N, int64_t K, const in
  * (O64_ERR_RANK for host memory or another GPU's), allocate nothing, use no scratch of the handle and
  * may be captured into a CUDA graph; two calls on different streams of one handle do not touch each
  * other's memory.  Operands whose base or pitch is not a multiple of 16 bytes are O64_ERR_ALIGN where
- * a product says so. */
+ * a product says so, and so is any pointer that is no multiple of its elements' size. */
 
 /* RMS norm with the residual's addition, rows of N columns (1 <= N <= 32768):
  *   s = x + r      h[j] = s[j] / sqrt(mean(s^2) + eps) * w[j]

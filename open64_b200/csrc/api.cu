@@ -807,6 +807,13 @@ static bool device_operands(o64_handle_t h, std::initializer_list<const void *> 
     return true;
 }
 
+// Elements lie on multiples of their size (a kernel's access to one that does not is a fault).
+static bool on_elements(int elem, std::initializer_list<const void *> ptrs) {
+    for (const void *p : ptrs)
+        if (reinterpret_cast<uintptr_t>(p) % elem) return false;
+    return true;
+}
+
 extern "C" int o64_rmsnorm_bf16(o64_handle_t h, int64_t T, int64_t N, const void *X, int64_t ldx, const void *R, int64_t ldr,
                                 void *S, int64_t lds, const void *W, int w_f32, float eps, int out_kind, int scale_block, void *Y,
                                 int64_t ldy, float *scales, int64_t ldscales, float *rstd, void *stream) {
@@ -820,6 +827,8 @@ extern "C" int o64_rmsnorm_bf16(o64_handle_t h, int64_t T, int64_t N, const void
     if (ldx < N || ldy < N || (R && ldr < N) || (S && lds < N)) return O64_ERR_CONFORM;
     if (e4m3 && ldscales < (scale_block ? (N + 127) / 128 : 1)) return O64_ERR_CONFORM;
     if (!device_operands(h, {X, R, S, W, Y, scales, rstd})) return O64_ERR_RANK;
+    if (!on_elements(2, {X, R, S}) || !on_elements(w_f32 ? 4 : 2, {W}) || !on_elements(e4m3 ? 1 : 2, {Y}) || !on_elements(4, {scales, rstd}))
+        return O64_ERR_ALIGN;
     DeviceGuard g(h->device);
     NormCall c;
     c.T = T, c.N = N, c.X = X, c.ldx = ldx, c.R = R, c.ldr = ldr, c.S = S, c.lds = lds, c.W = W, c.w_f32 = w_f32 != 0;
@@ -843,12 +852,14 @@ extern "C" int o64_rmsnorm_bf16_backward(o64_handle_t h, int64_t T, int64_t N, c
     if (T == 0) {  // the sum over no rows
         if (!dW) return O64_OK;
         if (!device_operands(h, {dW})) return O64_ERR_RANK;
+        if (!on_elements(4, {dW})) return O64_ERR_ALIGN;
         CUDA_TRY(cudaMemsetAsync(dW, 0, (size_t)N * 4, s));
         return O64_OK;
     }
     if (!dY || !S || !W || !rstd || !dX || (dW && !workspace)) return O64_ERR_RANK;
     if (lddy < N || lds < N || lddx < N || (dR && lddr < N)) return O64_ERR_CONFORM;
     if (!device_operands(h, {dY, S, W, rstd, dR, dX, dW, workspace})) return O64_ERR_RANK;
+    if (!on_elements(2, {dY, S, dR, dX}) || !on_elements(w_f32 ? 4 : 2, {W}) || !on_elements(4, {rstd, dW, workspace})) return O64_ERR_ALIGN;
     NormBackwardCall c;
     c.T = T, c.N = N, c.dY = dY, c.lddy = lddy, c.S = S, c.lds = lds, c.W = W, c.w_f32 = w_f32 != 0, c.rstd = rstd;
     c.dR = dR, c.lddr = lddr, c.dX = dX, c.lddx = lddx, c.dW = dW, c.workspace = static_cast<float *>(workspace), c.stream = s;
@@ -870,6 +881,7 @@ static int grouped_entry(o64_handle_t h, GroupedCall c, void *stream) {
     if (c.ldc < c_cols || (c.wgrad && c.G > 1 && c.stride_c < (c_rows - 1) * c.ldc + c_cols)) return O64_ERR_CONFORM;
     if (c.epi == GEPI_SWIGLU_E4M3 && c.ldsc < c.N / 128) return O64_ERR_CONFORM;
     if (!device_operands(h, {c.A, c.B, c.C, c.scale_a, c.scale_b, c.scale_c, c.offsets})) return O64_ERR_RANK;
+    if (!on_elements(gepi_bytes(c.epi), {c.C}) || !on_elements(4, {c.scale_a, c.scale_b, c.scale_c, c.offsets})) return O64_ERR_ALIGN;
     DeviceGuard g(h->device);
     c.status_word = h->status_word;
     c.num_sms = h->num_sms;
