@@ -69,14 +69,17 @@ struct GroupedParams {
 
 // A group's rows, kept inside [top, T) whatever the offsets say; *bad: they are not ascending within 0 .. T.  A walk
 // over the groups passes the end of those before: offsets that overlap then make no more tiles than others, which is
-// what the grids and the one tile of a cluster that divides K are sized for.
+// what the grids and the one tile of a cluster that divides K are sized for.  WRITTEN: the kernel may exist while the one
+// before it still writes the offsets (see umma_grouped_rows.cu); else they come by the read-only path, which the compiler
+// moves freely.
+template <bool WRITTEN>
 __device__ __forceinline__ void group_rows(const GroupedParams &p, int g, int top, int &begin, int &end, bool *bad = nullptr) {
     if (!p.offsets) {
         begin = 0;
         end = p.T;
         return;
     }
-    const int a = p.offsets[g], b = p.offsets[g + 1];
+    const int a = WRITTEN ? p.offsets[g] : __ldg(p.offsets + g), b = WRITTEN ? p.offsets[g + 1] : __ldg(p.offsets + g + 1);
     begin = min(max(a, top), p.T);
     end = min(max(b, begin), p.T);
     if (bad) *bad = a < 0 || b < a || b > p.T;

@@ -81,7 +81,7 @@ struct TileWalk {
 template <bool WGRAD>
 __device__ __forceinline__ bool next_tile(const GroupedParams &p, TileWalk &w, int t, int block_k, GroupTile &tile) {
     for (; w.g < p.G; ++w.g) {
-        group_rows(p, w.g, w.top, tile.begin, tile.end);
+        group_rows<false>(p, w.g, w.top, tile.begin, tile.end);
         const int rows = tile.end - tile.begin;
         const int mt = WGRAD ? p.num_m_tiles : (rows + kGpTileM - 1) / kGpTileM;
         const int tiles = mt * p.num_n_tiles;  // (the host has checked that all of them together fit an int)
@@ -212,7 +212,7 @@ grouped_pair_kernel(const __grid_constant__ CUtensorMap tm_a, const __grid_const
         for (int g = lane; g < p.G; g += 32) {
             int b, e;
             bool bad;
-            group_rows(p, g, 0, b, e, &bad);
+            group_rows<false>(p, g, 0, b, e, &bad);
             if (bad) atomicCAS(p.status, 0, kBadOffsets);
         }
     }
@@ -723,7 +723,7 @@ grouped_pair_kernel(const __grid_constant__ CUtensorMap tm_a, const __grid_const
 __global__ void grouped_zero_kernel(const GroupedParams p, int elem, int wgrad) {
     for (int g = blockIdx.y; g < p.G; g += gridDim.y) {
         int b = 0, e = p.rows_m;
-        if (!wgrad) group_rows(p, g, 0, b, e);
+        if (!wgrad) group_rows<false>(p, g, 0, b, e);
         uint8_t *c = static_cast<uint8_t *>(p.C) + (wgrad ? (long long)g * p.stride_c * elem : 0);
         for (long long r = b + blockIdx.x; r < e; r += gridDim.x) {
             for (long long i = threadIdx.x; i < (long long)p.N * elem; i += blockDim.x) c[r * p.ldc * elem + i] = 0;

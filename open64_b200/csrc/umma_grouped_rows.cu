@@ -73,7 +73,7 @@ template <int TOK>
 __device__ __forceinline__ bool next_rows_tile(const GroupedParams &p, RowsWalk &w, int t, RowsTile &tile) {
     for (; w.g < p.G; ++w.g) {
         int begin, end;
-        group_rows(p, w.g, w.top, begin, end);
+        group_rows<true>(p, w.g, w.top, begin, end);
         const int tt = (end - begin + TOK - 1) / TOK;
         const int tiles = tt * p.num_n_tiles;
         if (t < w.base + tiles) {
@@ -206,7 +206,7 @@ grouped_rows_kernel(const __grid_constant__ CUtensorMap tm_x, const __grid_const
         for (int g = lane; g < p.G; g += 32) {
             int b, e;
             bool bad;
-            group_rows(p, g, 0, b, e, &bad);
+            group_rows<true>(p, g, 0, b, e, &bad);
             if (bad) atomicCAS(p.status, 0, kBadOffsets);
         }
     }
