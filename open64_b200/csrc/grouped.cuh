@@ -125,17 +125,22 @@ __device__ __forceinline__ float rcp_approx(float x) {  // 1 ulp; below 2^-126 z
     return r;
 }
 
-// silu(g) * u = g / (1 + exp(-g)) * u, within 2^-20 of the value.  exp(x) = 2^hi * (1 + lo ln 2) with x log2(e) = hi + lo in two
-// floats: in one, its rounding alone is 2^-20 of the result at g = -20 and four times that at -80.  The power is within
-// 2^-22, the reciprocal 2^-23, five roundings 2^-24 each.  x stays between -87, where exp(x) is nothing beside 1, and 88, where
-// the reciprocal is zero (g -> -inf: the result is below 1e-35 of u), so that neither hi nor 2^hi is infinite.
-__device__ __forceinline__ float silu_mul(float g, float u) {
+// silu(g) * u = g / (1 + exp(-g)) * u, within 2^-20 of the value.  With x = -g (between -104 and 104) and x log2(e) = hi + lo in two
+// floats, exp(x) = 2^hi (1 + lo ln 2): in one float, its rounding alone is 2^-20 of the result at g = -20 and four times that at
+// -80.  The correction goes to the quotient r = 1 / (1 + 2^hi), where it is -r (1 - r) lo ln 2 and 2^hi may be infinite: r is
+// zero then and the result, below 1e-35 of u, too.  The power is within 2^-22, the reciprocal 2^-23, six roundings 2^-24 each.
+// Two values at a time, by packed arithmetic (8 experts' 2 x 14336 x 4096: 1142 us, 1143 with the fast exp alone).
+__device__ __forceinline__ float2 silu_mul2(float2 g, float2 u) {
     constexpr float kLog2e = 1.44269502f, kLog2eRest = 1.92596299e-8f, kLn2 = 0.693147181f;
-    const float x = fminf(fmaxf(-g, -87.0f), 88.0f);
-    const float hi = x * kLog2e;
-    const float lo = fmaf(x, kLog2eRest, fmaf(x, kLog2e, -hi));
-    const float p = ex2_approx(hi);
-    return g * rcp_approx(1.0f + fmaf(p, lo * kLn2, p)) * u;
+    const float2 x = make_float2(fminf(fmaxf(-g.x, -104.0f), 104.0f), fminf(fmaxf(-g.y, -104.0f), 104.0f));
+    const float2 hi = __fmul2_rn(x, make_float2(kLog2e, kLog2e));
+    float2 lo = __ffma2_rn(x, make_float2(kLog2e, kLog2e), make_float2(-hi.x, -hi.y));
+    lo = __ffma2_rn(x, make_float2(kLog2eRest, kLog2eRest), lo);
+    const float2 d = __fadd2_rn(make_float2(ex2_approx(hi.x), ex2_approx(hi.y)), make_float2(1.0f, 1.0f));
+    float2 r = make_float2(rcp_approx(d.x), rcp_approx(d.y));
+    const float2 rest = __fmul2_rn(__ffma2_rn(r, r, make_float2(-r.x, -r.y)), make_float2(kLn2, kLn2));  // -r (1 - r) ln 2
+    r = __ffma2_rn(rest, lo, r);
+    return __fmul2_rn(__fmul2_rn(g, r), u);
 }
 
 }  // namespace o64

@@ -648,8 +648,7 @@ grouped_pair_kernel(const __grid_constant__ CUtensorMap tm_a, const __grid_const
 #pragma unroll
                 for (int j = 0; j < 32; ++j) {
                     float2 &h = acc[0][j];
-                    h.x = silu_mul(h.x, acc[1][j].x);
-                    h.y = silu_mul(h.y, acc[1][j].y);
+                    h = silu_mul2(h, acc[1][j]);
                     amax = max_nan(amax, max_nan(fabsf(h.x), fabsf(h.y)));
                 }
                 // the row's other 64 columns are with the warp of the other half
@@ -688,7 +687,7 @@ grouped_pair_kernel(const __grid_constant__ CUtensorMap tm_a, const __grid_const
                 if constexpr (EPI == GEPI_SWIGLU_BF16) {
 #pragma unroll
                     for (int j = 0; j < 32; ++j)
-                        acc[0][j] = make_float2(silu_mul(acc[0][j].x, acc[1][j].x), silu_mul(acc[0][j].y, acc[1][j].y));
+                        acc[0][j] = silu_mul2(acc[0][j], acc[1][j]);
                 }
 #pragma unroll
                 for (int s = 0; s < (kSwiglu ? 1 : 2); ++s) {

@@ -547,10 +547,7 @@ grouped_rows_kernel(const __grid_constant__ CUtensorMap tm_x, const __grid_const
                     __syncwarp();  // (orders memory, which the shuffle does not: the other lanes read what lane 0 has waited for)
                     if (!ok) break;
 #pragma unroll
-                    for (int j = 0; j < TOK / 2; ++j) {
-                        acc[j].x = silu_mul(acc[j].x, xch[(2 * j) * 128 + n_in]);
-                        acc[j].y = silu_mul(acc[j].y, xch[(2 * j + 1) * 128 + n_in]);
-                    }
+                    for (int j = 0; j < TOK / 2; ++j) acc[j] = silu_mul2(acc[j], make_float2(xch[(2 * j) * 128 + n_in], xch[(2 * j + 1) * 128 + n_in]));
                     __syncwarp();
                     if (lane == 0) mbar_arrive(up_empty_bar(quarter));
                     if constexpr (EPI == GEPI_SWIGLU_BF16) {
@@ -637,7 +634,8 @@ grouped_rows_kernel(const __grid_constant__ CUtensorMap tm_x, const __grid_const
             float4 x = total4(c, 0);
             if constexpr (kSwiglu) {
                 const float4 u = total4(c, 1);
-                x = make_float4(silu_mul(x.x, u.x), silu_mul(x.y, u.y), silu_mul(x.z, u.z), silu_mul(x.w, u.w));
+                const float2 a = silu_mul2(make_float2(x.x, x.y), make_float2(u.x, u.y)), b = silu_mul2(make_float2(x.z, x.w), make_float2(u.z, u.w));
+                x = make_float4(a.x, a.y, b.x, b.y);
             }
             h[4 * c] = x.x, h[4 * c + 1] = x.y, h[4 * c + 2] = x.z, h[4 * c + 3] = x.w;
         }
