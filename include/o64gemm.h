@@ -238,7 +238,8 @@ int o64_gemm_s8_scaled(o64_handle_t h, int64_t M, int64_t N, int64_t K, const in
  * where scale_block = 128 makes blocks of 128 columns, scales [T][ceil(N/128)] with ldscales floats
  * between rows (what the block-scaled products read), and scale_block = 0 one block per row, scales[T]
  * at a distance of ldscales (scaleA of o64_gemm_fp8_scaled with ldscales = 1).  A NaN makes its block's
- * scale NaN.  rstd (may be NULL): 1 / sqrt(mean(s^2) + eps) for each row, for the backward pass. */
+ * scale NaN.  rstd (may be NULL): 1 / sqrt(mean(s^2) + eps) for each row, for the backward pass; the sum of squares is
+ * fp32, so that a row where it passes 3.4e38 has 0 here and in h, as one with an infinite value has. */
 int o64_rmsnorm_bf16(o64_handle_t h, int64_t T, int64_t N, const void *X, int64_t ldx, const void *R, int64_t ldr,
                      void *S, int64_t lds, const void *W, int w_f32, float eps, int out_kind, int scale_block, void *Y,
                      int64_t ldy, float *scales, int64_t ldscales, float *rstd, void *stream);
@@ -276,8 +277,8 @@ int o64_gemm_fp8_block_swiglu(o64_handle_t h, int64_t M, int64_t N, int64_t K, c
  * ascending within 0 .. T) bound them: group g has rows offsets[g] .. offsets[g+1]-1, possibly none.
  * Group g multiplies B + g * stride_b ([N,K], or [K,N] with transB == 0).  Rows of C before offsets[0]
  * and from offsets[G] on are left as they are.  Offsets that are not ascending within 0 .. T are never
- * followed out of the operands; the rows concerned are undefined and o64_last_status reports
- * O64_ERR_CONFORM.  Scales of the e4m3 forms as above, stride_sb floats between the groups' scales of B.
+ * followed out of the operands and make no more work than others; the rows concerned are undefined and
+ * o64_last_status reports O64_ERR_CONFORM.  Scales of the e4m3 forms as above, stride_sb floats between the groups' scales of B.
  * Bases, pitches and strides of A and B: multiples of 16 bytes. */
 int o64_gemm_grouped_bf16(o64_handle_t h, int64_t G, int64_t T, int64_t N, int64_t K, const void *A, int64_t lda,
                           const int32_t *offsets, const void *B, int64_t ldb, int64_t stride_b, int transB, void *C, int64_t ldc,

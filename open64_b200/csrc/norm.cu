@@ -9,8 +9,8 @@
 // norm is taken of the sum in fp32; the stream s that goes on to the next layer is that sum rounded
 // to bf16 once.
 //
-// Bound by HBM: 16384 x 8192 with the residual to e4m3 157 us = 6.0 TB/s (0.92 of a copy), backward 8192 x 8192 with the
-// residual 94 us = 5.7 TB/s.  Many rows run on a few blocks per SM that stay: rows come in by bulk copies, a ring of
+// Bound by HBM: 16384 x 8192 with the residual to e4m3 153 to 174 us on several B200s = 5.4 to 6.1 TB/s (0.83 to 0.94 of a
+// copy), backward 8192 x 8192 with the residual 94 us = 5.7 TB/s.  Many rows run on a few blocks per SM that stay: rows come in by bulk copies, a ring of
 // three ahead, so that loads go on while a row is reduced, converted and stored, and a thread keeps its
 // columns of w.  Few rows run on a block per row that loads for itself.
 //
@@ -31,7 +31,10 @@ namespace o64 {
 namespace {
 
 constexpr int kNormMaxThreads = 512;
-constexpr int kRingCols = 256;  // narrower rows run on the block-per-row kernel
+// Narrower rows run on the block-per-row kernel.  (A measured choice only above: 65536 x 256 to e4m3 84 us there and 48 on the ring.
+// Below, the ring would take less as well, 65536 x 192 48 us and not 85, backward 40 and not 46, but for unaligned rows backward,
+// 127 columns 61 us and not 52.)
+constexpr int kRingCols = 256;
 
 // Eight consecutive bf16 values of a row; columns >= n read as zero.
 template <bool VEC>
@@ -469,7 +472,7 @@ __global__ void __launch_bounds__(kRingMaxThreads) norm_forward_ring_kernel(cons
 // (an aligned chunk with one byte of an allocation lies inside it), read from shared memory at the row's own offset;
 // results go back through shared memory too, so that a warp's stores are contiguous.  Two bytes at a time straight from
 // and to global memory, 10000 rows of 5003 with the residual took 248 us to e4m3 and 286 us backward;
-// 112 us and 157 us this way.
+// 120 us and 164 us this way.
 struct OddRow {
     const __nv_bfloat16 *row;
     __device__ __forceinline__ uint32_t shift() const { return (uint32_t)(reinterpret_cast<uintptr_t>(row) & 15u); }
@@ -886,11 +889,14 @@ int launch_forward(const FwdParams &p, bool e4m3, dim3 grid, dim3 block, cudaStr
 
 // Blocks that stay on an SM for rows of N columns with `operands` of them on their way, and the depth of their
 // rings: 1024 threads and all shared memory of an SM, at most three rows ahead.  Two vectors a thread: with four, 8191
-// rows of 5000 ran backward in 75 us instead of 70 and 6247 rows of 9984 to e4m3 in 92 us instead of 65.
+// rows of 5000 ran backward in 75 us instead of 70 and 6247 rows of 9984 to e4m3 in 92 us instead of 71.
 struct RingShape {
     int threads, blocks_per_sm, stages;
     size_t smem;
 };
+// The rings are for two rows a resident block and more: 592 rows of 1024 to e4m3 4.3 us on a block per row, 3.7 on the ring, 296
+// rows 2.8 and 3.5; 1184 x 4096 9.6 and 7.5, 296 x 4096 3.7 and 4.2.  (Backward the ring is ahead from one row a block on: 592 x 4096
+// 15.4 and 10.7, 1184 x 4096 19.2 and 12.9.)
 bool ring_shape(int64_t N, int operands, int extra_bytes_per_col, RingShape *r, bool odd = false) {
     r->threads = threads_for(N, kRingNv);
     if (r->threads > kRingMaxThreads) return false;

@@ -1,7 +1,7 @@
 // Products grouped by expert, and the block-scaled e4m3 product, for few rows: every weight is read once
 // for a handful of rows of A, so the weights' way from HBM is all that counts.
 //
-// The operands change places: 128 rows of a weight are the MMA's M and the rows of A its N (16, 32 or 64),
+// The operands change places: 128 rows of a weight are the MMA's M and the rows of A its N (16, 32, 64 or 128),
 // so that nothing is spent on rows that are not there - shared memory, TMEM reads and sums go by 16 rows, not
 // by 128 - and the ring holds nearly 200 KB of weights on their way per SM.  A thread then owns one column
 // of C (one weight row) and all rows of the tile.  With the SwiGLU tail a tile is 128 gate and the 128

@@ -491,7 +491,8 @@ class Engine:
 
     def gemm_grouped_bf16(self, A, offsets, B, transB=True, out=None):
         """A[rows of g] @ op(B[g]) for each group g: A [T,K] bf16 sorted by group, offsets int32 [G+1] on the
-        device, B [G,N,K] (or [G,K,N]: transB False).  Rows outside offsets[0] .. offsets[G] are left as they are."""
+        device, B [G,N,K] (or [G,K,N]: transB False).  Rows outside offsets[0] .. offsets[G] are left as they are (in a new
+        result, one without `out`: undefined)."""
         T, K = _matrix(A, "A", _BF16).shape
         if len(B.shape) != 3 or B.dtype is not _BF16 or B.shape[2 if transB else 1] != K:
             _want(B, "B", (_BF16,), (None, None, K) if transB else (None, K, None))
@@ -528,7 +529,8 @@ class Engine:
         return out
 
     def gemm_grouped_fp8_block(self, A8, scaleA, offsets, B8, scaleB, transB=True, out=None):
-        """gemm_fp8_block by group: A8 [T,K] sorted by group, B8 [G,N,K] (or [G,K,N]), scaleB one per 128 x 128."""
+        """gemm_fp8_block by group: A8 [T,K] sorted by group, B8 [G,N,K] (or [G,K,N]), scaleB one per 128 x 128.  Rows outside the
+        groups as in gemm_grouped_bf16."""
         if B8.dim() != 3:
             raise O64Error(_lib.ERR_RANK, f"B8: rank {B8.dim()}")
         T, N, K, A8, scaleA, B8, scaleB = self._block_operands(A8, scaleA, B8, scaleB, transB, False, B8.shape[0])
@@ -541,7 +543,7 @@ class Engine:
         return out
 
     def gemm_grouped_fp8_block_swiglu(self, A8, scaleA, offsets, B8, scaleB, out_kind=_lib.OUT_E4M3, out=None, scales=None):
-        """gemm_fp8_block_swiglu by group: B8 [G,2N,K]."""
+        """gemm_fp8_block_swiglu by group: B8 [G,2N,K].  Rows outside the groups as in gemm_grouped_bf16."""
         if B8.dim() != 3:
             raise O64Error(_lib.ERR_RANK, f"B8: rank {B8.dim()}")
         T, N, K, A8, scaleA, B8, scaleB = self._block_operands(A8, scaleA, B8, scaleB, True, True, B8.shape[0])
@@ -558,7 +560,8 @@ class Engine:
     def mlp_swiglu_fp8(self, x, norm_weight, W13, scale13, W2, scale2, residual=None, offsets=None, eps=1e-6):
         """The 8-bit feed-forward block: norm(x + residual) in e4m3, silu(gate) * up in e4m3, down projection.
         W13 [2F,D] and W2 [D,F] e4m3 with a scale per 128 x 128 - or [G,2F,D] and [G,D,F] with `offsets`,
-        rows of x sorted by expert.  Returns (out bf16, the stream after the addition)."""
+        rows of x (and of the results) sorted by expert: a router that reads the normed rows calls rms_norm itself, sorts
+        its result and its scales, and goes on with the two products.  Returns (out bf16, the stream after the addition)."""
         a, sa, stream, _ = self.rms_norm(x, norm_weight, residual, eps, _lib.OUT_E4M3)
         if offsets is None:
             h, sh = self.gemm_fp8_block_swiglu(a, sa, W13, scale13)
